@@ -22,7 +22,7 @@ QMRI_ERR_HIP = -3
 QMRI_ERR_NONFINITE = -4
 QMRI_ERR_NOMEM = -5
 
-QMRI_F32, QMRI_F64, QMRI_I16, QMRI_U16 = 0, 1, 2, 3
+QMRI_F32, QMRI_F64, QMRI_I16, QMRI_U16, QMRI_F16, QMRI_BF16 = 0, 1, 2, 3, 4, 5
 INIT_SCALAR, INIT_PER_VOXEL, INIT_LOGLIN = 0, 1, 2
 MAX_ECHOES = 32
 # samples per voxel the general lmdif kernel keeps (include/qmri.h: E <= QMRI_LM_MAX_ECHOES and (n + 3) * E <= 320)
@@ -147,6 +147,42 @@ class QmriLmfitArgs(ctypes.Structure):
     ]
 
 
+class QmriLogits(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("background", ctypes.c_int32),
+        ("rows", ctypes.c_int64), ("inner", ctypes.c_int64), ("stride_outer", ctypes.c_int64),
+        ("stride_inner", ctypes.c_int64), ("stride_class", ctypes.c_int64), ("classes", ctypes.c_int32),
+        ("reserved", ctypes.c_int32), ("temperature", ctypes.c_double),
+    ]
+
+
+class QmriLabelScoresArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", QmriLogits), ("labels", ctypes.c_void_p), ("l_kind", ctypes.c_int32), ("top", ctypes.c_int32),
+        ("ignore_label", ctypes.c_int64), ("log_prob", ctypes.c_void_p), ("entropy", ctypes.c_void_p),
+        ("norm", ctypes.c_void_p), ("top_log_prob", ctypes.c_void_p), ("top_label", ctypes.c_void_p),
+        ("grad_log_prob", ctypes.c_void_p), ("grad_entropy", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+        ("grad_stride_outer", ctypes.c_int64), ("grad_stride_inner", ctypes.c_int64), ("grad_stride_class", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("device", ctypes.c_int32),
+        ("reserved", ctypes.c_int32), ("stream", ctypes.c_void_p),
+    ]
+
+
+class QmriDistillArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", QmriLogits), ("top_label", ctypes.c_void_p), ("values", ctypes.c_void_p), ("l_kind", ctypes.c_int32),
+        ("v_dtype", ctypes.c_int32), ("entries", ctypes.c_int32), ("tail", ctypes.c_int32), ("loss", ctypes.c_void_p),
+        ("norm", ctypes.c_void_p), ("log_tail", ctypes.c_void_p), ("grad_loss", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+        ("grad_stride_outer", ctypes.c_int64), ("grad_stride_inner", ctypes.c_int64), ("grad_stride_class", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("device", ctypes.c_int32),
+        ("reserved", ctypes.c_int32), ("stream", ctypes.c_void_p),
+    ]
+
+
+L_KINDS = {"int32": 0, "uint8": 1, "int16": 2, "int64": 3}
+SCORE_DTYPES = {"float32": QMRI_F32, "float16": QMRI_F16, "bfloat16": QMRI_BF16}
+MAX_TOP = 64
+
 MODELS = {"monoexponential": 0, "biexponential": 1}
 MODEL_NPARAMS = {"monoexponential": 2, "biexponential": 4}
 # "fp16x3" is the parity mode (logits within 1e-3 of an fp64 run); "fp16x3-general" forces it onto the general
@@ -162,6 +198,9 @@ EXPORTS = (
     "qmri_conv2d_nhwc_host", "qmri_dess_t2_device", "qmri_dess_t2_host", "qmri_rss_host",
     "qmri_lmfit_defaults", "qmri_lmfit_device", "qmri_lmfit_host", "qmri_region_stats_host",
     "qmri_region_stats_device", "qmri_host_alloc", "qmri_host_free", "qmri_device_mem_info", "qmri_selftest_fp64",
+    "qmri_label_scores_device", "qmri_label_scores_host", "qmri_label_scores_grad_device", "qmri_label_scores_grad_host",
+    "qmri_label_scores_workspace", "qmri_distill_device", "qmri_distill_host", "qmri_distill_grad_device",
+    "qmri_distill_grad_host", "qmri_distill_workspace",
 )
 
 _lib = None
@@ -297,6 +336,14 @@ def load():
         lib.qmri_lmfit_device.restype = ctypes.c_int
         lib.qmri_lmfit_host.argtypes = [ctypes.POINTER(QmriLmfitArgs)]
         lib.qmri_lmfit_host.restype = ctypes.c_int
+        for op, args in (("label_scores", QmriLabelScoresArgs), ("distill", QmriDistillArgs)):
+            for name in (f"qmri_{op}_device", f"qmri_{op}_host", f"qmri_{op}_grad_device", f"qmri_{op}_grad_host"):
+                fn = getattr(lib, name)
+                fn.argtypes = [ctypes.POINTER(args)]
+                fn.restype = ctypes.c_int
+            fn = getattr(lib, f"qmri_{op}_workspace")
+            fn.argtypes = [ctypes.POINTER(args), ctypes.POINTER(ctypes.c_uint64)]
+            fn.restype = ctypes.c_int
         _lib = lib
         return lib
 
@@ -825,3 +872,96 @@ def rss_host(echo1, echo2, method="rss", device=None):
     check(lib.qmri_rss_host(_ptr(e1), _ptr(e2), qdtype(e1.dtype), e1.size, 0 if method == "rss" else 1,
                             _ptr(out), _dev(device)))
     return out
+
+
+# ---- operators on a network's answers: dosma_amd.models.answers is the array-level interface -----------------------------
+class Rows:
+    """Geometry of a batch of category scores (include/qmri.h: qmri_logits): row n begins at element
+    ``(n // inner) * so + (n % inner) * si``, its classes lie ``sc`` elements apart."""
+
+    __slots__ = ("rows", "classes", "inner", "so", "si", "sc")
+
+    def __init__(self, rows, classes, inner=None, so=0, si=None, sc=1):
+        self.rows, self.classes = rows, classes
+        self.inner = max(rows, 1) if inner is None else inner
+        self.so, self.si, self.sc = so, classes if si is None else si, sc
+
+
+def _fill_logits(a, ptr, dtype, rows, temperature, background):
+    z = a.logits
+    z.data, z.dtype, z.background = ptr, SCORE_DTYPES[dtype], 1 if background else 0
+    z.rows, z.inner, z.classes = rows.rows, rows.inner, rows.classes
+    z.stride_outer, z.stride_inner, z.stride_class = rows.so, rows.si, rows.sc
+    z.temperature = float(temperature)
+
+
+def _fill_grad(a, ptr, rows):
+    a.grad = ptr
+    a.grad_stride_outer, a.grad_stride_inner, a.grad_stride_class = rows.so, rows.si, rows.sc
+
+
+def _run_answers(op, a, host, device, stream, workspace):
+    """``workspace(bytes)`` -> device pointer: memory of the caller's own allocator for the calls that need some."""
+    lib = load()
+    if host:
+        require_device()
+        a.device = _dev(device)
+        check(getattr(lib, f"qmri_{op}_host")(ctypes.byref(a)))
+        return
+    a.device, a.stream = int(device), stream
+    if workspace is not None:
+        need = ctypes.c_uint64(0)
+        check(getattr(lib, f"qmri_{op}_workspace")(ctypes.byref(a), ctypes.byref(need)))
+        if need.value:
+            a.workspace, a.workspace_bytes = workspace(need.value), need.value
+    check(getattr(lib, f"qmri_{op}_device")(ctypes.byref(a)))
+
+
+def label_scores(logits_ptr, dtype, rows, *, labels_ptr=None, l_dtype=None, top=0, ignore_label=-1, temperature=1.0,
+                 background=False, log_prob=None, entropy=None, norm=None, top_log_prob=None, top_label=None, host=False,
+                 device=None, stream=None, workspace=None):
+    """``qmri_label_scores_device`` (raw device pointers, e.g. ``tensor.data_ptr()``) or, with ``host=True``,
+    ``qmri_label_scores_host``.  ``dtype``: "float32" | "float16" | "bfloat16"; ``rows``: a :class:`Rows`."""
+    a = QmriLabelScoresArgs()
+    _fill_logits(a, logits_ptr, dtype, rows, temperature, background)
+    if labels_ptr is not None:
+        a.labels, a.l_kind = labels_ptr, L_KINDS[l_dtype]
+    a.top, a.ignore_label = int(top), int(ignore_label)
+    a.log_prob, a.entropy, a.norm, a.top_log_prob, a.top_label = log_prob, entropy, norm, top_log_prob, top_label
+    _run_answers("label_scores", a, host, device, stream, workspace)
+
+
+def label_scores_grad(logits_ptr, dtype, rows, grad_ptr, grad_rows, norm, *, labels_ptr=None, l_dtype=None, ignore_label=-1,
+                      temperature=1.0, background=False, entropy=None, grad_log_prob=None, grad_entropy=None, host=False,
+                      device=None, stream=None):
+    a = QmriLabelScoresArgs()
+    _fill_logits(a, logits_ptr, dtype, rows, temperature, background)
+    _fill_grad(a, grad_ptr, grad_rows)
+    if labels_ptr is not None:
+        a.labels, a.l_kind = labels_ptr, L_KINDS[l_dtype]
+    a.ignore_label = int(ignore_label)
+    a.norm, a.entropy, a.grad_log_prob, a.grad_entropy = norm, entropy, grad_log_prob, grad_entropy
+    _run_answers("label_scores_grad", a, host, device, stream, None)
+
+
+def distill(logits_ptr, dtype, rows, top_label_ptr, l_dtype, values_ptr, v_dtype, entries, *, tail=False, temperature=1.0,
+            background=False, loss=None, norm=None, log_tail=None, host=False, device=None, stream=None, workspace=None):
+    """``qmri_distill_device`` / ``qmri_distill_host``."""
+    a = QmriDistillArgs()
+    _fill_logits(a, logits_ptr, dtype, rows, temperature, background)
+    a.top_label, a.l_kind, a.values, a.v_dtype = top_label_ptr, L_KINDS[l_dtype], values_ptr, SCORE_DTYPES[v_dtype]
+    a.entries, a.tail = int(entries), 1 if tail else 0
+    a.loss, a.norm, a.log_tail = loss, norm, log_tail
+    _run_answers("distill", a, host, device, stream, workspace)
+
+
+def distill_grad(logits_ptr, dtype, rows, grad_ptr, grad_rows, top_label_ptr, l_dtype, values_ptr, v_dtype, entries, norm,
+                 grad_loss, *, log_tail=None, tail=False, temperature=1.0, background=False, host=False, device=None,
+                 stream=None):
+    a = QmriDistillArgs()
+    _fill_logits(a, logits_ptr, dtype, rows, temperature, background)
+    _fill_grad(a, grad_ptr, grad_rows)
+    a.top_label, a.l_kind, a.values, a.v_dtype = top_label_ptr, L_KINDS[l_dtype], values_ptr, SCORE_DTYPES[v_dtype]
+    a.entries, a.tail = int(entries), 1 if tail else 0
+    a.norm, a.log_tail, a.grad_loss = norm, log_tail, grad_loss
+    _run_answers("distill_grad", a, host, device, stream, None)

@@ -14,8 +14,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libqmri_hip.so")
-SOURCES = ["qmri_capi.hip", "monoexp_lm.hip", "linfit.hip", "lm_generic.hip", "unet_kernels.hip", "unet_rw.hip", "unet_s3.hip", "unet_c4.hip", "unet_d4.hip", "unet_enc0.hip", "unet_engine.hip", "dess.hip", "region_stats.hip"]
+SOURCES = ["qmri_capi.hip", "monoexp_lm.hip", "linfit.hip", "lm_generic.hip", "unet_kernels.hip", "unet_rw.hip", "unet_s3.hip", "unet_c4.hip", "unet_d4.hip", "unet_enc0.hip", "unet_engine.hip", "dess.hip", "region_stats.hip",
+           "label_scores.hip", "distill.hip", "answers_capi.hip"]
 ARCH = "gfx950"
+# packed fp32 instructions are kept out of these sources: their sums must not depend on the form the compiler picks
+_NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+EXTRA_FLAGS = {"label_scores.hip": _NO_PACKED, "distill.hip": _NO_PACKED}
 
 
 def _hipcc():
@@ -45,7 +49,7 @@ def build_variant(name: str, extra_flags) -> str:
         if os.path.exists(obj) and os.path.getmtime(obj) > max(
                 [os.path.getmtime(os.path.join(CSRC, f)) for f in os.listdir(CSRC)] + [os.path.getmtime(os.path.join(ROOT, "include", "qmri.h"))]):
             continue
-        cmd = [_hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", *extra_flags,
+        cmd = [_hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", *EXTRA_FLAGS.get(src, []), *extra_flags,
                "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c", os.path.join(CSRC, src), "-o", obj]
         procs.append((src, subprocess.Popen(cmd)))
     for src, p in procs:
@@ -85,7 +89,7 @@ def _build_locked(bdir: str, verbose: bool, force: bool = False) -> str:
         if (not force and os.path.exists(obj)
                 and os.path.getmtime(obj) > max(os.path.getmtime(os.path.join(CSRC, src)), hdr_time)):
             continue
-        cmd = [_hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
+        cmd = [_hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", *EXTRA_FLAGS.get(src, []),
                "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd))

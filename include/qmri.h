@@ -53,7 +53,9 @@ typedef enum qmri_dtype {
     QMRI_F32 = 0,
     QMRI_F64 = 1,
     QMRI_I16 = 2,
-    QMRI_U16 = 3
+    QMRI_U16 = 3,
+    QMRI_F16 = 4, /* half / bfloat16: category scores and what belongs to them (qmri_logits) only */
+    QMRI_BF16 = 5
 } qmri_dtype;
 
 /* initial guess p0 = (a0, b0) of  y = a * exp(b * x) */
@@ -382,6 +384,106 @@ int qmri_region_stats_host(const qmri_region_stats_args *args); /* values / labe
 /* values / labels already on the device (e.g. the tc map a fit has just written); label_keys and out stay host
  * pointers; the call enqueues on `hip_stream` and returns after the 4 x (nkeys + 1) results have arrived */
 int qmri_region_stats_device(const qmri_region_stats_args *args, void *hip_stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * ---- What a network's answers say: log probabilities, entropy, alternatives, distillation ---------------------------
+ * The reference keeps `model.predict(...) > 0.5` and nothing else of a network's answer (/root/reference/dosma/models/
+ * oaiunet2d.py:305-316).  The entries below read the category scores themselves -- of qmri_unet2d_forward, or of any other
+ * network -- as one softmax per row (voxel, token, ...):
+ *     p_j = exp((z_j - M) / T) / s,   M = max z,   s = sum_j exp((z_j - M) / T)
+ * `background` adds an implicit category 0 of score 0 in front of the C classes (category = class + 1).  For the networks of
+ * this library, whose classes have sigmoid heads, that is the distribution of the label under the condition that a voxel
+ * carries at most one tissue: P(0) = 1 / (1 + sum e^{z_c}), P(c) = e^{z_c} / (1 + sum e^{z_c}).
+ *
+ * Geometry: row n of `rows` begins at data + (n / inner) * stride_outer + (n % inner) * stride_inner, its classes lie
+ * stride_class apart (all in elements): rows of classes are (inner = rows, stride_inner = C, stride_class = 1), the
+ * (B, C, H, W) answers of a torch network (inner = H W, stride_outer = C H W, stride_inner = 1, stride_class = H W).
+ * Per-row arrays ([rows] ...) are dense in the order of n.
+ *
+ * Special scores.  -inf: a category that is not offered (probability 0, never an alternative).  A row of nothing but -inf is
+ * empty: log probability -inf, entropy 0, no alternatives, loss 0, gradient 0.  NaN or +inf: the row's results are NaN. */
+typedef struct qmri_logits {
+    const void *data;     /* category scores */
+    int32_t dtype;        /* QMRI_F32 | QMRI_F16 | QMRI_BF16 */
+    int32_t background;   /* 1: implicit category 0 of score 0 */
+    int64_t rows;
+    int64_t inner;        /* 1 <= inner */
+    int64_t stride_outer, stride_inner, stride_class; /* >= 0; 0 repeats a broadcast score */
+    int32_t classes;      /* C >= 1, without the background */
+    int32_t reserved;
+    double temperature;   /* T > 0 */
+} qmri_logits;
+/* element type of labels */
+#define QMRI_L_I32 0
+#define QMRI_L_U8 1
+#define QMRI_L_I16 2
+#define QMRI_L_I64 3
+#define QMRI_MAX_TOP 64 /* alternatives per row; teacher entries per row */
+typedef struct qmri_label_scores_args {
+    qmri_logits logits;
+    const void *labels;   /* nullable [rows]: the given label of every row */
+    int32_t l_kind;       /* QMRI_L_* */
+    int32_t top;          /* alternatives wanted: 0 .. min(QMRI_MAX_TOP, categories) */
+    int64_t ignore_label; /* rows with this label have none: log_prob 0, no gradient from it.  Any other label that is not a
+                             category gives NaN (and a NaN gradient) */
+    /* results of qmri_label_scores_*, each nullable; entropy and norm are inputs of qmri_label_scores_grad_* */
+    float *log_prob;      /* [rows] log p_label */
+    float *entropy;       /* [rows] -sum p log p (nats) */
+    float *norm;          /* [rows][2]: M and ln s -- what the gradient needs; M / T + ln s = log sum exp(z / T) */
+    float *top_log_prob;  /* [rows][top] the largest log probabilities, in falling order (ties: lowest category first) */
+    int32_t *top_label;   /* [rows][top] their categories; -1 (with log probability -inf) where fewer are offered */
+    /* gradient: grad = grad_log_prob d log_prob / dz + grad_entropy d entropy / dz */
+    const float *grad_log_prob; /* nullable [rows]; needs labels */
+    const float *grad_entropy;  /* nullable [rows]; needs entropy */
+    void *grad;                 /* same type and classes as the logits, rounded once */
+    int64_t grad_stride_outer, grad_stride_inner, grad_stride_class;
+    void *workspace;            /* nullable: device memory of at least qmri_label_scores_workspace() bytes, in use until the
+                                   call's work is done; NULL: taken from the stream's memory pool (not while capturing) */
+    uint64_t workspace_bytes;
+    int32_t device;
+    int32_t reserved;
+    void *stream;
+} qmri_label_scores_args;
+int qmri_label_scores_device(const qmri_label_scores_args *args);      /* device pointers, asynchronous on args->stream */
+int qmri_label_scores_grad_device(const qmri_label_scores_args *args); /* device pointers, asynchronous; no workspace */
+int qmri_label_scores_workspace(const qmri_label_scores_args *args, uint64_t *bytes); /* 0: none needed */
+/* host pointers, synchronous; logits and grad are dense rows (inner = rows, stride_inner = classes, stride_class = 1) */
+int qmri_label_scores_host(const qmri_label_scores_args *args);
+int qmri_label_scores_grad_host(const qmri_label_scores_args *args);
+
+/* Divergence (nats) of a student's answers from a teacher's K best ones, per row:
+ *   tail 0:  q = softmax(values / T) over the entries;            loss = sum_k q_k (log q_k - log p_{label_k})
+ *   tail 1:  values are log probabilities (at the same T, float32), q_k = exp(value_k), and the rest q_t = 1 - sum q_k of the
+ *            teacher's mass is compared with the student's mass p_t outside the entries:  loss += q_t (log q_t - log p_t);
+ *            q_t <= K 2^-24 (the rounding of the stored values) counts as 0
+ * An entry whose label is not a category (-1, as qmri_label_scores leaves it) is an empty slot; a row without any entry has
+ * loss 0 and gradient 0.  The same label twice: both entries count (and are left out of the tail once). */
+typedef struct qmri_distill_args {
+    qmri_logits logits;   /* the student's */
+    const void *top_label; /* [rows][entries] */
+    const void *values;    /* [rows][entries] */
+    int32_t l_kind;        /* QMRI_L_I32 | QMRI_L_I64 */
+    int32_t v_dtype;       /* QMRI_F32 | QMRI_F16 | QMRI_BF16 (tail: QMRI_F32) */
+    int32_t entries;       /* 1 .. QMRI_MAX_TOP */
+    int32_t tail;
+    /* results of qmri_distill_*, each nullable; norm and log_tail are inputs of qmri_distill_grad_* */
+    float *loss;           /* [rows] */
+    float *norm;           /* [rows][2] as above */
+    float *log_tail;       /* [rows] log p_t (tail 1) */
+    const float *grad_loss; /* [rows] */
+    void *grad;            /* d sum_n grad_loss_n loss_n / dz: same type and classes as the logits, rounded once */
+    int64_t grad_stride_outer, grad_stride_inner, grad_stride_class;
+    void *workspace;       /* as in qmri_label_scores_args */
+    uint64_t workspace_bytes;
+    int32_t device;
+    int32_t reserved;
+    void *stream;
+} qmri_distill_args;
+int qmri_distill_device(const qmri_distill_args *args);
+int qmri_distill_grad_device(const qmri_distill_args *args);
+int qmri_distill_workspace(const qmri_distill_args *args, uint64_t *bytes);
+int qmri_distill_host(const qmri_distill_args *args);
+int qmri_distill_grad_host(const qmri_distill_args *args);
 
 /* Mean kernel time in ms of the last qmri_monoexp_fit_device call on this thread that was issued
  * with timing enabled (qmri_set_timing(1)); measured with hipEvents on the launch stream. */
