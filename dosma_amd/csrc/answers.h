@@ -6,6 +6,8 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "qmri.h"
 
 namespace qmri {
@@ -19,7 +21,20 @@ struct LogitsK {
     int C, bg;
     float c2;    // log2(e) / T: exp((z - M) / T) = exp2((z - M) * c2)
     float invT;  // 1 / T
+    // n / inner for n < 2^31 as (n * magic) >> shift: shift = 31 + ceil(log2 inner), magic = ceil(2^shift / inner) < 2^32; the
+    // error magic * inner - 2^shift is below 2^(shift - 31), so n times it stays below 2^shift.  magic 0: rows do not fit 31 bits
+    unsigned magic;
+    int shift;
 };
+inline void set_division(LogitsK &g) {
+    g.magic = 0;
+    g.shift = 0;
+    if (g.rows > 0x7fffffffll || g.inner >= g.rows) return;
+    int b = 0;
+    while ((1ll << b) < g.inner) ++b;
+    g.shift = 31 + b;
+    g.magic = (unsigned)(((1ull << g.shift) + (unsigned long long)g.inner - 1) / (unsigned long long)g.inner);
+}
 
 struct ScoresK {
     LogitsK g;
@@ -80,31 +95,145 @@ __device__ __forceinline__ long long load_label(const void *p, int kind, long lo
 
 __device__ __forceinline__ long long row_base(const LogitsK &g, long long n, long long so, long long si) {
     if (g.inner >= g.rows) return n * si;
-    // (a 64-bit division is some 100 instructions: rows that fit 32 bits take the short one)
-    long long o;
-    if (g.rows <= 0x7fffffffll) o = (unsigned)n / (unsigned)g.inner;
-    else o = n / g.inner;
+    const long long o = g.magic ? (long long)(((unsigned long long)(unsigned)n * g.magic) >> g.shift) : n / g.inner;
     return o * so + (n - o * g.inner) * si;
 }
 
-// Running statistics of a row or of a part of one: maximum m, s = sum exp2((z - m) c2), t = sum exp2((z - m) c2) (z - m) c2.
-// Everything is held in 32 bits.  A part without any offered category is (-inf, 0, 0).
-struct RowStat {
-    float m, s, t;
+// ---- scores of a row ------------------------------------------------------------------------------------------------------
+// A vector is 16 bytes of scores, at the alignment of one score: rows of odd length begin anywhere, and the memory takes a
+// 16-byte load at any address (aligned ones are not split off: the peeling costs more than the odd line)
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);
+template <typename T>
+struct Vec {
+    T v[kVec<T>];
 };
-
-// exponent of the change of reference from m to M >= m.  Clamped: -inf (nothing seen yet) times a zero sum must stay zero.
-__device__ __forceinline__ float shift2(float m, float M, float c2) {
-    return m == M ? 0.f : fmaxf((m - M) * c2, -1.0e4f);
-}
-__device__ __forceinline__ RowStat join(const RowStat &a, const RowStat &b, float c2) {
-    RowStat r;
-    r.m = fmaxf(a.m, b.m);
-    const float da = shift2(a.m, r.m, c2), db = shift2(b.m, r.m, c2);
-    const float fa = exp2_hw(da), fb = exp2_hw(db);
-    r.s = a.s * fa + b.s * fb;
-    r.t = fa * (a.t + da * a.s) + fb * (b.t + db * b.s);
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T *p) {
+    Vec<T> r;
+    __builtin_memcpy(&r, p, 16);
     return r;
+}
+// the first n scores of a vector that ends behind its row, the rest -inf
+template <typename T>
+__device__ __forceinline__ Vec<T> load_part(const T *p, int n) {
+    Vec<T> r;
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) r.v[i] = i < n ? p[i] : static_cast<T>(kNegInf);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_part(T *p, const Vec<T> &r, int n) {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i)
+        if (i < n) p[i] = r.v[i];
+}
+
+// NaN goes through a maximum here (v_maximum3_f32), so a row's NaN reaches its statistics without a test of its own
+__device__ __forceinline__ float maxn(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// exponents are kept above -200: exp2 of that is 0 already, and 0 * -200 is 0 where 0 * -inf would not be
+__device__ __forceinline__ float clamp2(float d) { return maxn(d, -200.f); }
+
+// what a row's sums refer to: its maximum, or the lowest finite value where nothing is offered
+__device__ __forceinline__ float reference(float M) { return maxn(M, -3.4028234663852886e38f); }
+
+// ---- reductions over 2, 4, .. 64 neighbouring lanes, the result in each of them: DPP moves and lane swaps, no LDS -------------
+template <int STEP>
+__device__ __forceinline__ void partner(unsigned x, unsigned &a, unsigned &b) {
+    if constexpr (STEP == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        a = r[0];
+        b = r[1];
+    } else if constexpr (STEP == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        a = r[0];
+        b = r[1];
+    } else {
+        // quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror, row_mirror: within 8 and 16 lanes the halves hold one value each by then
+        constexpr int ctrl = STEP == 1 ? 0xB1 : STEP == 2 ? 0x4E : STEP == 4 ? 0x141 : 0x140;
+        a = x;
+        b = (unsigned)__builtin_amdgcn_update_dpp((int)x, (int)x, ctrl, 0xf, 0xf, false);
+    }
+}
+template <int G, int STEP = 1>
+__device__ __forceinline__ float group_max(float x) {
+    if constexpr (STEP < G) {
+        unsigned a, b;
+        partner<STEP>(__float_as_uint(x), a, b);
+        return group_max<G, STEP * 2>(maxn(__uint_as_float(a), __uint_as_float(b)));
+    }
+    return x;
+}
+template <int G, int STEP = 1>
+__device__ __forceinline__ float group_sum(float x) {
+    if constexpr (STEP < G) {
+        unsigned a, b;
+        partner<STEP>(__float_as_uint(x), a, b);
+        return group_sum<G, STEP * 2>(__uint_as_float(a) + __uint_as_float(b));
+    }
+    return x;
+}
+template <int G, int STEP = 1>
+__device__ __forceinline__ unsigned group_maxu(unsigned x) {
+    if constexpr (STEP < G) {
+        unsigned a, b;
+        partner<STEP>(x, a, b);
+        return group_maxu<G, STEP * 2>(a > b ? a : b);
+    }
+    return x;
+}
+template <int G, int STEP = 1>
+__device__ __forceinline__ int group_min(int x) {
+    if constexpr (STEP < G) {
+        unsigned a, b;
+        partner<STEP>((unsigned)x, a, b);
+        return group_min<G, STEP * 2>((int)a < (int)b ? (int)a : (int)b);
+    }
+    return x;
+}
+
+// sum of 2^k values as a tree
+template <int N>
+__device__ __forceinline__ float tree_sum(const float (&v)[N]) {
+    float a[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = v[i];
+#pragma unroll
+    for (int h = N / 2; h > 0; h >>= 1)
+#pragma unroll
+        for (int i = 0; i < h; ++i) a[i] += a[i + h];
+    return a[0];
+}
+
+// Running statistics of a part of a row: the maximum m of its scores (-inf: none offered), and relative to a finite reference
+// ref  s = sum exp2((z - ref) c2),  t = sum exp2((z - ref) c2) (z - ref) c2.  Everything is held in 32 bits.
+struct RowStat {
+    float m, ref, s, t;
+};
+__device__ __forceinline__ RowStat no_stat() { return {kNegInf, -3.4028234663852886e38f, 0.f, 0.f}; }
+// the sums of r relative to another reference
+__device__ __forceinline__ void rebase(RowStat &r, float ref, float c2) {
+    const float d = r.ref == ref ? 0.f : maxn((r.ref - ref) * c2, -1.0e4f);
+    const float f = exp2_hw(d);
+    r.t = f * (r.t + d * r.s);
+    r.s *= f;
+    r.ref = ref;
+}
+// all lanes of a wave together
+__device__ __forceinline__ RowStat wave_join(RowStat r, float c2) {
+    const float M = group_max<64>(r.m);
+    rebase(r, reference(M), c2);
+    r.m = M;
+    r.s = group_sum<64>(r.s);
+    r.t = group_sum<64>(r.t);
+    return r;
+}
+__device__ __forceinline__ RowStat join(RowStat a, RowStat b, float c2) {
+    const float M = maxn(a.m, b.m), ref = reference(M);
+    rebase(a, ref, c2);
+    rebase(b, ref, c2);
+    return {M, ref, a.s + b.s, a.t + b.t};
 }
 
 // what a wave's lanes have written to LDS is visible to its other lanes from here on
@@ -116,6 +245,13 @@ __device__ __forceinline__ void wave_sync() {
 
 // a better than b in the order of the alternatives: larger score, ties to the lower label
 __device__ __forceinline__ bool better(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
+
+// How the rows of a call are cut for the kernels that give a block a row (contiguous classes, more than 1024 of them): segments
+// of whole 16-byte vectors, at most 65536 scores each (the distillation kernel marks the teacher's labels in LDS, a bit a score)
+struct Cut {
+    int segs, len;
+};
+Cut cut_rows(const LogitsK &g, int num_cu);
 
 hipError_t label_scores_launch(const ScoresK &k, int dtype, int num_cu, hipStream_t st);
 size_t label_scores_workspace_bytes(const ScoresK &k, int dtype, int num_cu);

@@ -130,6 +130,7 @@ qmri::LogitsK geometry(const qmri_logits &l) {
     g.bg = l.background;
     g.c2 = (float)(1.4426950408889634074 / l.temperature);
     g.invT = (float)(1.0 / l.temperature);
+    qmri::set_division(g);
     return g;
 }
 

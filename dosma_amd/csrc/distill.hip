@@ -4,181 +4,892 @@
 //   tail = 0:  q = softmax(v / T) over the entries,            L = sum_k q_k (log q_k - log p_{i_k})
 //   tail = 1:  q_k = e^{v_k}, q_t = 1 - sum q_k, p_t = sum_{j not in i} p_j,   L = (the same sum) + q_t (log q_t - log p_t)
 //   g_j = w / T [ Q p_j - sum_{k: i_k = j} q_k - [j not in i] q_t p_j / p_t ],   Q = sum_k q_k + q_t
+//
+// The student's scores are read once (and the gradient written once); p_t is summed over the categories outside the entries,
+// never as a difference.  Who owns a row is as in label_scores.hip: a lane (up to 8 classes, or classes that do not lie
+// together), 2 .. 64 lanes (up to 1024 contiguous classes), one or several blocks (more).
 #include "answers.h"
 
 namespace qmri {
 namespace {
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
+constexpr float kSlack = 4.f;  // (a lane's reference follows its maximum when that has grown by a factor of 16)
 
 __device__ __forceinline__ float load_value(const DistillK &k, long long i) {
     if (k.v_dtype == QMRI_F32) return static_cast<const float *>(k.values)[i];
     if (k.v_dtype == QMRI_F16) return to_f32(static_cast<const f16_t *>(k.values)[i]);
     return to_f32(static_cast<const bf16_t *>(k.values)[i]);
 }
+// entry q of row n: its label (-1: empty slot) and value
+__device__ __forceinline__ int load_entry(const DistillK &k, long long n, int q, int cats, float &v) {
+    const long long l = load_label(k.labels, k.l_kind, n * k.K + q);
+    v = load_value(k, n * k.K + q);
+    return (l >= 0 && l < cats) ? (int)l : -1;
+}
 
-// The teacher's side of a row, one entry a lane: label (-1: empty slot), q and log q; the mass outside the entries.
+// ---- the teacher's side of a row ----------------------------------------------------------------------------------------------
+// An entry's weight is q = exp2((v - m) * c2) * scale, its logarithm (v - m) * (1 / T) + lscale: with the tail m = 0, T = 1 and
+// scale = 1, without it m is the largest value and scale = 1 / sum.
 struct Teacher {
-    int idx;
-    float q, lq;
-    float rest, total;  // q_t, Q: the same in every lane
-    bool any;
+    float m, c2, invT, scale, lscale;
+    float rest, total;  // q_t, Q
+    bool some;          // any entry that counts
 };
-__device__ __forceinline__ Teacher teacher_wave(const DistillK &k, long long n, int lane, int cats) {
-    Teacher t = {-1, 0.f, kNegInf, 0.f, 0.f, false};
-    float v = kNegInf;
-    if (lane < k.K) {
-        const long long l = load_label(k.labels, k.l_kind, n * k.K + lane);
-        if (l >= 0 && l < cats) {
-            t.idx = (int)l;
-            v = load_value(k, n * k.K + lane);
-        }
-    }
-    const bool ok = t.idx >= 0;
-    t.any = __ballot(ok) != 0ull;
-    const float m = wave_max(v);
+__device__ __forceinline__ float weight(const Teacher &t, float v) { return exp2_hw((v - t.m) * t.c2) * t.scale; }
+__device__ __forceinline__ float log_weight(const Teacher &t, float v) { return (v - t.m) * t.invT + t.lscale; }
+// From what the entries give together: their number, largest value m, sum of exp2((v - base) c2), base = m or (tail) 0, and in
+// the tail the sum without one entry of the largest value.
+__device__ __forceinline__ Teacher teacher_of(const DistillK &k, bool any, float m, float sum, float others) {
+    Teacher t;
     if (k.tail) {
-        t.lq = v;
-        t.q = ok ? expf(v) : 0.f;
-        // q_t = (1 - e^{v_max}) - the other entries: exact for a teacher that is sure of itself
-        const unsigned long long at = __ballot(ok && v == m);
-        const int first = at ? __ffsll(at) - 1 : 0;
-        const float others = wave_sum(lane == first ? 0.f : t.q);
+        t.m = 0.f;
+        t.c2 = kLog2e;
+        t.invT = 1.f;
+        t.scale = 1.f;
+        t.lscale = 0.f;
+        // 1 - sum q as (1 - e^{v_max}) - the others: nothing cancels for a teacher that is sure of itself
         const float rest = -expm1f(m) - others;
-        t.rest = (!t.any || rest <= (float)k.K * 5.9604645e-8f) ? 0.f : rest;
-        t.total = wave_sum(t.q) + t.rest;
+        t.rest = (any && !(rest <= (float)k.K * 5.9604645e-8f)) ? rest : 0.f;
+        t.total = sum + t.rest;
+        t.some = any;
     } else {
-        const float d = (v - m) * k.g.invT;
-        const float e = (ok && m > kNegInf) ? expf(d) : (v != v ? v : 0.f);
-        const float s = wave_sum(e);
-        if (s == 0.f) t.any = false;
-        t.q = (ok && s != 0.f) ? e / s : 0.f;
-        t.lq = d - logf(s);
-        t.total = t.any ? 1.f : 0.f;
+        t.m = m;
+        t.c2 = k.g.c2;
+        t.invT = k.g.invT;
+        t.scale = 1.f / sum;
+        t.lscale = -logf(sum);
+        t.rest = 0.f;
+        t.some = any && sum != 0.f;
+        t.total = t.some ? 1.f : 0.f;
     }
     return t;
 }
+__device__ __forceinline__ float teacher_term(const DistillK &k, float v, float m) {
+    return k.tail ? exp2_hw(v * kLog2e) : (m == kNegInf ? (v != v ? v : 0.f) : exp2_hw((v - m) * k.g.c2));
+}
+// by G lanes, entries q = gl, gl + G, ..
+template <int G>
+__device__ __forceinline__ Teacher teacher_group(const DistillK &k, long long n, int gl, int cats) {
+    float m = kNegInf;
+    float cnt = 0.f;
+    for (int q = gl; q < k.K; q += G) {
+        float v;
+        if (load_entry(k, n, q, cats, v) >= 0) {
+            m = maxn(m, v);
+            cnt = 1.f;
+        }
+    }
+    m = group_max<G>(m);
+    const bool any = group_max<G>(cnt) > 0.f;
+    float sum = 0.f, others = 0.f;
+    int first = 0x7fffffff;
+    for (int q = gl; q < k.K; q += G) {
+        float v;
+        if (load_entry(k, n, q, cats, v) < 0) continue;
+        const float e = teacher_term(k, v, m);
+        sum += e;
+        if (v == m && first == 0x7fffffff) first = q;
+        else others += e;
+    }
+    const int one = group_min<G>(first);
+    if (first != one && first != 0x7fffffff) others += teacher_term(k, m, m);
+    return teacher_of(k, any, m, group_sum<G>(sum), group_sum<G>(others));
+}
+template <>
+__device__ __forceinline__ Teacher teacher_group<1>(const DistillK &k, long long n, int, int cats) {
+    float m = kNegInf;
+    bool any = false;
+    for (int q = 0; q < k.K; ++q) {
+        float v;
+        if (load_entry(k, n, q, cats, v) >= 0) {
+            m = maxn(m, v);
+            any = true;
+        }
+    }
+    float sum = 0.f, others = 0.f;
+    bool left_out = false;
+    for (int q = 0; q < k.K; ++q) {
+        float v;
+        if (load_entry(k, n, q, cats, v) < 0) continue;
+        const float e = teacher_term(k, v, m);
+        sum += e;
+        if (v == m && !left_out) left_out = true;
+        else others += e;
+    }
+    return teacher_of(k, any, m, sum, others);
+}
 
-// One wave a row, any strides.
+// ---- results of a row -----------------------------------------------------------------------------------------------------------
+// s: of all categories, so: of those outside the entries, both relative to reference(M)
+struct Student {
+    float ref, ls;
+    bool empty;
+};
+__device__ __forceinline__ Student student_of(float M, float s) { return {reference(M), __builtin_amdgcn_logf(s) * kLn2, s == 0.f}; }
+__device__ __forceinline__ float entry_loss(const DistillK &k, const Teacher &t, const Student &p, float v, float z) {
+    const float q = weight(t, v);
+    const float lp = (z == kNegInf && p.ls == p.ls) ? kNegInf : (z - p.ref) * k.g.invT - p.ls;
+    return q == 0.f ? 0.f : q * (log_weight(t, v) - lp);
+}
 template <typename T>
-__global__ __launch_bounds__(256) void distill_wave_kernel(const DistillK k) {
-    __shared__ int s_idx[4][64];
+__device__ __forceinline__ float gather(const LogitsK &g, const T *z, int l) {
+    return l < g.bg ? 0.f : to_f32(z[(long long)(l - g.bg) * g.sc]);
+}
+// ln of the sum outside the entries, relative to p.ref.  A student that leaves less than 2^-100 out there (its terms vanish next to
+// the maximum's) has it summed again relative to the largest outside: the G lanes read the row once more.  Rare.
+template <int G, typename T>
+__device__ __forceinline__ float log_outside(const DistillK &k, long long n, const T *z, int gl, int cats, const Student &p, const Teacher &t, float so) {
+    if (!k.tail) return 0.f;
+    if (!(so < 7.888609e-31f) || t.rest == 0.f || p.empty) return __builtin_amdgcn_logf(so) * kLn2;
+    auto score = [&](int j) {
+        float v;
+        for (int q = 0; q < k.K; ++q)
+            if (load_entry(k, n, q, cats, v) == j) return kNegInf;
+        return gather(k.g, z, j);
+    };
+    float m = kNegInf, s = 0.f;
+    for (int j = gl; j < cats; j += G) m = maxn(m, score(j));
+    m = group_max<G>(m);
+    for (int j = gl; j < cats; j += G) s += exp2_hw((score(j) - reference(m)) * k.g.c2);
+    s = group_sum<G>(s);
+    return s == 0.f ? kNegInf : (m - p.ref) * k.g.invT + __builtin_amdgcn_logf(s) * kLn2;
+}
+__device__ __forceinline__ void write_row(const DistillK &k, long long n, float M, float lso, const Student &p, const Teacher &t, float loss) {
+    const float lt = p.empty ? kNegInf : lso - p.ls;
+    if (k.tail && t.rest != 0.f) loss += t.rest * (logf(t.rest) - lt);
+    if (k.loss) k.loss[n] = (p.empty || !t.some) ? 0.f : loss;
+    if (k.norm) *reinterpret_cast<float2 *>(k.norm + 2 * n) = make_float2(p.ls != p.ls ? p.ls : M, p.ls);
+    if (k.log_tail) k.log_tail[n] = lt;
+}
+
+// ---- small: one lane a row ----------------------------------------------------------------------------------------------------
+template <typename T, int N, bool CONTIG>
+__device__ __forceinline__ void load_small(const T *z, long long sc, T (&v)[N]) {
+    if (CONTIG) {
+        __builtin_memcpy(&v, z, sizeof(v));
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = z[j * sc];
+    }
+}
+template <typename T, int N, bool BG, bool CONTIG>
+__global__ __launch_bounds__(256) void distill_small_kernel(const DistillK k) {
     const LogitsK &g = k.g;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, cats = g.C + g.bg;
-    const long long nw = (long long)gridDim.x * 4;
-    for (long long n = (long long)blockIdx.x * 4 + w; n < g.rows; n += nw) {
+    constexpr int CATS = N + BG;
+    const long long stride = (long long)gridDim.x * 256;
+    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < g.rows; n += stride) {
+        T raw[N];
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
-        const Teacher t = teacher_wave(k, n, lane, cats);
-        s_idx[w][lane] = t.idx;
-        wave_sync();
-        float M = kNegInf;
-        for (int j = lane; j < cats; j += 64) M = fmaxf(M, (g.bg && j == 0) ? 0.f : to_f32(z[(long long)(j - g.bg) * g.sc]));
-        M = wave_max(M);
-        float s = 0.f, st = 0.f;
-        for (int j = lane; j < cats; j += 64) {
-            const float v = (g.bg && j == 0) ? 0.f : to_f32(z[(long long)(j - g.bg) * g.sc]);
-            const float e = v == kNegInf ? 0.f : exp2_hw((v - M) * g.c2);
-            s += e;
-            if (k.tail) {
-                bool in = false;
-                for (int q = 0; q < k.K; ++q) in |= s_idx[w][q] == j;
-                if (!in) st += e;
-            }
+        load_small<T, N, CONTIG>(z, g.sc, raw);
+        const Teacher t = teacher_group<1>(k, n, 0, CATS);
+        float x[CATS];
+        if (BG) x[0] = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j + BG] = to_f32(raw[j]);
+        float M = x[0];
+#pragma unroll
+        for (int j = 1; j < CATS; ++j) M = maxn(M, x[j]);
+        const float ref = reference(M);
+        float e[CATS], s = 0.f, so = 0.f;
+#pragma unroll
+        for (int j = 0; j < CATS; ++j) {
+            e[j] = exp2_hw((x[j] - ref) * g.c2);
+            s += e[j];
         }
-        s = wave_sum(s);
-        st = wave_sum(st);
-        const bool empty = M == kNegInf && s == 0.f;
-        const float ls = logf(s), lt = logf(st) - ls;
-        float part = 0.f;
-        if (t.idx >= 0) {
-            const float v = (g.bg && t.idx == 0) ? 0.f : to_f32(z[(long long)(t.idx - g.bg) * g.sc]);
-            const float lp = (v - M) * g.invT - ls;
-            part = t.q == 0.f ? 0.f : t.q * (t.lq - lp);
+        const Student p = student_of(M, s);
+        unsigned in = 0u;
+        float loss = 0.f;
+        for (int q = 0; q < k.K; ++q) {
+            float v, zl = 0.f;
+            const int l = load_entry(k, n, q, CATS, v);
+            if (l < 0) continue;
+            in |= 1u << l;
+#pragma unroll
+            for (int j = 0; j < CATS; ++j) zl = l == j ? x[j] : zl;
+            loss += entry_loss(k, t, p, v, zl);
         }
-        float loss = wave_sum(part);
-        if (k.tail && t.rest != 0.f) loss += t.rest * (logf(t.rest) - lt);
-        if (lane == 0) {
-            if (k.loss) k.loss[n] = (empty || !t.any) ? 0.f : loss;
-            if (k.norm) {
-                k.norm[2 * n] = ls != ls ? ls : M;
-                k.norm[2 * n + 1] = ls;
-            }
-            if (k.log_tail) k.log_tail[n] = empty ? kNegInf : lt;
-        }
-        wave_sync();
+#pragma unroll
+        for (int j = 0; j < CATS; ++j) so += (in >> j) & 1u ? 0.f : e[j];
+        write_row(k, n, M, log_outside<1>(k, n, z, 0, CATS, p, t, so), p, t, loss);
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void distill_grad_wave_kernel(const DistillK k) {
-    __shared__ int s_idx[4][64];
-    __shared__ float s_q[4][64];
+// What a row's gradient needs: g_j = f (total p_j - [outside] rest p_j / p_t) for the others, f (total p_j - sum q) for an entry's label
+struct GradRow {
+    float M, l2s, total, share, f;  // share = q_t / p_t
+    bool zero;
+};
+__device__ __forceinline__ GradRow grad_row(const DistillK &k, long long n, const Teacher &t) {
+    GradRow r;
+    const float2 nm = *reinterpret_cast<const float2 *>(k.norm + 2 * n);
+    r.M = nm.x;
+    r.l2s = nm.y * kLog2e;
+    r.total = t.total;
+    // q_t / p_t reaches e^80 and more where the student leaves next to nothing outside: it is kept as a logarithm, in units of 2
+    r.share = (k.tail && t.rest != 0.f) ? __builtin_amdgcn_logf(t.rest) - k.log_tail[n] * kLog2e : kNegInf;
+    r.f = k.g_loss[n] * k.g.invT;
+    r.zero = nm.x == kNegInf || !t.some;
+    return r;
+}
+__device__ __forceinline__ float grad_outside(const GradRow &r, float c2, float v) {
+    const float d = (v - r.M) * c2 - r.l2s, p = exp2_hw(d);
+    const float o = v == kNegInf ? 0.f : exp2_hw(d + r.share);  // (the share of a row with nothing outside is infinite)
+    return r.zero ? 0.f : r.f * fmaf(r.total, p, -o);
+}
+__device__ __forceinline__ float grad_inside(const GradRow &r, float c2, float v, float qs) {
+    const float p = exp2_hw((v - r.M) * c2 - r.l2s);
+    return r.zero ? 0.f : r.f * fmaf(r.total, p, -qs);
+}
+
+template <typename T, int N, bool CONTIG>
+__global__ __launch_bounds__(256) void distill_grad_small_kernel(const DistillK k) {
     const LogitsK &g = k.g;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, cats = g.C + g.bg;
-    const long long nw = (long long)gridDim.x * 4;
-    for (long long n = (long long)blockIdx.x * 4 + w; n < g.rows; n += nw) {
+    const int cats = N + g.bg;
+    const long long stride = (long long)gridDim.x * 256;
+    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < g.rows; n += stride) {
+        T raw[N];
+        load_small<T, N, CONTIG>(static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si), g.sc, raw);
+        T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi);
+        const Teacher t = teacher_group<1>(k, n, 0, cats);
+        const GradRow r = grad_row(k, n, t);
+        unsigned in = 0u;
+        float qs[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) qs[j] = 0.f;
+        for (int q = 0; q < k.K; ++q) {
+            float v;
+            const int l = load_entry(k, n, q, cats, v) - g.bg;
+            const float w = weight(t, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (l == j) {
+                    qs[j] += w;
+                    in |= 1u << j;
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float v = to_f32(raw[j]);
+            raw[j] = from_f32<T>((in >> j) & 1u ? grad_inside(r, g.c2, v, qs[j]) : grad_outside(r, g.c2, v));
+        }
+        if (CONTIG) {
+            __builtin_memcpy(out, &raw, sizeof(raw));
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) out[j * k.gsc] = raw[j];
+        }
+    }
+}
+
+// ---- group: G lanes a row, 16 scores a lane ------------------------------------------------------------------------------------
+// The labels of the entries are marked in LDS, one 16-bit word for each lane's scores.
+template <int G, int V>
+__device__ __forceinline__ void mark(unsigned *bits, int c) {  // bits: the block's words, two lanes a word
+    const int vec = c / V, owner = (int)(threadIdx.x / G) * G + vec % G, bit = (vec / G) * V + c % V;
+    atomicOr(&bits[owner >> 1], 1u << ((owner & 1) * 16 + bit));
+}
+template <typename T, int G>
+__global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
+    __shared__ unsigned s_bits[128];
+    const LogitsK &g = k.g;
+    constexpr int V = kVec<T>, NV = 16 / V, ROWS = 256 / G;
+    const int gl = threadIdx.x % G, cats = g.C + g.bg;
+    for (long long n0 = (long long)blockIdx.x * ROWS; n0 < g.rows; n0 += (long long)gridDim.x * ROWS) {
+        const long long nr = n0 + threadIdx.x / G;
+        const bool live = nr < g.rows;
+        const long long n = live ? nr : g.rows - 1;
+        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
+        float x[17];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = (i * G + gl) * V;
+            const Vec<T> r = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[i * V + e] = to_f32(r.v[e]);
+        }
+        x[16] = (g.bg && gl == 0) ? 0.f : kNegInf;
+        unsigned in = 0u;
+        float back_in = 0.f;  // 1: the implicit category is an entry
+        if (k.tail) {
+            if ((threadIdx.x & 1) == 0) s_bits[threadIdx.x >> 1] = 0u;
+            wave_sync();
+            for (int q = gl; q < k.K; q += G) {
+                float v;
+                const int c = load_entry(k, n, q, cats, v) - g.bg;
+                if (c >= 0) mark<G, V>(s_bits, c);
+                else if (g.bg && c == -1) back_in = 1.f;
+            }
+            wave_sync();
+            in = s_bits[threadIdx.x >> 1] >> ((threadIdx.x & 1) * 16) & 0xffffu;
+            wave_sync();
+            // (an empty slot is -1 - bg: with the background it is -2, without it the flag is not read)
+            back_in = group_max<G>(back_in);
+        }
+        const Teacher t = teacher_group<G>(k, n, gl, cats);
+        float M = x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) M = maxn(M, x[i]);
+        M = group_max<G>(M);
+        const float ref = reference(M);
+        float e[16], eo[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            e[i] = exp2_hw((x[i] - ref) * g.c2);
+            eo[i] = (in >> i) & 1u ? 0.f : e[i];
+        }
+        const float eb = exp2_hw((x[16] - ref) * g.c2);
+        const float s = group_sum<G>(tree_sum(e) + eb);
+        const float so = k.tail ? group_sum<G>(tree_sum(eo) + (back_in > 0.f ? 0.f : eb)) : 0.f;
+        const Student p = student_of(M, s);
+        float loss = 0.f;
+        for (int q = gl; q < k.K; q += G) {
+            float v;
+            const int l = load_entry(k, n, q, cats, v);
+            if (l >= 0) loss += entry_loss(k, t, p, v, l < g.bg ? 0.f : to_f32(z[l - g.bg]));
+        }
+        loss = group_sum<G>(loss);
+        const float lso = log_outside<G>(k, n, z, gl, cats, p, t, so);
+        if (live && gl == 0) write_row(k, n, M, lso, p, t, loss);
+    }
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK k) {
+    __shared__ unsigned s_bits[128];
+    __shared__ T s_val[256 * 16];  // what an entry's lane has worked out for its label
+    const LogitsK &g = k.g;
+    constexpr int V = kVec<T>, NV = 16 / V, ROWS = 256 / G;
+    const int gl = threadIdx.x % G, cats = g.C + g.bg;
+    for (long long n0 = (long long)blockIdx.x * ROWS; n0 < g.rows; n0 += (long long)gridDim.x * ROWS) {
+        const long long nr = n0 + threadIdx.x / G;
+        const bool live = nr < g.rows;
+        const long long n = live ? nr : g.rows - 1;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
         T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi);
-        const Teacher t = teacher_wave(k, n, lane, cats);
-        s_idx[w][lane] = t.idx;
-        s_q[w][lane] = t.q;
+        Vec<T> x[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = (i * G + gl) * V;
+            x[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
+        }
+        const Teacher t = teacher_group<G>(k, n, gl, cats);
+        const GradRow r = grad_row(k, n, t);
+        if ((threadIdx.x & 1) == 0) s_bits[threadIdx.x >> 1] = 0u;
         wave_sync();
-        const float M = k.norm[2 * n], ls = k.norm[2 * n + 1];
-        const float f = k.g_loss[n] * g.invT;
-        const float lt = (k.tail && t.rest != 0.f) ? k.log_tail[n] : 0.f;
-        const bool zero = (M == kNegInf && !(ls != ls)) || !t.any;
-        for (int c = lane; c < g.C; c += 64) {
-            const float v = to_f32(z[(long long)c * g.sc]);
-            const float lp = (v - M) * g.invT - ls, p = exp2_hw(lp * kLog2e);
+        for (int q = gl; q < k.K; q += G) {
+            float v;
+            const int l = load_entry(k, n, q, cats, v), c = l - g.bg;
+            if (l < 0 || c < 0) continue;
+            // the same label twice: every one of its entries sums all of them, in the order of the entries, and writes the same value
             float qs = 0.f;
-            bool in = false;
-            for (int q = 0; q < k.K; ++q)
-                if (s_idx[w][q] == c + g.bg) {
-                    in = true;
-                    qs += s_q[w][q];
-                }
-            float r = t.total * p - qs;
-            if (!in && t.rest != 0.f && p != 0.f) r -= t.rest * exp2_hw((lp - lt) * kLog2e);
-            out[(long long)c * k.gsc] = from_f32<T>(zero ? 0.f : r * f);
+            for (int o = 0; o < k.K; ++o) {
+                float vo;
+                if (load_entry(k, n, o, cats, vo) == l) qs += weight(t, vo);
+            }
+            const int vec = c / V, owner = (int)(threadIdx.x / G) * G + vec % G, bit = (vec / G) * V + c % V;
+            s_val[owner * 16 + bit] = from_f32<T>(grad_inside(r, g.c2, to_f32(z[c]), qs));
+            mark<G, V>(s_bits, c);
+        }
+        wave_sync();
+        const unsigned in = s_bits[threadIdx.x >> 1] >> ((threadIdx.x & 1) * 16) & 0xffffu;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = (i * G + gl) * V;
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[i].v[e] = from_f32<T>(grad_outside(r, g.c2, to_f32(x[i].v[e])));
+            if ((in >> (i * V)) & ((1u << V) - 1u)) {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if ((in >> (i * V + e)) & 1u) x[i].v[e] = s_val[threadIdx.x * 16 + i * V + e];
+            }
+            if (!live) continue;
+            if (j + V <= g.C) __builtin_memcpy(out + j, &x[i], 16);
+            else store_part(out + j, x[i], g.C - j);
         }
         wave_sync();
     }
 }
 
-unsigned wave_grid(long long rows, int num_cu) {
-    long long b = (rows + 3) / 4;
-    const long long cap = (long long)num_cu * 32;
-    return (unsigned)(b < cap ? b : cap);
+// ---- block: four waves a segment of a row --------------------------------------------------------------------------------------
+// The tail's sum leaves the entries' labels out: a bit a score in LDS, looked up a vector at a time.
+constexpr int kSegWords = 65536 / 32;
+
+// wave 0, one entry a lane: the loss of a finished row
+template <typename T>
+__device__ __forceinline__ void finish_row(const DistillK &k, long long n, const T *z, float M, float s, float so) {
+    const int lane = threadIdx.x & 63, cats = k.g.C + k.g.bg;
+    const Teacher t = teacher_group<64>(k, n, lane, cats);
+    const Student p = student_of(M, s);
+    float loss = 0.f;
+    if (lane < k.K) {
+        float v;
+        const int l = load_entry(k, n, lane, cats, v);
+        if (l >= 0) loss = entry_loss(k, t, p, v, gather(k.g, z, l));
+    }
+    loss = group_sum<64>(loss);
+    const float lso = log_outside<64>(k, n, z, lane, cats, p, t, so);
+    if (lane == 0) write_row(k, n, M, lso, p, t, loss);
+}
+
+template <typename T, bool TAIL>
+__global__ __launch_bounds__(256) void distill_block_kernel(const DistillK k, const Cut cut) {
+    __shared__ RowStat s_stat[4];
+    __shared__ unsigned s_bits[TAIL ? kSegWords : 1];
+    __shared__ int s_back;
+    const LogitsK &g = k.g;
+    constexpr int V = kVec<T>, U = 16 / V, TILE = 64 * 16;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const long long work = g.rows * cut.segs;
+    for (long long item = blockIdx.x; item < work; item += gridDim.x) {
+        const long long n = cut.segs == 1 ? item : item / cut.segs;
+        const int seg = cut.segs == 1 ? 0 : (int)(item - n * cut.segs);
+        const int c0 = seg * cut.len, c1 = c0 + cut.len < g.C ? c0 + cut.len : g.C;
+        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
+        Vec<T> nx[U];
+        auto fetch = [&](int c) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = c + u * 64 * V + lane * V;
+                nx[u] = j + V <= c1 ? load_vec(z + j) : load_part(z + j, c1 - j);
+            }
+        };
+        int c = c0 + w * TILE;
+        if (c < c1) fetch(c);
+        if (TAIL) {
+            for (int i = threadIdx.x; i < (c1 - c0 + 31) / 32; i += 256) s_bits[i] = 0u;
+            if (threadIdx.x == 0) s_back = 0;
+            __syncthreads();
+            if ((int)threadIdx.x < k.K) {
+                float v;
+                const int l = load_entry(k, n, threadIdx.x, g.C + g.bg, v), j = l - g.bg - c0;
+                if (l >= 0 && l < g.bg) s_back = 1;
+                else if (l >= 0 && j >= 0 && j < c1 - c0) atomicOr(&s_bits[j >> 5], 1u << (j & 31));
+            }
+            __syncthreads();
+        }
+        // t holds the sum outside the entries here
+        RowStat r = no_stat();
+        if (g.bg && seg == 0 && threadIdx.x == 0) r = {0.f, 0.f, 1.f, (TAIL && s_back) ? 0.f : 1.f};
+        for (; c < c1; c += 4 * TILE) {
+            Vec<T> now[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) now[u] = nx[u];
+            if (c + 4 * TILE < c1) fetch(c + 4 * TILE);
+            float x[16], cm = kNegInf;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                x[i] = to_f32(now[i / V].v[i % V]);
+                cm = maxn(cm, x[i]);
+            }
+            r.m = maxn(r.m, cm);
+            if ((cm - r.ref) * g.c2 > kSlack) {
+                const float f = exp2_hw(maxn((r.ref - cm) * g.c2, -1.0e4f));
+                r.s *= f;
+                r.t *= f;
+                r.ref = cm;
+            }
+            float e[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) e[i] = exp2_hw((x[i] - r.ref) * g.c2);
+            const float sum = tree_sum(e);
+            r.s += sum;
+            if (TAIL) {
+                unsigned in = 0u;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int j = c + u * 64 * V + lane * V - c0;
+                    in |= (j < c1 - c0 ? s_bits[j >> 5] >> (j & 31) & ((1u << V) - 1u) : 0u) << (u * V);
+                }
+                if (in) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) e[i] = (in >> i) & 1u ? 0.f : e[i];
+                    r.t += tree_sum(e);
+                } else {
+                    r.t += sum;
+                }
+            }
+        }
+        {
+            const float M = group_max<64>(r.m), ref = reference(M);
+            const float f = r.ref == ref ? 1.f : exp2_hw(maxn((r.ref - ref) * g.c2, -1.0e4f));
+            r = {M, ref, group_sum<64>(r.s * f), TAIL ? group_sum<64>(r.t * f) : 0.f};
+        }
+        if (lane == 0) s_stat[w] = r;
+        __syncthreads();
+        if (w == 0) {
+            const float M = maxn(maxn(s_stat[0].m, s_stat[1].m), maxn(s_stat[2].m, s_stat[3].m)), ref = reference(M);
+            float s = 0.f, so = 0.f;
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+                const float f = s_stat[o].ref == ref ? 1.f : exp2_hw(maxn((s_stat[o].ref - ref) * g.c2, -1.0e4f));
+                s += s_stat[o].s * f;
+                so += s_stat[o].t * f;
+            }
+            if (cut.segs > 1) {
+                if (lane == 0) static_cast<float4 *>(k.ws)[item] = make_float4(M, s, so, 0.f);
+            } else {
+                finish_row(k, n, z, M, s, so);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// The segments' parts of a row together: one wave a row.
+template <typename T>
+__global__ __launch_bounds__(64) void distill_join_kernel(const DistillK k, const Cut cut) {
+    const LogitsK &g = k.g;
+    for (long long n = blockIdx.x; n < g.rows; n += gridDim.x) {
+        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
+        const float4 *p = static_cast<const float4 *>(k.ws) + n * cut.segs;
+        float m = kNegInf;
+        for (int q = threadIdx.x; q < cut.segs; q += 64) m = maxn(m, p[q].x);
+        const float M = group_max<64>(m), ref = reference(M);
+        float s = 0.f, so = 0.f;
+        for (int q = threadIdx.x; q < cut.segs; q += 64) {
+            const float4 a = p[q];
+            const float r = reference(a.x), f = r == ref ? 1.f : exp2_hw(maxn((r - ref) * g.c2, -1.0e4f));
+            s += a.y * f;
+            so += a.z * f;
+        }
+        finish_row(k, n, z, M, group_sum<64>(s), group_sum<64>(so));
+    }
+}
+
+// A block takes 256 lanes x 16 scores of a row at a time.  The entries' labels are marked as above; the few vectors that hold one
+// look it up among the entries.
+template <typename T>
+__global__ __launch_bounds__(256) void distill_grad_block_kernel(const DistillK k, long long tiles) {
+    constexpr int V = kVec<T>, NV = 16 / V, TILE = 256 * 16;
+    __shared__ unsigned s_bits[TILE / 32];
+    __shared__ int s_l[64];
+    __shared__ float s_q[64];
+    __shared__ GradRow s_row;
+    const LogitsK &g = k.g;
+    for (long long item = blockIdx.x; item < g.rows * tiles; item += gridDim.x) {
+        const long long n = item / tiles;
+        const int c0 = (int)(item - n * tiles) * TILE;
+        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
+        T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi);
+        Vec<T> x[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = c0 + (i * 256 + threadIdx.x) * V;
+            x[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
+        }
+        if (threadIdx.x < TILE / 32) s_bits[threadIdx.x] = 0u;
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const int lane = threadIdx.x;
+            const Teacher t = teacher_group<64>(k, n, lane, g.C + g.bg);
+            float v = 0.f;
+            const int l = lane < k.K ? load_entry(k, n, lane, g.C + g.bg, v) : -1, c = l - g.bg;
+            s_l[lane] = l < 0 ? -1 : c;
+            s_q[lane] = l < 0 ? 0.f : weight(t, v);
+            if (l >= 0 && c >= c0 && c < c0 + TILE) atomicOr(&s_bits[(c - c0) >> 5], 1u << ((c - c0) & 31));
+            const GradRow r = grad_row(k, n, t);
+            if (lane == 0) s_row = r;
+        }
+        __syncthreads();
+        const GradRow r = s_row;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = c0 + (i * 256 + threadIdx.x) * V;
+            const unsigned in = s_bits[(j - c0) >> 5] >> ((j - c0) & 31) & ((1u << V) - 1u);
+            Vec<T> y;
+#pragma unroll
+            for (int e = 0; e < V; ++e) y.v[e] = from_f32<T>(grad_outside(r, g.c2, to_f32(x[i].v[e])));
+            if (in) {
+                for (int q = 0; q < k.K; ++q) {
+                    const int at = s_l[q] - j;
+                    if (s_l[q] < 0 || at < 0 || at >= V) continue;
+                    float qs = 0.f;  // (the same label twice: each time the sum of all its entries, in their order)
+                    for (int o = 0; o < k.K; ++o) qs += s_l[o] == s_l[q] ? s_q[o] : 0.f;
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (e == at) y.v[e] = from_f32<T>(grad_inside(r, g.c2, to_f32(x[i].v[e]), qs));
+                }
+            }
+            if (j + V <= g.C) __builtin_memcpy(out + j, &y, 16);
+            else store_part(out + j, y, g.C - j);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- planes: one lane a row, more than 8 classes that do not lie together ------------------------------------------------------
+// Which of the 32 categories from c are entries: the row's labels are read again for each 32 (they stay in the caches).
+__device__ __forceinline__ unsigned marks(const DistillK &k, long long n, int c, int cats) {
+    unsigned in = 0u;
+    for (int q = 0; q < k.K; ++q) {
+        const long long l = load_label(k.labels, k.l_kind, n * k.K + q) - c;
+        if (l >= 0 && l < 32 && l + c < cats) in |= 1u << (int)l;
+    }
+    return in;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void distill_planes_kernel(const DistillK k) {
+    const LogitsK &g = k.g;
+    const int cats = g.C + g.bg;
+    const long long stride = (long long)gridDim.x * 256;
+    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < g.rows; n += stride) {
+        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
+        RowStat r = no_stat();  // (t: the sum outside the entries)
+        for (int c0 = 0; c0 < cats; c0 += 32) {
+            const unsigned in = k.tail ? marks(k, n, c0, cats) : 0u;
+#pragma unroll
+            for (int i0 = 0; i0 < 32; i0 += 8) {
+                if (c0 + i0 >= cats) break;
+                float x[8], cm = kNegInf;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int j = c0 + i0 + i;
+                    x[i] = j >= cats ? kNegInf : j < g.bg ? 0.f : to_f32(z[(long long)(j - g.bg) * g.sc]);
+                    cm = maxn(cm, x[i]);
+                }
+                r.m = maxn(r.m, cm);
+                if ((cm - r.ref) * g.c2 > kSlack) {
+                    const float f = exp2_hw(maxn((r.ref - cm) * g.c2, -1.0e4f));
+                    r.s *= f;
+                    r.t *= f;
+                    r.ref = cm;
+                }
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = exp2_hw((x[i] - r.ref) * g.c2);
+                r.s += tree_sum(e);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = (in >> (i0 + i)) & 1u ? 0.f : e[i];
+                r.t += tree_sum(e);
+            }
+        }
+        const float ref = reference(r.m), f = r.ref == ref ? 1.f : exp2_hw(maxn((r.ref - ref) * g.c2, -1.0e4f));
+        const Student p = student_of(r.m, r.s * f);
+        const Teacher t = teacher_group<1>(k, n, 0, cats);
+        float loss = 0.f;
+        for (int q = 0; q < k.K; ++q) {
+            float v;
+            const int l = load_entry(k, n, q, cats, v);
+            if (l >= 0) loss += entry_loss(k, t, p, v, gather(g, z, l));
+        }
+        write_row(k, n, r.m, log_outside<1>(k, n, z, 0, cats, p, t, r.t * f), p, t, loss);
+    }
+}
+
+// The same with too few rows for a lane each: a wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void distill_wave_kernel(const DistillK k) {
+    __shared__ int s_l[4][64];
+    const LogitsK &g = k.g;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, cats = g.C + g.bg;
+    for (long long n = (long long)blockIdx.x * 4 + w; n < g.rows; n += (long long)gridDim.x * 4) {
+        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
+        float v;
+        s_l[w][lane] = lane < k.K ? load_entry(k, n, lane, cats, v) : -1;
+        wave_sync();
+        RowStat r = no_stat();
+        for (int j0 = 0; j0 < cats; j0 += 256) {
+            float x[4], cm = kNegInf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = j0 + i * 64 + lane;
+                x[i] = j < cats ? gather(g, z, j) : kNegInf;
+                cm = maxn(cm, x[i]);
+            }
+            r.m = maxn(r.m, cm);
+            if ((cm - r.ref) * g.c2 > kSlack) {
+                const float f = exp2_hw(maxn((r.ref - cm) * g.c2, -1.0e4f));
+                r.s *= f;
+                r.t *= f;
+                r.ref = cm;
+            }
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = exp2_hw((x[i] - r.ref) * g.c2);
+            r.s += tree_sum(e);
+            if (k.tail) {
+                for (int q = 0; q < k.K; ++q) {
+                    const int at = s_l[w][q] - j0 - lane;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[i] = at == i * 64 ? 0.f : e[i];
+                }
+                r.t += tree_sum(e);
+            }
+        }
+        const float M = group_max<64>(r.m), ref = reference(M);
+        const float f = r.ref == ref ? 1.f : exp2_hw(maxn((r.ref - ref) * g.c2, -1.0e4f));
+        finish_row(k, n, z, M, group_sum<64>(r.s * f), group_sum<64>(r.t * f));
+        wave_sync();
+    }
+}
+
+// a block 256 rows and 32 classes
+template <typename T>
+__global__ __launch_bounds__(256) void distill_grad_planes_kernel(const DistillK k, int parts) {
+    const LogitsK &g = k.g;
+    const int cats = g.C + g.bg;
+    const long long blocks = (g.rows + 255) / 256;
+    for (long long item = blockIdx.x; item < blocks * parts; item += gridDim.x) {
+        const long long rb = item / parts;
+        const int c0 = (int)(item - rb * parts) * 32, c1 = c0 + 32 < g.C ? c0 + 32 : g.C;
+        const long long n = rb * 256 + threadIdx.x;
+        if (n >= g.rows) continue;
+        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
+        T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi);
+        const Teacher t = teacher_group<1>(k, n, 0, cats);
+        const GradRow r = grad_row(k, n, t);
+        const unsigned in = marks(k, n, c0 + g.bg, cats);
+#pragma unroll
+        for (int i0 = 0; i0 < 32; i0 += 8) {
+            const int c = c0 + i0;
+            if (c >= c1) break;
+            T raw[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < c1) raw[i] = z[(long long)(c + i) * g.sc];
+            float qs[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) qs[i] = 0.f;
+            if ((in >> i0) & 0xffu) {
+                for (int q = 0; q < k.K; ++q) {
+                    float v;
+                    const int at = load_entry(k, n, q, cats, v) - g.bg - c;
+                    const float wq = weight(t, v);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) qs[i] += at == i ? wq : 0.f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < c1) {
+                    const float v = to_f32(raw[i]);
+                    out[(long long)(c + i) * k.gsc] =
+                        from_f32<T>((in >> (i0 + i)) & 1u ? grad_inside(r, g.c2, v, qs[i]) : grad_outside(r, g.c2, v));
+                }
+        }
+    }
+}
+
+// ---- dispatch ------------------------------------------------------------------------------------------------------------------
+unsigned grid_of(long long blocks, int num_cu, int per_cu) {
+    const long long cap = (long long)num_cu * per_cu;
+    return (unsigned)(blocks < 1 ? 1 : blocks < cap ? blocks : cap);
+}
+bool contiguous(const LogitsK &g) { return g.sc == 1 || g.C == 1; }
+
+template <typename T, int N>
+void small(const DistillK &k, bool contig, int num_cu, hipStream_t st) {
+    const dim3 grid(grid_of((k.g.rows + 255) / 256, num_cu, 64)), block(256);
+    if (contig) {
+        if (k.g.bg) hipLaunchKernelGGL((distill_small_kernel<T, N, true, true>), grid, block, 0, st, k);
+        else hipLaunchKernelGGL((distill_small_kernel<T, N, false, true>), grid, block, 0, st, k);
+    } else {
+        if (k.g.bg) hipLaunchKernelGGL((distill_small_kernel<T, N, true, false>), grid, block, 0, st, k);
+        else hipLaunchKernelGGL((distill_small_kernel<T, N, false, false>), grid, block, 0, st, k);
+    }
+}
+template <typename T, int N>
+void small_grad(const DistillK &k, bool contig, int num_cu, hipStream_t st) {
+    const dim3 grid(grid_of((k.g.rows + 255) / 256, num_cu, 64)), block(256);
+    if (contig) hipLaunchKernelGGL((distill_grad_small_kernel<T, N, true>), grid, block, 0, st, k);
+    else hipLaunchKernelGGL((distill_grad_small_kernel<T, N, false>), grid, block, 0, st, k);
+}
+template <typename T, int G>
+void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
+    const dim3 grid(grid_of((k.g.rows + 256 / G - 1) / (256 / G), num_cu, 64)), block(256);
+    if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G>), grid, block, 0, st, k);
+    else hipLaunchKernelGGL((distill_group_kernel<T, G>), grid, block, 0, st, k);
+}
+
+template <typename T>
+void launch(const DistillK &k, int num_cu, hipStream_t st) {
+    const LogitsK &g = k.g;
+    const bool contig = contiguous(g);
+    if (g.C <= 8) {
+        switch (g.C) {
+            case 1: return small<T, 1>(k, contig, num_cu, st);
+            case 2: return small<T, 2>(k, contig, num_cu, st);
+            case 3: return small<T, 3>(k, contig, num_cu, st);
+            case 4: return small<T, 4>(k, contig, num_cu, st);
+            case 5: return small<T, 5>(k, contig, num_cu, st);
+            case 6: return small<T, 6>(k, contig, num_cu, st);
+            case 7: return small<T, 7>(k, contig, num_cu, st);
+            default: return small<T, 8>(k, contig, num_cu, st);
+        }
+    }
+    if (!contig) {
+        // (as in label_scores.hip: a lane a row from 64 rows a compute unit on, or where rows are short)
+        if (g.C <= 64 || g.rows >= 64ll * num_cu)
+            hipLaunchKernelGGL(distill_planes_kernel<T>, dim3(grid_of((g.rows + 255) / 256, num_cu, 64)), dim3(256), 0, st, k);
+        else
+            hipLaunchKernelGGL(distill_wave_kernel<T>, dim3(grid_of((g.rows + 3) / 4, num_cu, 32)), dim3(256), 0, st, k);
+        return;
+    }
+    if (g.C <= 32) return group<T, 2>(k, false, num_cu, st);
+    if (g.C <= 64) return group<T, 4>(k, false, num_cu, st);
+    if (g.C <= 128) return group<T, 8>(k, false, num_cu, st);
+    if (g.C <= 256) return group<T, 16>(k, false, num_cu, st);
+    if (g.C <= 512) return group<T, 32>(k, false, num_cu, st);
+    if (g.C <= 1024) return group<T, 64>(k, false, num_cu, st);
+    const Cut cut = cut_rows(g, num_cu);
+    const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
+    if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true>), grid, dim3(256), 0, st, k, cut);
+    else hipLaunchKernelGGL((distill_block_kernel<T, false>), grid, dim3(256), 0, st, k, cut);
+    if (cut.segs > 1) hipLaunchKernelGGL(distill_join_kernel<T>, dim3(grid_of(g.rows, num_cu, 64)), dim3(64), 0, st, k, cut);
+}
+
+template <typename T>
+void launch_grad(const DistillK &k, int num_cu, hipStream_t st) {
+    const LogitsK &g = k.g;
+    const bool contig = contiguous(g) && (k.gsc == 1 || g.C == 1);
+    if (g.C <= 8) {
+        switch (g.C) {
+            case 1: return small_grad<T, 1>(k, contig, num_cu, st);
+            case 2: return small_grad<T, 2>(k, contig, num_cu, st);
+            case 3: return small_grad<T, 3>(k, contig, num_cu, st);
+            case 4: return small_grad<T, 4>(k, contig, num_cu, st);
+            case 5: return small_grad<T, 5>(k, contig, num_cu, st);
+            case 6: return small_grad<T, 6>(k, contig, num_cu, st);
+            case 7: return small_grad<T, 7>(k, contig, num_cu, st);
+            default: return small_grad<T, 8>(k, contig, num_cu, st);
+        }
+    }
+    if (!contig) {
+        const int parts = (g.C + 31) / 32;
+        hipLaunchKernelGGL(distill_grad_planes_kernel<T>, dim3(grid_of((g.rows + 255) / 256 * parts, num_cu, 64)), dim3(256), 0, st, k, parts);
+        return;
+    }
+    if (g.C <= 32) return group<T, 2>(k, true, num_cu, st);
+    if (g.C <= 64) return group<T, 4>(k, true, num_cu, st);
+    if (g.C <= 128) return group<T, 8>(k, true, num_cu, st);
+    if (g.C <= 256) return group<T, 16>(k, true, num_cu, st);
+    if (g.C <= 512) return group<T, 32>(k, true, num_cu, st);
+    if (g.C <= 1024) return group<T, 64>(k, true, num_cu, st);
+    const long long tiles = (g.C + 4095) / 4096;
+    hipLaunchKernelGGL(distill_grad_block_kernel<T>, dim3(grid_of(g.rows * tiles, num_cu, 256)), dim3(256), 0, st, k, tiles);
 }
 
 }  // namespace
 
-size_t distill_workspace_bytes(const DistillK &, int, int) { return 0; }
+size_t distill_workspace_bytes(const DistillK &k, int, int num_cu) {
+    if (k.g.C <= 1024 || !contiguous(k.g)) return 0;
+    const Cut cut = cut_rows(k.g, num_cu);
+    return cut.segs > 1 ? (size_t)k.g.rows * cut.segs * 16 : 0;
+}
 
 hipError_t distill_launch(const DistillK &k, int dtype, int num_cu, hipStream_t st) {
     (void)hipGetLastError();
-    const dim3 g(wave_grid(k.g.rows, num_cu)), b(256);
-    if (dtype == QMRI_F32) hipLaunchKernelGGL(distill_wave_kernel<float>, g, b, 0, st, k);
-    else if (dtype == QMRI_F16) hipLaunchKernelGGL(distill_wave_kernel<f16_t>, g, b, 0, st, k);
-    else hipLaunchKernelGGL(distill_wave_kernel<bf16_t>, g, b, 0, st, k);
+    if (dtype == QMRI_F32) launch<float>(k, num_cu, st);
+    else if (dtype == QMRI_F16) launch<f16_t>(k, num_cu, st);
+    else launch<bf16_t>(k, num_cu, st);
     return hipGetLastError();
 }
 
 hipError_t distill_grad_launch(const DistillK &k, int dtype, int num_cu, hipStream_t st) {
     (void)hipGetLastError();
-    const dim3 g(wave_grid(k.g.rows, num_cu)), b(256);
-    if (dtype == QMRI_F32) hipLaunchKernelGGL(distill_grad_wave_kernel<float>, g, b, 0, st, k);
-    else if (dtype == QMRI_F16) hipLaunchKernelGGL(distill_grad_wave_kernel<f16_t>, g, b, 0, st, k);
-    else hipLaunchKernelGGL(distill_grad_wave_kernel<bf16_t>, g, b, 0, st, k);
+    if (dtype == QMRI_F32) launch_grad<float>(k, num_cu, st);
+    else if (dtype == QMRI_F16) launch_grad<f16_t>(k, num_cu, st);
+    else launch_grad<bf16_t>(k, num_cu, st);
     return hipGetLastError();
 }
 

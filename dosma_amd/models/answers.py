@@ -24,9 +24,11 @@ from dosma_amd import _hostpool, _lib
 __all__ = ["LabelScores", "DistillLoss", "label_scores", "label_scores_grad", "distill_loss", "distill_loss_grad"]
 
 #: ``log_prob`` (None without labels), ``entropy`` in nats, ``norm`` (..., 2): the row maximum M and ln sum exp((z - M) / T),
-#: which the gradient needs (M / T + norm[..., 1] is log sum exp(z / T)); ``top_log_prob`` / ``top_label`` (..., top) or None
+#: which the gradient needs (M / T + norm[..., 1] is log sum exp(z / T)); None unless asked for; ``top_log_prob`` / ``top_label``
+#: (..., top) or None
 LabelScores = namedtuple("LabelScores", "log_prob entropy norm top_log_prob top_label")
-#: ``loss`` in nats, ``norm`` as above, ``log_tail``: log probability outside the teacher's entries (None without the tail)
+#: ``loss`` in nats, ``norm`` as above, ``log_tail``: log probability outside the teacher's entries (None without the tail); both
+#: None unless ``norm`` is asked for
 DistillLoss = namedtuple("DistillLoss", "loss norm log_tail")
 
 
@@ -129,11 +131,11 @@ class _TorchCall:
         return {"device": self.device.index, "stream": self.stream}
 
 
-def _scores_tensor(x, labels, dim, top, temperature, background, ignore_label):
+def _scores_tensor(x, labels, dim, top, norm, temperature, background, ignore_label):
     x, dim, shape, rows = _tensor_logits(x, dim)
     call = _TorchCall(x)
     lab = None if labels is None else _tensor_arg("labels", labels, shape, x.device, _lib.L_KINDS)
-    out = LabelScores(None if lab is None else call.empty(shape), call.empty(shape), call.empty(shape + (2,)),
+    out = LabelScores(None if lab is None else call.empty(shape), call.empty(shape), call.empty(shape + (2,)) if norm else None,
                       call.empty(shape + (top,)) if top > 0 else None, call.empty(shape + (top,), "int32") if top > 0 else None)
     ptr = [None if t is None else t.data_ptr() for t in out]
     _lib.label_scores(x.data_ptr(), _name(x.dtype), rows, labels_ptr=None if lab is None else lab.data_ptr(),
@@ -160,14 +162,15 @@ def _scores_grad_tensor(x, labels, norm, grad_log_prob, entropy, grad_entropy, d
     return grad
 
 
-def _distill_tensor(x, top_label, values, dim, temperature, tail, background):
+def _distill_tensor(x, top_label, values, dim, norm, temperature, tail, background):
     x, dim, shape, rows = _tensor_logits(x, dim)
     call = _TorchCall(x)
     lab, val, K = _teacher_tensors(top_label, values, shape, x.device)
-    out = DistillLoss(call.empty(shape), call.empty(shape + (2,)), call.empty(shape) if tail else None)
+    out = DistillLoss(call.empty(shape), call.empty(shape + (2,)) if norm else None, call.empty(shape) if norm and tail else None)
+    ptr = [None if t is None else t.data_ptr() for t in out]
     _lib.distill(x.data_ptr(), _name(x.dtype), rows, lab.data_ptr(), _name(lab.dtype), val.data_ptr(), _name(val.dtype), K,
-                 tail=tail, temperature=temperature, background=background, loss=out.loss.data_ptr(), norm=out.norm.data_ptr(),
-                 log_tail=out.log_tail.data_ptr() if tail else None, workspace=call.workspace, **call.kw())
+                 tail=tail, temperature=temperature, background=background, loss=ptr[0], norm=ptr[1], log_tail=ptr[2],
+                 workspace=call.workspace, **call.kw())
     return out
 
 
@@ -204,7 +207,7 @@ def _autograd(name):
         class ScoresFunction(torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, labels, kw, top):
-                r = _scores_tensor(x, labels, top=top, **kw)
+                r = _scores_tensor(x, labels, top=top, norm=True, **kw)
                 ctx.kw = kw
                 ctx.set_materialize_grads(False)
                 ctx.mark_non_differentiable(*[t for t in r[2:] if t is not None])
@@ -222,7 +225,7 @@ def _autograd(name):
         class DistillFunction(torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, top_label, values, kw):
-                r = _distill_tensor(x, top_label, values, **kw)
+                r = _distill_tensor(x, top_label, values, norm=True, **kw)
                 ctx.kw = kw
                 ctx.set_materialize_grads(False)
                 ctx.mark_non_differentiable(*[t for t in r[1:] if t is not None])
@@ -275,11 +278,12 @@ def _address(a):
     return None if a is None else a.ctypes.data
 
 
-def _scores_array(x, labels, dim, top, temperature, background, ignore_label, device):
+def _scores_array(x, labels, dim, top, norm, temperature, background, ignore_label, device):
     x, dim, shape, rows = _array_logits(x, dim)
     lab = None if labels is None else _array_arg("labels", labels, shape, _lib.L_KINDS)
     out = LabelScores(None if lab is None else _hostpool.empty(shape, np.float32), _hostpool.empty(shape, np.float32),
-                      _hostpool.empty(shape + (2,), np.float32), _hostpool.empty(shape + (top,), np.float32) if top > 0 else None,
+                      _hostpool.empty(shape + (2,), np.float32) if norm else None,
+                      _hostpool.empty(shape + (top,), np.float32) if top > 0 else None,
                       _hostpool.empty(shape + (top,), np.int32) if top > 0 else None)
     ptr = [_address(a) for a in out]
     _lib.label_scores(_address(x), x.dtype.name, rows, labels_ptr=_address(lab), l_dtype=None if lab is None else lab.dtype.name,
@@ -288,22 +292,24 @@ def _scores_array(x, labels, dim, top, temperature, background, ignore_label, de
     return out
 
 
-def label_scores(logits, labels=None, *, dim=-1, top=0, temperature=1.0, background=False, ignore_label=-1, device=None):
+def label_scores(logits, labels=None, *, dim=-1, top=0, norm=False, temperature=1.0, background=False, ignore_label=-1,
+                 device=None):
     """Log probability of the given ``labels``, entropy and the ``top`` best categories of every row -> :class:`LabelScores`.
 
     ``labels``: int32 / uint8 / int16 / int64 categories; rows with ``ignore_label`` have none (log_prob 0), any other value
     that is not a category gives NaN.  ``top`` (0 .. 64, at most the number of categories): alternatives in falling order,
-    ties to the lower category; label -1 with log probability -inf where fewer are offered.  Tensors that require gradients:
-    ``log_prob`` and ``entropy`` are differentiable (first order), the alternatives are not.  ``device``: of numpy calls."""
+    ties to the lower category; label -1 with log probability -inf where fewer are offered.  ``norm=True``: also what
+    :func:`label_scores_grad` needs.  Tensors that require gradients: ``log_prob`` and ``entropy`` are differentiable (first
+    order), the alternatives are not.  ``device``: of numpy calls."""
     top = int(top)
     if not 0 <= top <= _lib.MAX_TOP:
         raise ValueError(f"top must be 0 .. {_lib.MAX_TOP}, got {top}")
     kw = dict(dim=dim, temperature=temperature, background=background, ignore_label=ignore_label)
     if not _is_torch(logits):
-        return _scores_array(logits, labels, top=top, device=device, **kw)
+        return _scores_array(logits, labels, top=top, norm=norm, device=device, **kw)
     if _wants_grad(logits):
         return LabelScores(*_autograd("scores").apply(logits, labels, kw, top))
-    return _scores_tensor(logits, labels, top=top, **kw)
+    return _scores_tensor(logits, labels, top=top, norm=norm, **kw)
 
 
 def label_scores_grad(logits, labels, norm, *, grad_log_prob=None, entropy=None, grad_entropy=None, dim=-1, temperature=1.0,
@@ -336,23 +342,24 @@ def _teacher_arrays(top_label, values, shape, tail):
     return _array_arg("top_label", top_label, shape, ("int32", "int64"), K), _array_arg("values", values, shape, _lib.SCORE_DTYPES, K), K
 
 
-def distill_loss(logits, top_label, values, *, dim=-1, temperature=1.0, tail=False, background=False, device=None):
+def distill_loss(logits, top_label, values, *, dim=-1, norm=False, temperature=1.0, tail=False, background=False, device=None):
     """Divergence (nats, per row) of the answers ``logits`` from a teacher's best ones -> :class:`DistillLoss`.
 
     ``top_label`` (..., K) int32 / int64 and ``values`` (..., K), K <= 64, are the teacher's categories and either its scores
     or log probabilities (``tail=False``: the teacher is ``softmax(values / temperature)`` over the entries) or float32 log
     probabilities at this ``temperature`` (``tail=True``: the rest of its mass is compared with the student's mass outside the
     entries) -- what ``label_scores(teacher, top=K, temperature=...)`` returns.  Entries whose label is not a category (-1) are
-    empty slots; a row of empty slots has loss 0.  ``loss`` is differentiable (first order) in the student's logits."""
+    empty slots; a row of empty slots has loss 0.  ``norm=True``: also what :func:`distill_loss_grad` needs.  ``loss`` is
+    differentiable (first order) in the student's logits."""
     kw = dict(dim=dim, temperature=temperature, tail=bool(tail), background=background)
     if _is_torch(logits):
         if _wants_grad(logits):
             return DistillLoss(*_autograd("distill").apply(logits, top_label, values, kw))
-        return _distill_tensor(logits, top_label, values, **kw)
+        return _distill_tensor(logits, top_label, values, norm=norm, **kw)
     x, dim, shape, rows = _array_logits(logits, dim)
     lab, val, K = _teacher_arrays(top_label, values, shape, tail)
-    out = DistillLoss(_hostpool.empty(shape, np.float32), _hostpool.empty(shape + (2,), np.float32),
-                      _hostpool.empty(shape, np.float32) if tail else None)
+    out = DistillLoss(_hostpool.empty(shape, np.float32), _hostpool.empty(shape + (2,), np.float32) if norm else None,
+                      _hostpool.empty(shape, np.float32) if norm and tail else None)
     _lib.distill(_address(x), x.dtype.name, rows, _address(lab), lab.dtype.name, _address(val), val.dtype.name, K, tail=tail,
                  temperature=temperature, background=background, loss=_address(out.loss), norm=_address(out.norm),
                  log_tail=_address(out.log_tail), host=True, device=device)

@@ -136,7 +136,7 @@ def _check_scores(z, dtype, layout, rng, T=1.0, top=0, bg=False, label_type="int
         if cats < 250 and rows > 3:
             labels[3] = cats + 1  # out of range
     lab = torch.from_numpy(labels.astype(label_type)).reshape(_rowshape(t, dim)).cuda()
-    r = A.label_scores(t, lab, dim=dim, top=top, temperature=T, background=bg, ignore_label=ignore)
+    r = A.label_scores(t, lab, dim=dim, top=top, norm=True, temperature=T, background=bg, ignore_label=ignore)
     want = ao.scores(full, T, labels, top, ignore)
     ls = want["norm"][:, 1]
     _same(_host(r.log_prob).reshape(-1), want["log_prob"], _tol_lp(want["lp"], ls, want["log_prob"]), "log_prob")
@@ -215,7 +215,7 @@ def _check_distill(z, dtype, layout, rng, K, T=1.0, tail=False, bg=False, index_
     ti = torch.from_numpy(idx.astype(index_type)).reshape(shp).cuda()
     tv = val.reshape(shp).cuda()
     w = rng.uniform(-2, 2, rows).astype(np.float32)
-    r = A.distill_loss(t, ti, tv, dim=dim, temperature=T, tail=tail, background=bg)
+    r = A.distill_loss(t, ti, tv, dim=dim, norm=True, temperature=T, tail=tail, background=bg)
     want = ao.distill(full, idx, val.double().numpy(), T, tail, w.astype(float))
     lp, M, ls = ao.log_softmax(full, T)
     base = _tol_ls(lp, ls)
@@ -404,7 +404,7 @@ def test_distill_special(C):
         for layout in ("rows", "planes"):
             t, dim, held = _tensor(z, "float32", layout, rng)
             ti, tv = torch.from_numpy(idx).cuda(), torch.from_numpy(val.astype(np.float32)).cuda()
-            r = A.distill_loss(t, ti, tv, dim=dim, tail=tail)
+            r = A.distill_loss(t, ti, tv, dim=dim, norm=True, tail=tail)
             want = ao.distill(held, idx, val.astype(np.float32).astype(float), 1.0, tail, np.ones(8))
             got = _host(r.loss)
             assert np.isnan(got[2]) and got[0] == 0 and got[4] == 0 and np.isposinf(got[1])
@@ -420,6 +420,27 @@ def test_distill_special(C):
             fin = np.isfinite(want["grad"]).all(-1)
             fin[2] = False
             assert np.allclose(g[fin], want["grad"][fin], rtol=0, atol=(C / 64 + 100) * U * 8)
+
+
+def test_a_sure_student_keeps_its_small_tail():
+    """The student leaves e^-150 outside the entries: the sum out there is taken relative to its own largest term."""
+    torch = torch_()
+    for C, layout in ((6, "rows"), (5, "planes"), (100, "rows"), (40, "planes"), (3000, "rows"), (200000, "rows"), (3000, "planes")):
+        rng = np.random.default_rng(C)
+        z = rng.standard_normal((3, C))
+        z[:, 2] += 150.0
+        t, dim, held = _tensor(z, "float32", layout, rng)
+        idx = np.tile(np.array([[2]]), (3, 1))
+        val = np.log(np.full((3, 1), 0.75)).astype(np.float32)
+        ti, tv = torch.from_numpy(idx).cuda(), torch.from_numpy(val).cuda()
+        r = A.distill_loss(t, ti, tv, dim=dim, norm=True, tail=True)
+        want = ao.distill(held, idx, val.astype(float), 1.0, True, np.ones(3))
+        # log p_t ~ -150: 3 u 150 of the distance to the maximum, and the sum of the outside
+        tol = U * (3 * 160 + _n(C) + 100)
+        assert np.all(np.abs(_host(r.log_tail) - want["log_tail"]) < tol)
+        assert np.all(np.abs(_host(r.loss) - want["loss"]) < tol)
+        g = _back(A.distill_loss_grad(t, ti, tv, r.norm, grad_loss=torch.ones(3, device="cuda"), log_tail=r.log_tail, dim=dim, tail=True), dim, C)
+        assert np.all(np.abs(g - want["grad"]) < 2 * tol * (np.abs(want["grad"]) + 1e-3))
 
 
 def test_a_sure_teacher_keeps_its_small_rest():
@@ -450,7 +471,7 @@ def test_broadcast_and_many_stride_inputs():
     assert np.allclose(_host(g)[:, 0], ref, rtol=0, atol=40 * 20 * U)
     # rows that need three strides: one dense copy, the same answers
     t = torch.from_numpy(rng.standard_normal((6, 7, 8, 9)).astype(np.float32)).cuda()[::2, ::3, ::2]
-    a, b = A.label_scores(t, top=3), A.label_scores(t.contiguous(), top=3)
+    a, b = A.label_scores(t, top=3, norm=True), A.label_scores(t.contiguous(), top=3, norm=True)
     assert all(torch.equal(x, y) for x, y in zip(a[1:], b[1:]))
     # the same scores in every layout give the same labels and nearly the same numbers
     t = torch.from_numpy(rng.standard_normal((4, 10, 6, 6)).astype(np.float32)).cuda()
@@ -510,7 +531,7 @@ def test_offsets_beyond_32_bits():
         dim = 0 if layout == "planes" else 1
         rows, C = (shape[1], shape[0]) if layout == "planes" else shape
         lab = torch.full((rows,), C - 1, dtype=torch.int32, device="cuda")
-        r = A.label_scores(z, lab, dim=dim, top=2)
+        r = A.label_scores(z, lab, dim=dim, top=2, norm=True)
         for n in (0, rows - 1):
             row = (z[:, n] if layout == "planes" else z[n]).double()
             m = row.max()
@@ -595,14 +616,14 @@ def test_another_stream_and_two_calls_at_once():
     rng = np.random.default_rng(2)
     data = [torch.from_numpy(rng.standard_normal((3, 70001)).astype(np.float32)).cuda() for _ in range(4)]
     data += [torch.from_numpy(rng.standard_normal((20000, 6)).astype(np.float32)).cuda() for _ in range(4)]
-    want = [A.label_scores(d, top=5) for d in data]
+    want = [A.label_scores(d, top=5, norm=True) for d in data]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(4)]
     got = [None] * len(data)
     for _ in range(5):
         for i, d in enumerate(data):
             with torch.cuda.stream(streams[i % 4]):
-                got[i] = A.label_scores(d, top=5)
+                got[i] = A.label_scores(d, top=5, norm=True)
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert all(torch.equal(x, y) for x, y in zip(w[1:], g[1:]))
@@ -624,9 +645,9 @@ def test_captured_and_replayed(shape, K):
         one = torch.ones(rows, device="cuda")
 
         def work(z=z, lab=lab, idx=idx, val=val, one=one):
-            s = A.label_scores(z, lab, top=min(K, C))
+            s = A.label_scores(z, lab, top=min(K, C), norm=True)
             g = A.label_scores_grad(z, lab, s.norm, grad_log_prob=one, entropy=s.entropy, grad_entropy=one)
-            d = A.distill_loss(z, idx, val, tail=True)
+            d = A.distill_loss(z, idx, val, norm=True, tail=True)
             h = A.distill_loss_grad(z, idx, val, d.norm, grad_loss=one, log_tail=d.log_tail, tail=True)
             return [*s, g, d.loss, h]
 
@@ -665,8 +686,8 @@ def test_the_same_bits_every_time():
         val = torch.zeros(shape[0], 4, device="cuda")
         first = None
         for _ in range(4):
-            s = A.label_scores(z, top=3, background=bg)
-            d = A.distill_loss(z, idx, val, background=bg)
+            s = A.label_scores(z, top=3, norm=True, background=bg)
+            d = A.distill_loss(z, idx, val, norm=True, background=bg)
             g = A.distill_loss_grad(z, idx, val, d.norm, grad_loss=torch.ones(shape[0], device="cuda"), background=bg)
             now = [*s[1:], d.loss, g]
             first = first or now
@@ -677,7 +698,7 @@ def test_numpy_arrays():
     rng = np.random.default_rng(4)
     z = rng.standard_normal((3, 4, 6, 5)).astype(np.float32)
     lab = rng.integers(0, 5, (3, 6, 5)).astype(np.uint8)
-    r = A.label_scores(z, lab, dim=1, background=True, top=2, temperature=1.5)
+    r = A.label_scores(z, lab, dim=1, background=True, top=2, norm=True, temperature=1.5)
     rows = ao.with_background(np.moveaxis(z, 1, -1).reshape(-1, 4).astype(float))
     want = ao.scores(rows, 1.5, lab.reshape(-1), 2)
     assert r.log_prob.shape == (3, 6, 5) and r.top_label.shape == (3, 6, 5, 2) and r.top_label.dtype == np.int32
@@ -687,12 +708,12 @@ def test_numpy_arrays():
     g = A.label_scores_grad(z, lab, r.norm, grad_log_prob=a, entropy=r.entropy, grad_entropy=a, dim=1, background=True, temperature=1.5)
     ref = ao.scores_grad(rows, 1.5, lab.reshape(-1), np.ones(90), np.ones(90))[:, 1:]
     assert g.shape == z.shape and np.allclose(np.moveaxis(g, 1, -1).reshape(-1, 4), ref, rtol=0, atol=200 * U)
-    d = A.distill_loss(z, r.top_label, r.top_log_prob, dim=1, background=True, tail=True, temperature=1.5)
+    d = A.distill_loss(z, r.top_label, r.top_log_prob, dim=1, norm=True, background=True, tail=True, temperature=1.5)
     # a network against its own answers: zero up to the rounding of the stored log probabilities
     assert np.abs(d.loss).max() < 100 * U
-    h = A.distill_loss_grad(z[::-1].copy(), r.top_label, r.top_log_prob, d.norm[::-1].copy(), grad_loss=a, log_tail=None, dim=1,
+    h = A.distill_loss_grad(z, r.top_label, r.top_log_prob, d.norm, grad_loss=a, log_tail=d.log_tail, dim=1, tail=True,
                             background=True, temperature=1.5)
-    assert h.shape == z.shape and np.isfinite(h).all()
+    assert h.shape == z.shape and np.abs(h).max() < 200 * U  # ... and its gradient
     half = A.label_scores(z.astype(np.float16), dim=1)
     assert half.entropy.dtype == np.float32
     empty = A.label_scores(np.zeros((0, 4), np.float32), np.zeros(0, np.int32), top=2)
