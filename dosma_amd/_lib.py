@@ -182,6 +182,7 @@ class QmriDistillArgs(ctypes.Structure):
 L_KINDS = {"int32": 0, "uint8": 1, "int16": 2, "int64": 3}
 SCORE_DTYPES = {"float32": QMRI_F32, "float16": QMRI_F16, "bfloat16": QMRI_BF16}
 MAX_TOP = 64
+SHORT_ROW = 1024  # QMRI_SHORT_ROW: no workspace up to this many classes
 
 MODELS = {"monoexponential": 0, "biexponential": 1}
 MODEL_NPARAMS = {"monoexponential": 2, "biexponential": 4}
@@ -892,7 +893,7 @@ def _fill_logits(a, ptr, dtype, rows, temperature, background):
     z.data, z.dtype, z.background = ptr, SCORE_DTYPES[dtype], 1 if background else 0
     z.rows, z.inner, z.classes = rows.rows, rows.inner, rows.classes
     z.stride_outer, z.stride_inner, z.stride_class = rows.so, rows.si, rows.sc
-    z.temperature = float(temperature)
+    z.temperature = temperature
 
 
 def _fill_grad(a, ptr, rows):
@@ -900,21 +901,30 @@ def _fill_grad(a, ptr, rows):
     a.grad_stride_outer, a.grad_stride_inner, a.grad_stride_class = rows.so, rows.si, rows.sc
 
 
-def _run_answers(op, a, host, device, stream, workspace):
-    """``workspace(bytes)`` -> device pointer: memory of the caller's own allocator for the calls that need some."""
-    lib = load()
+def _run_answers(entries, a, host, device, stream, workspace):
+    """``entries``: names of the host, device and workspace entry.  ``workspace(bytes)`` -> device pointer: memory of the
+    caller's own allocator for the calls that need some."""
+    lib = _lib or load()
     if host:
         require_device()
         a.device = _dev(device)
-        check(getattr(lib, f"qmri_{op}_host")(ctypes.byref(a)))
+        check(getattr(lib, entries[0])(ctypes.byref(a)))
         return
-    a.device, a.stream = int(device), stream
-    if workspace is not None:
+    a.device, a.stream = device, stream
+    if workspace is not None and a.logits.classes > SHORT_ROW:
         need = ctypes.c_uint64(0)
-        check(getattr(lib, f"qmri_{op}_workspace")(ctypes.byref(a), ctypes.byref(need)))
+        check(getattr(lib, entries[2])(ctypes.byref(a), ctypes.byref(need)))
         if need.value:
             a.workspace, a.workspace_bytes = workspace(need.value), need.value
-    check(getattr(lib, f"qmri_{op}_device")(ctypes.byref(a)))
+    rc = getattr(lib, entries[1])(ctypes.byref(a))
+    if rc != QMRI_OK:
+        check(rc)
+
+
+_LABEL_SCORES = ("qmri_label_scores_host", "qmri_label_scores_device", "qmri_label_scores_workspace")
+_LABEL_SCORES_GRAD = ("qmri_label_scores_grad_host", "qmri_label_scores_grad_device")
+_DISTILL = ("qmri_distill_host", "qmri_distill_device", "qmri_distill_workspace")
+_DISTILL_GRAD = ("qmri_distill_grad_host", "qmri_distill_grad_device")
 
 
 def label_scores(logits_ptr, dtype, rows, *, labels_ptr=None, l_dtype=None, top=0, ignore_label=-1, temperature=1.0,
@@ -928,7 +938,7 @@ def label_scores(logits_ptr, dtype, rows, *, labels_ptr=None, l_dtype=None, top=
         a.labels, a.l_kind = labels_ptr, L_KINDS[l_dtype]
     a.top, a.ignore_label = int(top), int(ignore_label)
     a.log_prob, a.entropy, a.norm, a.top_log_prob, a.top_label = log_prob, entropy, norm, top_log_prob, top_label
-    _run_answers("label_scores", a, host, device, stream, workspace)
+    _run_answers(_LABEL_SCORES, a, host, device, stream, workspace)
 
 
 def label_scores_grad(logits_ptr, dtype, rows, grad_ptr, grad_rows, norm, *, labels_ptr=None, l_dtype=None, ignore_label=-1,
@@ -941,7 +951,7 @@ def label_scores_grad(logits_ptr, dtype, rows, grad_ptr, grad_rows, norm, *, lab
         a.labels, a.l_kind = labels_ptr, L_KINDS[l_dtype]
     a.ignore_label = int(ignore_label)
     a.norm, a.entropy, a.grad_log_prob, a.grad_entropy = norm, entropy, grad_log_prob, grad_entropy
-    _run_answers("label_scores_grad", a, host, device, stream, None)
+    _run_answers(_LABEL_SCORES_GRAD, a, host, device, stream, None)
 
 
 def distill(logits_ptr, dtype, rows, top_label_ptr, l_dtype, values_ptr, v_dtype, entries, *, tail=False, temperature=1.0,
@@ -952,7 +962,7 @@ def distill(logits_ptr, dtype, rows, top_label_ptr, l_dtype, values_ptr, v_dtype
     a.top_label, a.l_kind, a.values, a.v_dtype = top_label_ptr, L_KINDS[l_dtype], values_ptr, SCORE_DTYPES[v_dtype]
     a.entries, a.tail = int(entries), 1 if tail else 0
     a.loss, a.norm, a.log_tail = loss, norm, log_tail
-    _run_answers("distill", a, host, device, stream, workspace)
+    _run_answers(_DISTILL, a, host, device, stream, workspace)
 
 
 def distill_grad(logits_ptr, dtype, rows, grad_ptr, grad_rows, top_label_ptr, l_dtype, values_ptr, v_dtype, entries, norm,
@@ -964,4 +974,4 @@ def distill_grad(logits_ptr, dtype, rows, grad_ptr, grad_rows, top_label_ptr, l_
     a.top_label, a.l_kind, a.values, a.v_dtype = top_label_ptr, L_KINDS[l_dtype], values_ptr, SCORE_DTYPES[v_dtype]
     a.entries, a.tail = int(entries), 1 if tail else 0
     a.norm, a.log_tail, a.grad_loss = norm, log_tail, grad_loss
-    _run_answers("distill_grad", a, host, device, stream, None)
+    _run_answers(_DISTILL_GRAD, a, host, device, stream, None)

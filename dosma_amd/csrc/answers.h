@@ -101,13 +101,25 @@ __device__ __forceinline__ long long row_base(const LogitsK &g, long long n, lon
 
 // ---- scores of a row ------------------------------------------------------------------------------------------------------
 // A vector is 16 bytes of scores, at the alignment of one score: rows of odd length begin anywhere, and the memory takes a
-// 16-byte load at any address (aligned ones are not split off: the peeling costs more than the odd line)
+// 16-byte load at any address (aligned ones are not split off: the peeling costs more than the odd line).  It is kept as four
+// words and widened from there: as 2-byte elements the compiler would take it apart and put it together again.
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 template <typename T>
 struct Vec {
-    T v[kVec<T>];
+    unsigned w[4];
 };
+template <typename T>
+__device__ __forceinline__ float get(const Vec<T> &r, int i) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[i]);
+    else if constexpr (std::is_same_v<T, bf16_t>) return __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
+    else return static_cast<float>(__builtin_bit_cast(T, (unsigned short)(i & 1 ? r.w[i / 2] >> 16 : r.w[i / 2])));
+}
+template <typename T>
+__device__ __forceinline__ unsigned bits_of(T v) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(unsigned, v);
+    else return __builtin_bit_cast(unsigned short, v);
+}
 template <typename T>
 __device__ __forceinline__ Vec<T> load_vec(const T *p) {
     Vec<T> r;
@@ -118,15 +130,64 @@ __device__ __forceinline__ Vec<T> load_vec(const T *p) {
 template <typename T>
 __device__ __forceinline__ Vec<T> load_part(const T *p, int n) {
     Vec<T> r;
+    unsigned b[kVec<T>];
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) r.v[i] = i < n ? p[i] : static_cast<T>(kNegInf);
+    for (int i = 0; i < kVec<T>; ++i) b[i] = bits_of(i < n ? p[i] : static_cast<T>(kNegInf));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) r.w[i] = b[i];
+        else r.w[i] = b[2 * i] | (b[2 * i + 1] << 16);
+    }
+    return r;
+}
+// values rounded to T
+template <typename T>
+__device__ __forceinline__ Vec<T> pack_vec(const float (&v)[kVec<T>]) {
+    Vec<T> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(v[i]);
+        else r.w[i] = bits_of(from_f32<T>(v[2 * i])) | (bits_of(from_f32<T>(v[2 * i + 1])) << 16);
+    }
     return r;
 }
 template <typename T>
-__device__ __forceinline__ void store_part(T *p, const Vec<T> &r, int n) {
+__device__ __forceinline__ void store_vec(T *p, const Vec<T> &r) {
+    __builtin_memcpy(p, &r, 16);
+}
+template <typename T>
+__device__ __forceinline__ void store_part(T *p, const float (&v)[kVec<T>], int n) {
 #pragma unroll
     for (int i = 0; i < kVec<T>; ++i)
-        if (i < n) p[i] = r.v[i];
+        if (i < n) p[i] = from_f32<T>(v[i]);
+}
+// 16 scores a lane: the wave's 1024 from p on, in vectors side by side; score i of a lane is the wave's tile_at<T>(lane, i)-th
+template <typename T>
+struct Tile {
+    Vec<T> v[16 / kVec<T>];
+};
+template <typename T>
+__device__ __forceinline__ int tile_at(int lane, int i) {
+    constexpr int V = kVec<T>;
+    return (i / V) * 64 * V + lane * V + i % V;
+}
+// n: scores of the row from p on (wave-uniform); what lies behind is -inf
+template <typename T>
+__device__ __forceinline__ Tile<T> load_tile(const T *p, int n) {
+    constexpr int V = kVec<T>;
+    const int lane = threadIdx.x & 63;
+    Tile<T> r;
+    if (n >= 1024) {
+#pragma unroll
+        for (int u = 0; u < 16 / V; ++u) r.v[u] = load_vec(p + u * 64 * V + lane * V);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 16 / V; ++u) {
+            const int j = u * 64 * V + lane * V;
+            r.v[u] = j + V <= n ? load_vec(p + j) : load_part(p + j, n - j);
+        }
+    }
+    return r;
 }
 
 // NaN goes through a maximum here (v_maximum3_f32), so a row's NaN reaches its statistics without a test of its own
@@ -236,6 +297,78 @@ __device__ __forceinline__ RowStat join(RowStat a, RowStat b, float c2) {
     return {M, ref, a.s + b.s, a.t + b.t};
 }
 
+// A lane's running sums over many scores.  The reference is kept in the units of the exponents, R = ref * c2 rounded: an exponent
+// is then one fused z * c2 - R, and as all of a row's terms are brought to one reference in the end, the rounding of R cancels.
+// It follows the lane's maximum only when that has grown by more than a factor of 16: nearly no step pays for a change.
+constexpr float kSlack = 4.f;
+// Scores whose product with c2 leaves the range of 32 bits cannot be summed like that; a row of such (the lowest value of the type
+// everywhere, for one) is summed again by differences (far_scores).
+constexpr float kFar = 1.0e37f;
+struct Running {
+    float m, R, s, t;
+};
+__device__ __forceinline__ Running no_scores() { return {kNegInf, -1.0e38f, 0.f, 0.f}; }
+template <int N>
+__device__ __forceinline__ float max_of(const float (&x)[N]) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = maxn(m, x[i]);
+    return m;
+}
+// cm: the largest of the scores that come next
+template <bool T2>
+__device__ __forceinline__ void raise(Running &r, float cm, float c2) {
+    r.m = maxn(r.m, cm);
+    if (fmaf(cm, c2, -r.R) > kSlack) {
+        const float R = cm * c2, d = fmaxf(r.R - R, -1.0e4f), f = exp2_hw(d);
+        r.t = T2 ? f * fmaf(d, r.s, r.t) : f * r.t;
+        r.s *= f;
+        r.R = R;
+    }
+}
+// t as the sum of exp2(d) d
+template <int N>
+__device__ __forceinline__ void add_scores(Running &r, const float (&x)[N], float c2) {
+    raise<true>(r, max_of(x), c2);
+    float e[N], et[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float d = clamp2(fmaf(x[i], c2, -r.R));
+        e[i] = exp2_hw(d);
+        et[i] = e[i] * d;
+    }
+    r.s += tree_sum(e);
+    r.t += tree_sum(et);
+}
+__device__ __forceinline__ bool far_scores(float M, float c2) { return M > kNegInf && !(fabsf(M) * c2 < kFar); }
+// factor that brings a lane's sums to reference(M), M the maximum over the lanes; d its exponent
+__device__ __forceinline__ float to_reference(const Running &r, float M, float c2, float &d) {
+    d = fminf(maxn(fmaf(-reference(M), c2, r.R), -1.0e4f), 64.f);  // (a lane that saw nothing has no sums: any factor will do)
+    return exp2_hw(d);
+}
+// the wave's sums together; far: the row's own scores again, j = first, first + step, .. of n, by differences
+template <typename F>
+__device__ __forceinline__ RowStat wave_stat(const Running &r, float c2, F score, int first, int step, int n) {
+    const float M = group_max<64>(r.m);
+    RowStat o = {M, reference(M), 0.f, 0.f};
+    if (far_scores(M, c2)) {
+        float s = 0.f, t = 0.f;
+        for (int j = first; j < n; j += step) {
+            const float d = clamp2((score(j) - o.ref) * c2), e = exp2_hw(d);
+            s += e;
+            t = fmaf(e, d, t);
+        }
+        o.s = group_sum<64>(s);
+        o.t = group_sum<64>(t);
+    } else {
+        float d;
+        const float f = to_reference(r, M, c2, d);
+        o.s = group_sum<64>(r.s * f);
+        o.t = group_sum<64>(f * fmaf(d, r.s, r.t));
+    }
+    return o;
+}
+
 // what a wave's lanes have written to LDS is visible to its other lanes from here on
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -247,11 +380,11 @@ __device__ __forceinline__ void wave_sync() {
 __device__ __forceinline__ bool better(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
 
 // How the rows of a call are cut for the kernels that give a block a row (contiguous classes, more than 1024 of them): segments
-// of whole 16-byte vectors, at most 65536 scores each (the distillation kernel marks the teacher's labels in LDS, a bit a score)
+// of whole 16-byte vectors, of at most `longest` scores
 struct Cut {
     int segs, len;
 };
-Cut cut_rows(const LogitsK &g, int num_cu);
+Cut cut_rows(const LogitsK &g, int num_cu, int longest);
 
 hipError_t label_scores_launch(const ScoresK &k, int dtype, int num_cu, hipStream_t st);
 size_t label_scores_workspace_bytes(const ScoresK &k, int dtype, int num_cu);

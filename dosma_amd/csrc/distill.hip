@@ -13,8 +13,6 @@
 namespace qmri {
 namespace {
 
-constexpr float kSlack = 4.f;  // (a lane's reference follows its maximum when that has grown by a factor of 16)
-
 __device__ __forceinline__ float load_value(const DistillK &k, long long i) {
     if (k.v_dtype == QMRI_F32) return static_cast<const float *>(k.values)[i];
     if (k.v_dtype == QMRI_F16) return to_f32(static_cast<const f16_t *>(k.values)[i]);
@@ -37,6 +35,12 @@ struct Teacher {
 };
 __device__ __forceinline__ float weight(const Teacher &t, float v) { return exp2_hw((v - t.m) * t.c2) * t.scale; }
 __device__ __forceinline__ float log_weight(const Teacher &t, float v) { return (v - t.m) * t.invT + t.lscale; }
+// 1 - e^x for x <= 0 (and a negative number beyond): near 0 the series, whose first term left out is below 2e-8 of the sum at -0.35
+__device__ __forceinline__ float one_minus_exp(float x) {
+    const float p = 1.f + x * 0.5f * (1.f + x * (1.f / 3.f) * (1.f + x * 0.25f * (1.f + x * 0.2f * (1.f + x * (1.f / 6.f) * (1.f + x * (1.f / 7.f))))));
+    return fabsf(x) < 0.35f ? -x * p : 1.f - exp2_hw(x * kLog2e);
+}
+__device__ __forceinline__ float ln(float x) { return __builtin_amdgcn_logf(x) * kLn2; }
 // From what the entries give together: their number, largest value m, sum of exp2((v - base) c2), base = m or (tail) 0, and in
 // the tail the sum without one entry of the largest value.
 __device__ __forceinline__ Teacher teacher_of(const DistillK &k, bool any, float m, float sum, float others) {
@@ -48,7 +52,7 @@ __device__ __forceinline__ Teacher teacher_of(const DistillK &k, bool any, float
         t.scale = 1.f;
         t.lscale = 0.f;
         // 1 - sum q as (1 - e^{v_max}) - the others: nothing cancels for a teacher that is sure of itself
-        const float rest = -expm1f(m) - others;
+        const float rest = one_minus_exp(m) - others;
         t.rest = (any && !(rest <= (float)k.K * 5.9604645e-8f)) ? rest : 0.f;
         t.total = sum + t.rest;
         t.some = any;
@@ -57,7 +61,7 @@ __device__ __forceinline__ Teacher teacher_of(const DistillK &k, bool any, float
         t.c2 = k.g.c2;
         t.invT = k.g.invT;
         t.scale = 1.f / sum;
-        t.lscale = -logf(sum);
+        t.lscale = -ln(sum);
         t.rest = 0.f;
         t.some = any && sum != 0.f;
         t.total = t.some ? 1.f : 0.f;
@@ -95,6 +99,52 @@ __device__ __forceinline__ Teacher teacher_group(const DistillK &k, long long n,
     if (first != one && first != 0x7fffffff) others += teacher_term(k, m, m);
     return teacher_of(k, any, m, group_sum<G>(sum), group_sum<G>(others));
 }
+// by a wave that holds an entry a lane (l < 0: none)
+__device__ __forceinline__ Teacher teacher_wave(const DistillK &k, int l, float v) {
+    const bool ok = l >= 0;
+    const float m = group_max<64>(ok ? v : kNegInf);
+    const float e = ok ? teacher_term(k, v, m) : 0.f;
+    const unsigned long long at = __ballot(ok && v == m);
+    const int first = at ? __ffsll(at) - 1 : -1;
+    return teacher_of(k, __ballot(ok) != 0ull, m, group_sum<64>(e), group_sum<64>((int)(threadIdx.x & 63) == first ? 0.f : e));
+}
+// K entries in registers
+template <int K>
+__device__ __forceinline__ void load_entries(const DistillK &k, long long n, int cats, int (&l)[K], float (&v)[K]) {
+    if (k.K == K && k.l_kind == QMRI_L_I32 && k.v_dtype == QMRI_F32) {
+        __builtin_memcpy(&l, static_cast<const int *>(k.labels) + n * K, sizeof(l));
+        __builtin_memcpy(&v, static_cast<const float *>(k.values) + n * K, sizeof(v));
+#pragma unroll
+        for (int q = 0; q < K; ++q) l[q] = (unsigned)l[q] < (unsigned)cats ? l[q] : -1;
+    } else {
+#pragma unroll
+        for (int q = 0; q < K; ++q) {
+            l[q] = -1;
+            v[q] = 0.f;
+            if (q < k.K) l[q] = load_entry(k, n, q, cats, v[q]);
+        }
+    }
+}
+template <int K>
+__device__ __forceinline__ Teacher teacher_lane(const DistillK &k, const int (&l)[K], const float (&v)[K]) {
+    float m = kNegInf, sum = 0.f, others = 0.f;
+    bool any = false, left_out = false;
+#pragma unroll
+    for (int q = 0; q < K; ++q)
+        if (l[q] >= 0) {
+            m = maxn(m, v[q]);
+            any = true;
+        }
+#pragma unroll
+    for (int q = 0; q < K; ++q) {
+        const float e = l[q] >= 0 ? teacher_term(k, v[q], m) : 0.f;
+        const bool first = l[q] >= 0 && v[q] == m && !left_out;
+        sum += e;
+        others += first ? 0.f : e;
+        left_out |= first;
+    }
+    return teacher_of(k, any, m, sum, others);
+}
 template <>
 __device__ __forceinline__ Teacher teacher_group<1>(const DistillK &k, long long n, int, int cats) {
     float m = kNegInf;
@@ -125,7 +175,7 @@ struct Student {
     float ref, ls;
     bool empty;
 };
-__device__ __forceinline__ Student student_of(float M, float s) { return {reference(M), __builtin_amdgcn_logf(s) * kLn2, s == 0.f}; }
+__device__ __forceinline__ Student student_of(float M, float s) { return {reference(M), ln(s), s == 0.f}; }
 __device__ __forceinline__ float entry_loss(const DistillK &k, const Teacher &t, const Student &p, float v, float z) {
     const float q = weight(t, v);
     const float lp = (z == kNegInf && p.ls == p.ls) ? kNegInf : (z - p.ref) * k.g.invT - p.ls;
@@ -140,7 +190,7 @@ __device__ __forceinline__ float gather(const LogitsK &g, const T *z, int l) {
 template <int G, typename T>
 __device__ __forceinline__ float log_outside(const DistillK &k, long long n, const T *z, int gl, int cats, const Student &p, const Teacher &t, float so) {
     if (!k.tail) return 0.f;
-    if (!(so < 7.888609e-31f) || t.rest == 0.f || p.empty) return __builtin_amdgcn_logf(so) * kLn2;
+    if (!(so < 7.888609e-31f) || t.rest == 0.f || p.empty) return ln(so);
     auto score = [&](int j) {
         float v;
         for (int q = 0; q < k.K; ++q)
@@ -152,65 +202,79 @@ __device__ __forceinline__ float log_outside(const DistillK &k, long long n, con
     m = group_max<G>(m);
     for (int j = gl; j < cats; j += G) s += exp2_hw((score(j) - reference(m)) * k.g.c2);
     s = group_sum<G>(s);
-    return s == 0.f ? kNegInf : (m - p.ref) * k.g.invT + __builtin_amdgcn_logf(s) * kLn2;
+    return s == 0.f ? kNegInf : (m - p.ref) * k.g.invT + ln(s);
 }
 __device__ __forceinline__ void write_row(const DistillK &k, long long n, float M, float lso, const Student &p, const Teacher &t, float loss) {
     const float lt = p.empty ? kNegInf : lso - p.ls;
-    if (k.tail && t.rest != 0.f) loss += t.rest * (logf(t.rest) - lt);
+    if (k.tail && t.rest != 0.f) loss += t.rest * (ln(t.rest) - lt);
     if (k.loss) k.loss[n] = (p.empty || !t.some) ? 0.f : loss;
     if (k.norm) *reinterpret_cast<float2 *>(k.norm + 2 * n) = make_float2(p.ls != p.ls ? p.ls : M, p.ls);
     if (k.log_tail) k.log_tail[n] = lt;
 }
 
 // ---- small: one lane a row ----------------------------------------------------------------------------------------------------
-template <typename T, int N, bool CONTIG>
-__device__ __forceinline__ void load_small(const T *z, long long sc, T (&v)[N]) {
-    if (CONTIG) {
+// K: entries held in registers (as many or fewer of them in use); 0: any number, read again where they are needed.
+template <typename T, int N>
+__device__ __forceinline__ void load_small(const LogitsK &g, const T *z, T (&v)[N]) {
+    if (g.sc == 1) {
         __builtin_memcpy(&v, z, sizeof(v));
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = z[j * sc];
+        for (int j = 0; j < N; ++j) v[j] = z[j * g.sc];
     }
 }
-template <typename T, int N, bool BG, bool CONTIG>
+template <typename T, int N, int K>
 __global__ __launch_bounds__(256) void distill_small_kernel(const DistillK k) {
     const LogitsK &g = k.g;
-    constexpr int CATS = N + BG;
+    const int cats = N + g.bg;
     const long long stride = (long long)gridDim.x * 256;
     for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < g.rows; n += stride) {
-        T raw[N];
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
-        load_small<T, N, CONTIG>(z, g.sc, raw);
-        const Teacher t = teacher_group<1>(k, n, 0, CATS);
-        float x[CATS];
-        if (BG) x[0] = 0.f;
+        T raw[N];
+        load_small<T, N>(g, z, raw);
+        int el[K > 0 ? K : 1];
+        float ev[K > 0 ? K : 1];
+        if (K) load_entries(k, n, cats, el, ev);
+        const Teacher t = K ? teacher_lane(k, el, ev) : teacher_group<1>(k, n, 0, cats);
+        // x[0]: the implicit category, or one that is not offered; x[j + 1]: class j
+        float x[N + 1], e[N + 1], s = 0.f, so = 0.f;
+        x[0] = g.bg ? 0.f : kNegInf;
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j + BG] = to_f32(raw[j]);
+        for (int j = 0; j < N; ++j) x[j + 1] = to_f32(raw[j]);
         float M = x[0];
 #pragma unroll
-        for (int j = 1; j < CATS; ++j) M = maxn(M, x[j]);
+        for (int j = 1; j <= N; ++j) M = maxn(M, x[j]);
         const float ref = reference(M);
-        float e[CATS], s = 0.f, so = 0.f;
 #pragma unroll
-        for (int j = 0; j < CATS; ++j) {
+        for (int j = 0; j <= N; ++j) {
             e[j] = exp2_hw((x[j] - ref) * g.c2);
             s += e[j];
         }
         const Student p = student_of(M, s);
         unsigned in = 0u;
         float loss = 0.f;
-        for (int q = 0; q < k.K; ++q) {
-            float v, zl = 0.f;
-            const int l = load_entry(k, n, q, CATS, v);
-            if (l < 0) continue;
-            in |= 1u << l;
+        auto entry = [&](int l, float v) {
+            if (l < 0) return;
+            float zl = 0.f;
+            const int at = l + 1 - g.bg;
+            in |= 1u << at;
 #pragma unroll
-            for (int j = 0; j < CATS; ++j) zl = l == j ? x[j] : zl;
+            for (int j = 0; j <= N; ++j) zl = at == j ? x[j] : zl;
             loss += entry_loss(k, t, p, v, zl);
+        };
+        if (K) {
+#pragma unroll
+            for (int q = 0; q < K; ++q) entry(el[q], ev[q]);
+        } else {
+            for (int q = 0; q < k.K; ++q) {
+                float v;
+                const int l = load_entry(k, n, q, cats, v);
+                entry(l, v);
+            }
         }
 #pragma unroll
-        for (int j = 0; j < CATS; ++j) so += (in >> j) & 1u ? 0.f : e[j];
-        write_row(k, n, M, log_outside<1>(k, n, z, 0, CATS, p, t, so), p, t, loss);
+        for (int j = 0; j <= N; ++j) so += (in >> j) & 1u ? 0.f : e[j];
+        write_row(k, n, M, log_outside<1>(k, n, z, 0, cats, p, t, so), p, t, loss);
     }
 }
 
@@ -241,38 +305,47 @@ __device__ __forceinline__ float grad_inside(const GradRow &r, float c2, float v
     return r.zero ? 0.f : r.f * fmaf(r.total, p, -qs);
 }
 
-template <typename T, int N, bool CONTIG>
+template <typename T, int N, int K>
 __global__ __launch_bounds__(256) void distill_grad_small_kernel(const DistillK k) {
     const LogitsK &g = k.g;
     const int cats = N + g.bg;
     const long long stride = (long long)gridDim.x * 256;
     for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < g.rows; n += stride) {
         T raw[N];
-        load_small<T, N, CONTIG>(static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si), g.sc, raw);
+        load_small<T, N>(g, static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si), raw);
         T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi);
-        const Teacher t = teacher_group<1>(k, n, 0, cats);
+        int el[K > 0 ? K : 1];
+        float ev[K > 0 ? K : 1];
+        if (K) load_entries(k, n, cats, el, ev);
+        const Teacher t = K ? teacher_lane(k, el, ev) : teacher_group<1>(k, n, 0, cats);
         const GradRow r = grad_row(k, n, t);
         unsigned in = 0u;
         float qs[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) qs[j] = 0.f;
-        for (int q = 0; q < k.K; ++q) {
-            float v;
-            const int l = load_entry(k, n, q, cats, v) - g.bg;
+        auto entry = [&](int l, float v) {
+            if (l < g.bg) return;
             const float w = weight(t, v);
+            in |= 1u << (l - g.bg);
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (l == j) {
-                    qs[j] += w;
-                    in |= 1u << j;
-                }
+            for (int j = 0; j < N; ++j) qs[j] += l - g.bg == j ? w : 0.f;
+        };
+        if (K) {
+#pragma unroll
+            for (int q = 0; q < K; ++q) entry(el[q], ev[q]);
+        } else {
+            for (int q = 0; q < k.K; ++q) {
+                float v;
+                const int l = load_entry(k, n, q, cats, v);
+                entry(l, v);
+            }
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const float v = to_f32(raw[j]);
             raw[j] = from_f32<T>((in >> j) & 1u ? grad_inside(r, g.c2, v, qs[j]) : grad_outside(r, g.c2, v));
         }
-        if (CONTIG) {
+        if (k.gsc == 1) {
             __builtin_memcpy(out, &raw, sizeof(raw));
         } else {
 #pragma unroll
@@ -305,7 +378,7 @@ __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
             const int j = (i * G + gl) * V;
             const Vec<T> r = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[i * V + e] = to_f32(r.v[e]);
+            for (int e = 0; e < V; ++e) x[i * V + e] = get(r, e);
         }
         x[16] = (g.bg && gl == 0) ? 0.f : kNegInf;
         unsigned in = 0u;
@@ -395,140 +468,146 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = (i * G + gl) * V;
+            float y[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[i].v[e] = from_f32<T>(grad_outside(r, g.c2, to_f32(x[i].v[e])));
+            for (int e = 0; e < V; ++e) y[e] = grad_outside(r, g.c2, get(x[i], e));
             if ((in >> (i * V)) & ((1u << V) - 1u)) {
 #pragma unroll
                 for (int e = 0; e < V; ++e)
-                    if ((in >> (i * V + e)) & 1u) x[i].v[e] = s_val[threadIdx.x * 16 + i * V + e];
+                    if ((in >> (i * V + e)) & 1u) y[e] = to_f32(s_val[threadIdx.x * 16 + i * V + e]);
             }
             if (!live) continue;
-            if (j + V <= g.C) __builtin_memcpy(out + j, &x[i], 16);
-            else store_part(out + j, x[i], g.C - j);
+            if (j + V <= g.C) store_vec(out + j, pack_vec<T>(y));
+            else store_part(out + j, y, g.C - j);
         }
         wave_sync();
     }
 }
 
-// ---- block: four waves a segment of a row --------------------------------------------------------------------------------------
+// ---- block: W waves a segment of a row -----------------------------------------------------------------------------------------
 // The tail's sum leaves the entries' labels out: a bit a score in LDS, looked up a vector at a time.
-constexpr int kSegWords = 65536 / 32;
+constexpr int kLongest = 131072;  // scores of a segment then: 16 KB of marks
 
 // wave 0, one entry a lane: the loss of a finished row
 template <typename T>
 __device__ __forceinline__ void finish_row(const DistillK &k, long long n, const T *z, float M, float s, float so) {
     const int lane = threadIdx.x & 63, cats = k.g.C + k.g.bg;
-    const Teacher t = teacher_group<64>(k, n, lane, cats);
+    float v = 0.f;
+    const int l = lane < k.K ? load_entry(k, n, lane, cats, v) : -1;
+    const float zl = l >= 0 ? gather(k.g, z, l) : 0.f;
+    const Teacher t = teacher_wave(k, l, v);
     const Student p = student_of(M, s);
-    float loss = 0.f;
-    if (lane < k.K) {
-        float v;
-        const int l = load_entry(k, n, lane, cats, v);
-        if (l >= 0) loss = entry_loss(k, t, p, v, gather(k.g, z, l));
-    }
+    float loss = l >= 0 ? entry_loss(k, t, p, v, zl) : 0.f;
     loss = group_sum<64>(loss);
     const float lso = log_outside<64>(k, n, z, lane, cats, p, t, so);
     if (lane == 0) write_row(k, n, M, lso, p, t, loss);
 }
 
-template <typename T, bool TAIL>
-__global__ __launch_bounds__(256) void distill_block_kernel(const DistillK k, const Cut cut) {
-    __shared__ RowStat s_stat[4];
-    __shared__ unsigned s_bits[TAIL ? kSegWords : 1];
+// x without the marked scores
+template <int N>
+__device__ __forceinline__ void add_outside(Running &r, const float (&x)[N], float c2, unsigned in) {
+    raise<false>(r, max_of(x), c2);
+    float e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = exp2_hw(fmaf(x[i], c2, -r.R));
+    const float s = tree_sum(e);
+    r.s += s;
+    if (in) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = (in >> i) & 1u ? 0.f : e[i];
+        r.t += tree_sum(e);
+    } else {
+        r.t += s;
+    }
+}
+template <typename T, bool TAIL, int W>
+__global__ __launch_bounds__(64 * W, 8) void distill_block_kernel(const DistillK k, const Cut cut) {
+    __shared__ RowStat s_stat[W];
+    extern __shared__ unsigned s_bits[];  // TAIL: cut.len bits
     __shared__ int s_back;
     const LogitsK &g = k.g;
-    constexpr int V = kVec<T>, U = 16 / V, TILE = 64 * 16;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    constexpr int V = kVec<T>, TILE = 1024;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cats = g.C + g.bg;
     const long long work = g.rows * cut.segs;
     for (long long item = blockIdx.x; item < work; item += gridDim.x) {
         const long long n = cut.segs == 1 ? item : item / cut.segs;
         const int seg = cut.segs == 1 ? 0 : (int)(item - n * cut.segs);
         const int c0 = seg * cut.len, c1 = c0 + cut.len < g.C ? c0 + cut.len : g.C;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
-        Vec<T> nx[U];
-        auto fetch = [&](int c) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = c + u * 64 * V + lane * V;
-                nx[u] = j + V <= c1 ? load_vec(z + j) : load_part(z + j, c1 - j);
-            }
-        };
         int c = c0 + w * TILE;
-        if (c < c1) fetch(c);
+        Tile<T> next;
+        if (c < c1) next = load_tile(z + c, c1 - c);
         if (TAIL) {
-            for (int i = threadIdx.x; i < (c1 - c0 + 31) / 32; i += 256) s_bits[i] = 0u;
+            for (int i = threadIdx.x; i < (c1 - c0 + 31) / 32; i += 64 * W) s_bits[i] = 0u;
             if (threadIdx.x == 0) s_back = 0;
             __syncthreads();
             if ((int)threadIdx.x < k.K) {
                 float v;
-                const int l = load_entry(k, n, threadIdx.x, g.C + g.bg, v), j = l - g.bg - c0;
+                const int l = load_entry(k, n, threadIdx.x, cats, v), j = l - g.bg - c0;
                 if (l >= 0 && l < g.bg) s_back = 1;
                 else if (l >= 0 && j >= 0 && j < c1 - c0) atomicOr(&s_bits[j >> 5], 1u << (j & 31));
             }
             __syncthreads();
         }
         // t holds the sum outside the entries here
-        RowStat r = no_stat();
-        if (g.bg && seg == 0 && threadIdx.x == 0) r = {0.f, 0.f, 1.f, (TAIL && s_back) ? 0.f : 1.f};
-        for (; c < c1; c += 4 * TILE) {
-            Vec<T> now[U];
+        Running r = no_scores();
+        const bool back = g.bg && seg == 0 && w == 0;
+        if (back && lane == 0) r = {0.f, 0.f, 1.f, (TAIL && s_back) ? 0.f : 1.f};
+        for (; c < c1; c += W * TILE) {
+            float x[16];
 #pragma unroll
-            for (int u = 0; u < U; ++u) now[u] = nx[u];
-            if (c + 4 * TILE < c1) fetch(c + 4 * TILE);
-            float x[16], cm = kNegInf;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[i] = to_f32(now[i / V].v[i % V]);
-                cm = maxn(cm, x[i]);
-            }
-            r.m = maxn(r.m, cm);
-            if ((cm - r.ref) * g.c2 > kSlack) {
-                const float f = exp2_hw(maxn((r.ref - cm) * g.c2, -1.0e4f));
-                r.s *= f;
-                r.t *= f;
-                r.ref = cm;
-            }
-            float e[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) e[i] = exp2_hw((x[i] - r.ref) * g.c2);
-            const float sum = tree_sum(e);
-            r.s += sum;
+            for (int i = 0; i < 16; ++i) x[i] = get(next.v[i / V], i % V);
+            if (c + W * TILE < c1) next = load_tile(z + c + W * TILE, c1 - c - W * TILE);
+            unsigned in = 0u;
             if (TAIL) {
-                unsigned in = 0u;
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
+                for (int u = 0; u < 16 / V; ++u) {
                     const int j = c + u * 64 * V + lane * V - c0;
                     in |= (j < c1 - c0 ? s_bits[j >> 5] >> (j & 31) & ((1u << V) - 1u) : 0u) << (u * V);
                 }
-                if (in) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) e[i] = (in >> i) & 1u ? 0.f : e[i];
-                    r.t += tree_sum(e);
-                } else {
-                    r.t += sum;
-                }
             }
+            add_outside(r, x, g.c2, in);
         }
-        {
-            const float M = group_max<64>(r.m), ref = reference(M);
-            const float f = r.ref == ref ? 1.f : exp2_hw(maxn((r.ref - ref) * g.c2, -1.0e4f));
-            r = {M, ref, group_sum<64>(r.s * f), TAIL ? group_sum<64>(r.t * f) : 0.f};
+        const float M = group_max<64>(r.m), ref = reference(M);
+        RowStat st = {M, ref, 0.f, 0.f};
+        if (far_scores(M, g.c2)) {  // (see answers.h)
+            float s = 0.f, so = 0.f;
+            for (int t0 = c0 + w * TILE; t0 < c1; t0 += W * TILE)
+                for (int j = t0 + lane; j < t0 + TILE && j < c1; j += 64) {
+                    const float e = exp2_hw((to_f32(z[j]) - ref) * g.c2);
+                    s += e;
+                    if (!TAIL || !(s_bits[(j - c0) >> 5] >> ((j - c0) & 31) & 1u)) so += e;
+                }
+            if (back && lane == 0) {
+                const float e = exp2_hw((0.f - ref) * g.c2);
+                s += e;
+                if (!(TAIL && s_back)) so += e;
+            }
+            st.s = group_sum<64>(s);
+            st.t = group_sum<64>(so);
+        } else {
+            float d;
+            const float f = to_reference(r, M, g.c2, d);
+            st.s = group_sum<64>(r.s * f);
+            st.t = TAIL ? group_sum<64>(r.t * f) : 0.f;
         }
-        if (lane == 0) s_stat[w] = r;
+        if (lane == 0) s_stat[w] = st;
         __syncthreads();
         if (w == 0) {
-            const float M = maxn(maxn(s_stat[0].m, s_stat[1].m), maxn(s_stat[2].m, s_stat[3].m)), ref = reference(M);
-            float s = 0.f, so = 0.f;
+            float MM = s_stat[0].m, s = 0.f, so = 0.f;
 #pragma unroll
-            for (int o = 0; o < 4; ++o) {
-                const float f = s_stat[o].ref == ref ? 1.f : exp2_hw(maxn((s_stat[o].ref - ref) * g.c2, -1.0e4f));
+            for (int o = 1; o < W; ++o) MM = maxn(MM, s_stat[o].m);
+            const float rr = reference(MM);
+#pragma unroll
+            for (int o = 0; o < W; ++o) {
+                const float f = s_stat[o].ref == rr ? 1.f : exp2_hw(maxn((s_stat[o].ref - rr) * g.c2, -1.0e4f));
                 s += s_stat[o].s * f;
                 so += s_stat[o].t * f;
             }
             if (cut.segs > 1) {
-                if (lane == 0) static_cast<float4 *>(k.ws)[item] = make_float4(M, s, so, 0.f);
+                if (lane == 0) static_cast<float4 *>(k.ws)[item] = make_float4(MM, s, so, 0.f);
             } else {
-                finish_row(k, n, z, M, s, so);
+                finish_row(k, n, z, MM, s, so);
             }
         }
         __syncthreads();
@@ -556,64 +635,70 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillK k, cons
     }
 }
 
-// A block takes 256 lanes x 16 scores of a row at a time.  The entries' labels are marked as above; the few vectors that hold one
-// look it up among the entries.
+// A block takes a segment of a row, 256 lanes x 16 scores at a time, as if none of them were an entry's label; those few are
+// written over at the end, when the block's other stores have arrived.
 template <typename T>
-__global__ __launch_bounds__(256) void distill_grad_block_kernel(const DistillK k, long long tiles) {
+__global__ __launch_bounds__(256) void distill_grad_block_kernel(const DistillK k, const Cut cut) {
     constexpr int V = kVec<T>, NV = 16 / V, TILE = 256 * 16;
-    __shared__ unsigned s_bits[TILE / 32];
-    __shared__ int s_l[64];
-    __shared__ float s_q[64];
     __shared__ GradRow s_row;
     const LogitsK &g = k.g;
-    for (long long item = blockIdx.x; item < g.rows * tiles; item += gridDim.x) {
-        const long long n = item / tiles;
-        const int c0 = (int)(item - n * tiles) * TILE;
+    for (long long item = blockIdx.x; item < g.rows * cut.segs; item += gridDim.x) {
+        const long long n = cut.segs == 1 ? item : item / cut.segs;
+        const int c0 = cut.segs == 1 ? 0 : (int)(item - n * cut.segs) * cut.len, c1 = c0 + cut.len < g.C ? c0 + cut.len : g.C;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
         T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi);
-        Vec<T> x[NV];
+        Vec<T> nx[NV];
+        auto fetch = [&](int c) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = c0 + (i * 256 + threadIdx.x) * V;
-            x[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
-        }
-        if (threadIdx.x < TILE / 32) s_bits[threadIdx.x] = 0u;
-        __syncthreads();
+            for (int i = 0; i < NV; ++i) {
+                const int j = c + (i * 256 + threadIdx.x) * V;
+                nx[i] = j + V <= c1 ? load_vec(z + j) : load_part(z + j, c1 - j);
+            }
+        };
+        fetch(c0);
+        int mine = -1;  // wave 0: the class of a lane's entry if it lies in this segment, and its gradient
+        T value = static_cast<T>(0.f);
         if (threadIdx.x < 64) {
             const int lane = threadIdx.x;
-            const Teacher t = teacher_group<64>(k, n, lane, g.C + g.bg);
             float v = 0.f;
             const int l = lane < k.K ? load_entry(k, n, lane, g.C + g.bg, v) : -1, c = l - g.bg;
-            s_l[lane] = l < 0 ? -1 : c;
-            s_q[lane] = l < 0 ? 0.f : weight(t, v);
-            if (l >= 0 && c >= c0 && c < c0 + TILE) atomicOr(&s_bits[(c - c0) >> 5], 1u << ((c - c0) & 31));
+            const bool here = l >= 0 && c >= c0 && c < c1;
+            const float zl = here ? to_f32(z[c]) : 0.f;
+            const Teacher t = teacher_wave(k, l, v);
             const GradRow r = grad_row(k, n, t);
             if (lane == 0) s_row = r;
+            const float q = l >= 0 ? weight(t, v) : 0.f;
+            float qs = 0.f;  // (the same label twice: each of its lanes has the sum of all its entries, in their order)
+            for (int o = 0; o < k.K; ++o) {
+                const float oq = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(q), o));
+                qs += __builtin_amdgcn_readlane(l, o) == l ? oq : 0.f;
+            }
+            if (here) {
+                mine = c;
+                value = from_f32<T>(grad_inside(r, g.c2, zl, qs));
+            }
         }
         __syncthreads();
         const GradRow r = s_row;
+        for (int c = c0; c < c1; c += TILE) {
+            Vec<T> now[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = c0 + (i * 256 + threadIdx.x) * V;
-            const unsigned in = s_bits[(j - c0) >> 5] >> ((j - c0) & 31) & ((1u << V) - 1u);
-            Vec<T> y;
+            for (int i = 0; i < NV; ++i) now[i] = nx[i];
+            if (c + TILE < c1) fetch(c + TILE);
 #pragma unroll
-            for (int e = 0; e < V; ++e) y.v[e] = from_f32<T>(grad_outside(r, g.c2, to_f32(x[i].v[e])));
-            if (in) {
-                for (int q = 0; q < k.K; ++q) {
-                    const int at = s_l[q] - j;
-                    if (s_l[q] < 0 || at < 0 || at >= V) continue;
-                    float qs = 0.f;  // (the same label twice: each time the sum of all its entries, in their order)
-                    for (int o = 0; o < k.K; ++o) qs += s_l[o] == s_l[q] ? s_q[o] : 0.f;
+            for (int i = 0; i < NV; ++i) {
+                const int j = c + (i * 256 + threadIdx.x) * V;
+                if (j >= c1) continue;
+                float y[V];
 #pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (e == at) y.v[e] = from_f32<T>(grad_inside(r, g.c2, to_f32(x[i].v[e]), qs));
-                }
+                for (int e = 0; e < V; ++e) y[e] = grad_outside(r, g.c2, get(now[i], e));
+                if (j + V <= c1) store_vec(out + j, pack_vec<T>(y));
+                else store_part(out + j, y, c1 - j);
             }
-            if (j + V <= g.C) __builtin_memcpy(out + j, &y, 16);
-            else store_part(out + j, y, g.C - j);
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+        if (mine >= 0) out[mine] = value;
     }
 }
 
@@ -634,37 +719,40 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillK k) {
     const long long stride = (long long)gridDim.x * 256;
     for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < g.rows; n += stride) {
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
-        RowStat r = no_stat();  // (t: the sum outside the entries)
+        Running r = no_scores();  // (t: the sum outside the entries)
         for (int c0 = 0; c0 < cats; c0 += 32) {
             const unsigned in = k.tail ? marks(k, n, c0, cats) : 0u;
 #pragma unroll
             for (int i0 = 0; i0 < 32; i0 += 8) {
                 if (c0 + i0 >= cats) break;
-                float x[8], cm = kNegInf;
+                float x[8];
+                if (c0 + i0 >= g.bg && c0 + i0 + 8 <= cats) {
+                    const T *p = z + (long long)(c0 + i0 - g.bg) * g.sc;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int j = c0 + i0 + i;
-                    x[i] = j >= cats ? kNegInf : j < g.bg ? 0.f : to_f32(z[(long long)(j - g.bg) * g.sc]);
-                    cm = maxn(cm, x[i]);
+                    for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i * g.sc]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = c0 + i0 + i < cats ? gather(g, z, c0 + i0 + i) : kNegInf;
                 }
-                r.m = maxn(r.m, cm);
-                if ((cm - r.ref) * g.c2 > kSlack) {
-                    const float f = exp2_hw(maxn((r.ref - cm) * g.c2, -1.0e4f));
-                    r.s *= f;
-                    r.t *= f;
-                    r.ref = cm;
-                }
-                float e[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = exp2_hw((x[i] - r.ref) * g.c2);
-                r.s += tree_sum(e);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = (in >> (i0 + i)) & 1u ? 0.f : e[i];
-                r.t += tree_sum(e);
+                add_outside(r, x, g.c2, (in >> i0) & 0xffu);
             }
         }
-        const float ref = reference(r.m), f = r.ref == ref ? 1.f : exp2_hw(maxn((r.ref - ref) * g.c2, -1.0e4f));
-        const Student p = student_of(r.m, r.s * f);
+        float sum = 0.f, so = 0.f;
+        if (far_scores(r.m, g.c2)) {  // (see answers.h)
+            unsigned in = 0u;
+            for (int j = 0; j < cats; ++j) {
+                if (k.tail && (j & 31) == 0) in = marks(k, n, j, cats);
+                const float e = exp2_hw((gather(g, z, j) - reference(r.m)) * g.c2);
+                sum += e;
+                so += (in >> (j & 31)) & 1u ? 0.f : e;
+            }
+        } else {
+            float d;
+            const float f = to_reference(r, r.m, g.c2, d);
+            sum = r.s * f;
+            so = r.t * f;
+        }
+        const Student p = student_of(r.m, sum);
         const Teacher t = teacher_group<1>(k, n, 0, cats);
         float loss = 0.f;
         for (int q = 0; q < k.K; ++q) {
@@ -672,7 +760,7 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillK k) {
             const int l = load_entry(k, n, q, cats, v);
             if (l >= 0) loss += entry_loss(k, t, p, v, gather(g, z, l));
         }
-        write_row(k, n, r.m, log_outside<1>(k, n, z, 0, cats, p, t, r.t * f), p, t, loss);
+        write_row(k, n, r.m, log_outside<1>(k, n, z, 0, cats, p, t, so), p, t, loss);
     }
 }
 
@@ -687,38 +775,43 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(const DistillK k) {
         float v;
         s_l[w][lane] = lane < k.K ? load_entry(k, n, lane, cats, v) : -1;
         wave_sync();
-        RowStat r = no_stat();
+        Running r = no_scores();
+        auto listed = [&](int j) {
+            bool in = false;
+            for (int q = 0; q < k.K; ++q) in |= s_l[w][q] == j;
+            return in;
+        };
         for (int j0 = 0; j0 < cats; j0 += 256) {
-            float x[4], cm = kNegInf;
+            float x[4];
+            unsigned in = 0u;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = j0 + i * 64 + lane;
                 x[i] = j < cats ? gather(g, z, j) : kNegInf;
-                cm = maxn(cm, x[i]);
             }
-            r.m = maxn(r.m, cm);
-            if ((cm - r.ref) * g.c2 > kSlack) {
-                const float f = exp2_hw(maxn((r.ref - cm) * g.c2, -1.0e4f));
-                r.s *= f;
-                r.t *= f;
-                r.ref = cm;
-            }
-            float e[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = exp2_hw((x[i] - r.ref) * g.c2);
-            r.s += tree_sum(e);
             if (k.tail) {
                 for (int q = 0; q < k.K; ++q) {
                     const int at = s_l[w][q] - j0 - lane;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) e[i] = at == i * 64 ? 0.f : e[i];
+                    if ((at & 63) == 0 && at >= 0 && at < 256) in |= 1u << (at >> 6);
                 }
-                r.t += tree_sum(e);
             }
+            add_outside(r, x, g.c2, in);
         }
-        const float M = group_max<64>(r.m), ref = reference(M);
-        const float f = r.ref == ref ? 1.f : exp2_hw(maxn((r.ref - ref) * g.c2, -1.0e4f));
-        finish_row(k, n, z, M, group_sum<64>(r.s * f), group_sum<64>(r.t * f));
+        const float M = group_max<64>(r.m);
+        float sum = 0.f, so = 0.f;
+        if (far_scores(M, g.c2)) {  // (see answers.h)
+            for (int j = lane; j < cats; j += 64) {
+                const float e = exp2_hw((gather(g, z, j) - reference(M)) * g.c2);
+                sum += e;
+                so += k.tail && listed(j) ? 0.f : e;
+            }
+        } else {
+            float d;
+            const float f = to_reference(r, M, g.c2, d);
+            sum = r.s * f;
+            so = r.t * f;
+        }
+        finish_row(k, n, z, M, group_sum<64>(sum), group_sum<64>(so));
         wave_sync();
     }
 }
@@ -778,21 +871,32 @@ unsigned grid_of(long long blocks, int num_cu, int per_cu) {
 bool contiguous(const LogitsK &g) { return g.sc == 1 || g.C == 1; }
 
 template <typename T, int N>
-void small(const DistillK &k, bool contig, int num_cu, hipStream_t st) {
+void small(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of((k.g.rows + 255) / 256, num_cu, 64)), block(256);
-    if (contig) {
-        if (k.g.bg) hipLaunchKernelGGL((distill_small_kernel<T, N, true, true>), grid, block, 0, st, k);
-        else hipLaunchKernelGGL((distill_small_kernel<T, N, false, true>), grid, block, 0, st, k);
+    if (grad) {
+        if (k.K <= 2) hipLaunchKernelGGL((distill_grad_small_kernel<T, N, 2>), grid, block, 0, st, k);
+        else if (k.K <= 4) hipLaunchKernelGGL((distill_grad_small_kernel<T, N, 4>), grid, block, 0, st, k);
+        else if (k.K <= 8) hipLaunchKernelGGL((distill_grad_small_kernel<T, N, 8>), grid, block, 0, st, k);
+        else hipLaunchKernelGGL((distill_grad_small_kernel<T, N, 0>), grid, block, 0, st, k);
     } else {
-        if (k.g.bg) hipLaunchKernelGGL((distill_small_kernel<T, N, true, false>), grid, block, 0, st, k);
-        else hipLaunchKernelGGL((distill_small_kernel<T, N, false, false>), grid, block, 0, st, k);
+        if (k.K <= 2) hipLaunchKernelGGL((distill_small_kernel<T, N, 2>), grid, block, 0, st, k);
+        else if (k.K <= 4) hipLaunchKernelGGL((distill_small_kernel<T, N, 4>), grid, block, 0, st, k);
+        else if (k.K <= 8) hipLaunchKernelGGL((distill_small_kernel<T, N, 8>), grid, block, 0, st, k);
+        else hipLaunchKernelGGL((distill_small_kernel<T, N, 0>), grid, block, 0, st, k);
     }
 }
-template <typename T, int N>
-void small_grad(const DistillK &k, bool contig, int num_cu, hipStream_t st) {
-    const dim3 grid(grid_of((k.g.rows + 255) / 256, num_cu, 64)), block(256);
-    if (contig) hipLaunchKernelGGL((distill_grad_small_kernel<T, N, true>), grid, block, 0, st, k);
-    else hipLaunchKernelGGL((distill_grad_small_kernel<T, N, false>), grid, block, 0, st, k);
+template <typename T>
+void small_of(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
+    switch (k.g.C) {
+        case 1: return small<T, 1>(k, grad, num_cu, st);
+        case 2: return small<T, 2>(k, grad, num_cu, st);
+        case 3: return small<T, 3>(k, grad, num_cu, st);
+        case 4: return small<T, 4>(k, grad, num_cu, st);
+        case 5: return small<T, 5>(k, grad, num_cu, st);
+        case 6: return small<T, 6>(k, grad, num_cu, st);
+        case 7: return small<T, 7>(k, grad, num_cu, st);
+        default: return small<T, 8>(k, grad, num_cu, st);
+    }
 }
 template <typename T, int G>
 void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
@@ -805,18 +909,7 @@ template <typename T>
 void launch(const DistillK &k, int num_cu, hipStream_t st) {
     const LogitsK &g = k.g;
     const bool contig = contiguous(g);
-    if (g.C <= 8) {
-        switch (g.C) {
-            case 1: return small<T, 1>(k, contig, num_cu, st);
-            case 2: return small<T, 2>(k, contig, num_cu, st);
-            case 3: return small<T, 3>(k, contig, num_cu, st);
-            case 4: return small<T, 4>(k, contig, num_cu, st);
-            case 5: return small<T, 5>(k, contig, num_cu, st);
-            case 6: return small<T, 6>(k, contig, num_cu, st);
-            case 7: return small<T, 7>(k, contig, num_cu, st);
-            default: return small<T, 8>(k, contig, num_cu, st);
-        }
-    }
+    if (g.C <= 8) return small_of<T>(k, false, num_cu, st);
     if (!contig) {
         // (as in label_scores.hip: a lane a row from 64 rows a compute unit on, or where rows are short)
         if (g.C <= 64 || g.rows >= 64ll * num_cu)
@@ -831,10 +924,16 @@ void launch(const DistillK &k, int num_cu, hipStream_t st) {
     if (g.C <= 256) return group<T, 16>(k, false, num_cu, st);
     if (g.C <= 512) return group<T, 32>(k, false, num_cu, st);
     if (g.C <= 1024) return group<T, 64>(k, false, num_cu, st);
-    const Cut cut = cut_rows(g, num_cu);
+    const Cut cut = cut_rows(g, num_cu, k.tail ? kLongest : 1 << 30);
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
-    if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true>), grid, dim3(256), 0, st, k, cut);
-    else hipLaunchKernelGGL((distill_block_kernel<T, false>), grid, dim3(256), 0, st, k, cut);
+    const unsigned marks = (unsigned)(cut.len + 31) / 32 * 4;
+    if (cut.len >= 16384) {  // (as in label_scores.hip)
+        if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true, 8>), grid, dim3(512), marks, st, k, cut);
+        else hipLaunchKernelGGL((distill_block_kernel<T, false, 8>), grid, dim3(512), 0, st, k, cut);
+    } else {
+        if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true, 4>), grid, dim3(256), marks, st, k, cut);
+        else hipLaunchKernelGGL((distill_block_kernel<T, false, 4>), grid, dim3(256), 0, st, k, cut);
+    }
     if (cut.segs > 1) hipLaunchKernelGGL(distill_join_kernel<T>, dim3(grid_of(g.rows, num_cu, 64)), dim3(64), 0, st, k, cut);
 }
 
@@ -842,18 +941,7 @@ template <typename T>
 void launch_grad(const DistillK &k, int num_cu, hipStream_t st) {
     const LogitsK &g = k.g;
     const bool contig = contiguous(g) && (k.gsc == 1 || g.C == 1);
-    if (g.C <= 8) {
-        switch (g.C) {
-            case 1: return small_grad<T, 1>(k, contig, num_cu, st);
-            case 2: return small_grad<T, 2>(k, contig, num_cu, st);
-            case 3: return small_grad<T, 3>(k, contig, num_cu, st);
-            case 4: return small_grad<T, 4>(k, contig, num_cu, st);
-            case 5: return small_grad<T, 5>(k, contig, num_cu, st);
-            case 6: return small_grad<T, 6>(k, contig, num_cu, st);
-            case 7: return small_grad<T, 7>(k, contig, num_cu, st);
-            default: return small_grad<T, 8>(k, contig, num_cu, st);
-        }
-    }
+    if (g.C <= 8) return small_of<T>(k, true, num_cu, st);
     if (!contig) {
         const int parts = (g.C + 31) / 32;
         hipLaunchKernelGGL(distill_grad_planes_kernel<T>, dim3(grid_of((g.rows + 255) / 256 * parts, num_cu, 64)), dim3(256), 0, st, k, parts);
@@ -865,15 +953,21 @@ void launch_grad(const DistillK &k, int num_cu, hipStream_t st) {
     if (g.C <= 256) return group<T, 16>(k, true, num_cu, st);
     if (g.C <= 512) return group<T, 32>(k, true, num_cu, st);
     if (g.C <= 1024) return group<T, 64>(k, true, num_cu, st);
-    const long long tiles = (g.C + 4095) / 4096;
-    hipLaunchKernelGGL(distill_grad_block_kernel<T>, dim3(grid_of(g.rows * tiles, num_cu, 256)), dim3(256), 0, st, k, tiles);
+    // a row's setup (its teacher) is worth several tiles; eight blocks on every compute unit hide it
+    const long long most = (g.C + 4095) / 4096;
+    long long want = (8ll * num_cu + g.rows - 1) / g.rows;
+    if (want > most) want = most;
+    Cut cut;
+    cut.len = (int)(((g.C + want - 1) / want + 4095) / 4096 * 4096);
+    cut.segs = (g.C + cut.len - 1) / cut.len;
+    hipLaunchKernelGGL(distill_grad_block_kernel<T>, dim3(grid_of(g.rows * cut.segs, num_cu, 64)), dim3(256), 0, st, k, cut);
 }
 
 }  // namespace
 
 size_t distill_workspace_bytes(const DistillK &k, int, int num_cu) {
-    if (k.g.C <= 1024 || !contiguous(k.g)) return 0;
-    const Cut cut = cut_rows(k.g, num_cu);
+    if (k.g.C <= QMRI_SHORT_ROW || !contiguous(k.g)) return 0;
+    const Cut cut = cut_rows(k.g, num_cu, k.tail ? kLongest : 1 << 30);
     return cut.segs > 1 ? (size_t)k.g.rows * cut.segs * 16 : 0;
 }
 

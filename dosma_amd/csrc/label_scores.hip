@@ -14,12 +14,11 @@
 
 namespace qmri {
 
-Cut cut_rows(const LogitsK &g, int num_cu) {
+Cut cut_rows(const LogitsK &g, int num_cu, int longest) {
     // enough blocks for every compute unit twice over, but at least 2048 scores (two rounds of a block's loads) for each
     long long want = g.rows >= 2ll * num_cu ? 1 : (2ll * num_cu + g.rows - 1) / g.rows;
-    const long long most = (g.C + 2047) / 2048;
+    const long long most = (g.C + 2047) / 2048, least = (g.C + longest - 1) / longest;
     if (want > most) want = most;
-    const long long least = (g.C + 65535) / 65536;
     if (want < least) want = least;
     Cut c;
     c.len = (int)(((g.C + want - 1) / want + 63) / 64 * 64);
@@ -133,7 +132,7 @@ __global__ __launch_bounds__(256) void scores_group_kernel(const ScoresK k) {
             const int j = (i * G + gl) * V;
             const Vec<T> r = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[i * V + e] = to_f32(r.v[e]);
+            for (int e = 0; e < V; ++e) x[i * V + e] = get(r, e);
         }
         x[16] = (g.bg && gl == 0) ? 0.f : kNegInf;
         int l;
@@ -177,181 +176,322 @@ __global__ __launch_bounds__(256) void scores_group_kernel(const ScoresK k) {
     }
 }
 
-// ---- the best of a long row: a sorted list over the 64 lanes of a wave ----------------------------------------------------------
-struct Best {
-    float v;  // lane i: the i-th best score seen by this wave
-    int i;    // its label
-    float floor;  // scores that are not above it cannot enter the list (the same in every lane)
-};
-// lane i takes lane i - 1's value
-__device__ __forceinline__ int from_left(int x) { return __builtin_amdgcn_update_dpp(x, x, 0x138, 0xf, 0xf, false); }
-// (wave-uniform v, i): into the list behind everything that is better
-__device__ __forceinline__ void best_insert(Best &b, float v, int i, int k) {
-    const int lane = threadIdx.x & 63;
-    const int pos = __popcll(__ballot(better(b.v, b.i, v, i)));
-    const float lv = __int_as_float(from_left(__float_as_int(b.v)));
-    const int li = from_left(b.i);
-    b.v = lane > pos ? lv : (lane == pos ? v : b.v);
-    b.i = lane > pos ? li : (lane == pos ? i : b.i);
-    b.floor = fmaxf(b.floor, __int_as_float(__builtin_amdgcn_readlane(__float_as_int(b.v), k - 1)));
+// ---- the best of a long row -----------------------------------------------------------------------------------------------------
+// A score can belong to the k best only if it is above a floor for which k others are known.  What passes the floor goes into a
+// buffer of the wave's in LDS; a full buffer is cut down to its k best, whose last is the new floor.  The order is (score falling,
+// label rising), so the result does not depend on who came first.
+__device__ __forceinline__ unsigned ordered(float f) {  // the order of floats as that of unsigned integers; -0 ranks as +0
+    const int u = __float_as_int(f + 0.f);
+    return (unsigned)(u ^ ((u >> 31) | (int)0x80000000));
 }
-// k-th largest of the lanes' values, less one step: k scores at least as large as it are known to exist, so nothing at or below
-// that step can belong to the best k.  A bitonic sort over the wave.
-__device__ __forceinline__ float kth_floor(float c, int k) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int w = 2; w <= 64; w <<= 1)
-#pragma unroll
-        for (int o = w >> 1; o > 0; o >>= 1) {
-            const float p = __shfl_xor(c, o);
-            const bool up = (lane & w) != 0;        // (w = 64: every lane falls)
-            const bool low = (lane & o) == 0;
-            c = (up != low) ? fmaxf(c, p) : fminf(c, p);
-        }
-    const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), k - 1));
-    if (!(f > kNegInf)) return kNegInf;
-    const int u = __float_as_int(f);
-    return f == 0.f ? __int_as_float(0x80000001u) : __int_as_float(f > 0.f ? u - 1 : u + 1);
+__device__ __forceinline__ float unordered(unsigned o) {
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
-// V neighbouring scores a lane, labels rising with the lane: what can still enter the list does.  In the order of the labels, so
-// that of equal scores the lower label comes first and a later equal one is not above the floor.
-template <int V>
-__device__ __forceinline__ void best_take(Best &b, const float (&x)[V], float cm, int first, int k) {
-    unsigned long long m = __ballot(cm > b.floor);
-    if (m == 0ull) return;
-    // many at once (the start of a row, or one that rises): sort the lanes' largest first, which leaves about k of them
-    if (__popcll(m) > 12) {
-        b.floor = fmaxf(b.floor, kth_floor(cm, k));
-        m = __ballot(cm > b.floor);
+constexpr unsigned kKeyNegInf = 0x007fffffu;  // ordered(-inf)
+// significant bits of a widened score's key: the lower ones are all alike
+template <typename T>
+constexpr int kKeyBits = 32;
+template <>
+constexpr int kKeyBits<f16_t> = 19;
+template <>
+constexpr int kKeyBits<bf16_t> = 16;
+
+// Which of the wave's 64 N (key, label) pairs are its k best; key 0: none.  The k-th largest key is found bit by bit.
+template <int N, int BITS>
+__device__ __forceinline__ unsigned select_best(const unsigned (&key)[N], const int (&id)[N], int k, bool (&win)[N]) {
+    auto count = [&](auto f) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += __popcll(__ballot(f(i)));
+        return c;
+    };
+    unsigned t = 0u;
+    for (int bit = 31; bit >= 32 - BITS; --bit) {
+        const unsigned at = t | (1u << bit);
+        if (count([&](int i) { return key[i] >= at; }) >= k) t = at;
     }
-    while (m) {
-        const int l = __ffsll(m) - 1;
-        m &= m - 1;
-        const int at = __builtin_amdgcn_readlane(first, l);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x[e]), l));
-            if (v > b.floor) best_insert(b, v, at + e, k);
+    // keys that agree with t in the significant bits are equal scores: of those the lowest labels
+    const unsigned top = BITS == 32 ? 0xffffffffu : ~((1u << (32 - BITS)) - 1u);
+    const int above = count([&](int i) { return (key[i] & top) > t; });
+    int last = 0x7fffffff;
+    if (t != 0u && above + count([&](int i) { return (key[i] & top) == t; }) > k) {
+        last = 0;
+        for (int bit = 30; bit >= 0; --bit) {  // the largest label of which fewer than k - above equals lie below
+            const int at = last | (1 << bit);
+            if (count([&](int i) { return (key[i] & top) == t && id[i] < at; }) < k - above) last = at;
         }
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) win[i] = key[i] != 0u && ((key[i] & top) > t || ((key[i] & top) == t && id[i] <= last));
+    return t;
 }
 
-// a segment's part of a row in the workspace: m, s (relative to reference(m)), t, then the list's scores and labels
+constexpr int kBuf = 192;
+struct WaveBest {
+    float *v;  // [kBuf] in LDS, this wave's
+    int *i;
+    int n;     // pairs in it
+    // a pair that does not come before (floor, bound) cannot be among the best
+    float floor;
+    int bound;
+    int k;
+    // where the set lanes of a ballot find their places
+    static __device__ __forceinline__ int place(unsigned long long m) {
+        return __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0u));
+    }
+    __device__ __forceinline__ bool passes(float x, int label) const { return x > floor || (x == floor && label < bound); }
+    template <int BITS>
+    __device__ __forceinline__ void cut() {
+        wave_sync();
+        const int lane = threadIdx.x & 63;
+        unsigned key[kBuf / 64];
+        int id[kBuf / 64];
+        float sv[kBuf / 64];
+        bool win[kBuf / 64];
+#pragma unroll
+        for (int q = 0; q < kBuf / 64; ++q) {
+            const int j = q * 64 + lane;
+            sv[q] = j < n ? v[j] : 0.f;
+            id[q] = j < n ? i[j] : 0;
+            key[q] = j < n ? ordered(sv[q]) : 0u;
+        }
+        select_best<kBuf / 64, BITS>(key, id, k, win);
+        wave_sync();
+        const bool full = n >= k;
+        n = 0;
+        float worst = __builtin_inff();
+#pragma unroll
+        for (int q = 0; q < kBuf / 64; ++q) {
+            const unsigned long long m = __ballot(win[q]);
+            if (win[q]) {
+                v[n + place(m)] = sv[q];
+                i[n + place(m)] = id[q];
+                worst = fminf(worst, sv[q]);
+            }
+            n += __popcll(m);
+        }
+        if (full) {  // the last of the best
+            floor = -group_max<64>(-worst);
+            int last = -1;
+#pragma unroll
+            for (int q = 0; q < kBuf / 64; ++q) last = win[q] && sv[q] == floor && id[q] > last ? id[q] : last;
+            bound = -group_min<64>(-last);
+        }
+        wave_sync();
+    }
+    // one pair a lane
+    template <int BITS>
+    __device__ __forceinline__ void take(float x, int label, bool in) {
+        if (__ballot(in && passes(x, label)) == 0ull) return;
+        if (n + 64 > kBuf) cut<BITS>();
+        const bool yes = in && passes(x, label);
+        const unsigned long long m = __ballot(yes);
+        if (yes) {
+            v[n + place(m)] = x;
+            i[n + place(m)] = label;
+        }
+        n += __popcll(m);
+    }
+};
+
+// The floor that 64 N values (N a lane) give: k of them are at least as large as the k-th, so only what is above a lower value
+// can be among the best.
+template <int N>
+__device__ __forceinline__ float first_floor(const float *m, int k) {
+    const int lane = threadIdx.x & 63;
+    unsigned key[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) key[q] = ordered(m[q * 64 + lane]);
+    unsigned t = 0u;
+    for (int bit = 31; bit >= 12; --bit) {  // (the upper 20 bits will do: a floor that is a little low only lets more through)
+        const unsigned at = t | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int q = 0; q < N; ++q) c += __popcll(__ballot(key[q] >= at));
+        if (c >= k) t = at;
+    }
+    return t > kKeyNegInf + 0x1000u ? unordered(t - 0x1000u) : kNegInf;  // (the next lower of these 20-bit keys)
+}
+
+// Up to 64 winners, one a lane (i < 0: none), into falling order: every lane counts the better ones.
+__device__ __forceinline__ int rank_of(float v, int i, int k) {
+    int r = 0;
+    for (int o = 0; o < k; ++o) {
+        const float ov = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), o));
+        const int oi = __builtin_amdgcn_readlane(i, o);
+        r += (oi >= 0 && (i < 0 || better(ov, oi, v, i))) ? 1 : 0;
+    }
+    return r;
+}
+
+// a segment's part of a row in the workspace: m, s (relative to reference(m)), t, then its best scores and their labels
 __device__ __forceinline__ size_t part_words(int k) { return 4 + 2 * (size_t)k; }
 
-// ---- block: four waves a segment of a row -----------------------------------------------------------------------------------
-// Per score: widen, subtract, multiply, clamp, exp2, two sums -- about 10 issue slots, of the 14 that a 2-byte score has at 5.5
-// TB/s: memory first, the vector unit close behind.  A lane's reference follows its maximum only when that has grown by more than
-// a factor of 16, so nearly no step pays for a change of reference.
-constexpr float kSlack = 4.f;
+// The W waves' lists, up to 64 pairs each at v, i + w * kBuf (i < 0: none), together: the k best to lanes 0 .. k - 1 of the wave
+// that asks, in falling order.  The lists are overwritten.
+template <int W, int BITS>
+__device__ __forceinline__ void final_best(float *tv, int *ti, int k, float &bv, int &bi) {
+    const int lane = threadIdx.x & 63;
+    unsigned key[W];
+    int id[W];
+    float sv[W];
+    bool win[W];
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+        id[q] = ti[q * kBuf + lane];
+        sv[q] = tv[q * kBuf + lane];
+        key[q] = id[q] < 0 ? 0u : ordered(sv[q]);
+    }
+    wave_sync();
+    select_best<W, BITS>(key, id, k, win);
+    int n = 0;
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+        const unsigned long long m = __ballot(win[q]);
+        if (win[q]) {
+            tv[n + WaveBest::place(m)] = sv[q];
+            ti[n + WaveBest::place(m)] = id[q];
+        }
+        n += __popcll(m);
+    }
+    wave_sync();
+    bv = lane < n ? tv[lane] : kNegInf;
+    bi = lane < n ? ti[lane] : -1;
+    const int r = rank_of(bv, bi, n);
+    wave_sync();
+    if (lane < n) {
+        tv[r] = bv;
+        ti[r] = bi;
+    }
+    wave_sync();
+    bv = lane < n ? tv[lane] : kNegInf;
+    bi = lane < n ? ti[lane] : -1;
+}
 
-template <typename T, bool TOP>
-__global__ __launch_bounds__(256) void scores_block_kernel(const ScoresK k, const Cut cut) {
-    __shared__ RowStat s_stat[4];
-    __shared__ float s_v[4][64];
-    __shared__ int s_i[4][64];
+// ---- block: W waves a segment of a row ------------------------------------------------------------------------------------------
+// Per score: widen, half a maximum, one fused multiply, clamp, exp2 (two slots), one and a half sums -- about 8 issue slots, of
+// the 14 that a 2-byte score has at 5.5 TB/s: memory first, the vector unit close behind.
+template <typename T, bool TOP, int W>
+__global__ __launch_bounds__(64 * W, TOP ? 5 : 8) void scores_block_kernel(const ScoresK k, const Cut cut) {
+    __shared__ RowStat s_stat[W];
+    __shared__ float s_max[TOP ? 64 * W : 1];  // the lanes' largest, or the scores of up to four lanes of each wave
+    __shared__ int s_first[TOP ? 4 * W : 1];
+    __shared__ float s_v[TOP ? W * kBuf : 1];
+    __shared__ int s_i[TOP ? W * kBuf : 1];
     const LogitsK &g = k.g;
-    constexpr int V = kVec<T>, U = 16 / V, TILE = 64 * 16;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    constexpr int TILE = 1024, BITS = kKeyBits<T>;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long work = g.rows * cut.segs;
     for (long long item = blockIdx.x; item < work; item += gridDim.x) {
         const long long n = cut.segs == 1 ? item : item / cut.segs;
         const int seg = cut.segs == 1 ? 0 : (int)(item - n * cut.segs);
         const int c0 = seg * cut.len, c1 = c0 + cut.len < g.C ? c0 + cut.len : g.C;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
-        RowStat r = no_stat();
-        Best b = {kNegInf, -1, kNegInf};
-        if (g.bg && seg == 0 && w == 0) {  // the implicit category: lane 0 has seen a score of 0
-            if (lane == 0) r = {0.f, 0.f, 1.f, 0.f};
-            if (TOP) best_insert(b, 0.f, 0, k.top);
-        }
-        Vec<T> nx[U];
-        auto fetch = [&](int c) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = c + u * 64 * V + lane * V;
-                nx[u] = j + V <= c1 ? load_vec(z + j) : load_part(z + j, c1 - j);
+        const bool back = g.bg && seg == 0 && w == 0;
+        Running r = no_scores();
+        if (back && lane == 0) r = {0.f, 0.f, 1.f, 0.f};  // the implicit category: lane 0 has seen a score of 0
+        WaveBest b = {s_v + (TOP ? w * kBuf : 0), s_i + (TOP ? w * kBuf : 0), 0, kNegInf, 0, k.top};
+        // the best k of the lanes' largest so far: nothing below the last of them can be among the best of the row
+        auto raise_floor = [&](float m) {
+            s_max[threadIdx.x] = m;
+            __syncthreads();
+            const float f = first_floor<W>(s_max, k.top);
+            if (f > b.floor) {
+                b.floor = f;
+                b.bound = 0;
             }
+            __syncthreads();
         };
+        const int rounds = (c1 - c0 + W * TILE - 1) / (W * TILE);
         int c = c0 + w * TILE;
-        if (c < c1) fetch(c);
-        for (; c < c1; c += 4 * TILE) {
-            Vec<T> now[U];
+        Tile<T> next;
+        if (c < c1) next = load_tile(z + c, c1 - c);
+        for (int it = 0; it < rounds; ++it, c += W * TILE) {
+            const bool mine = c < c1;
+            float x[16];
+            if (mine) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) now[u] = nx[u];
-            if (c + 4 * TILE < c1) fetch(c + 4 * TILE);
-            float x[16], um[U], cm = kNegInf;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                um[u] = kNegInf;
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    x[u * V + e] = to_f32(now[u].v[e]);
-                    um[u] = maxn(um[u], x[u * V + e]);
-                }
-                cm = maxn(cm, um[u]);
+                for (int i = 0; i < 16; ++i) x[i] = get(next.v[i / kVec<T>], i % kVec<T>);
+                if (c + W * TILE < c1) next = load_tile(z + c + W * TILE, c1 - c - W * TILE);
             }
-            r.m = maxn(r.m, cm);
-            if ((cm - r.ref) * g.c2 > kSlack) rebase(r, cm, g.c2);
-            float e[16], et[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float d = clamp2((x[i] - r.ref) * g.c2);
-                e[i] = exp2_hw(d);
-                et[i] = e[i] * d;
-            }
-            r.s += tree_sum(e);
-            r.t += tree_sum(et);
-            if (TOP) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    float xv[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) xv[i] = x[u * V + i];
-                    best_take<V>(b, xv, um[u], c + u * 64 * V + lane * V + g.bg, k.top);
+            if (TOP && it == 0) {
+                float cm = back && lane == 0 ? 0.f : kNegInf;
+                if (mine) cm = fmaxf(cm, max_of(x));
+                raise_floor(cm);
+                if (back && b.passes(0.f, 0)) {
+                    if (lane == 0) {
+                        b.v[0] = 0.f;
+                        b.i[0] = 0;
+                    }
+                    b.n = 1;
                 }
             }
+            if (mine) {
+                add_scores(r, x, g.c2);
+                if (TOP) {
+                    // lanes that hold something for the list hand their 16 scores over through LDS, four lanes at a time, so that
+                    // all 64 lanes look at one each
+                    float *stage = s_max + w * 64;
+                    for (unsigned long long m = __ballot(max_of(x) >= b.floor); m != 0ull;) {
+                        const int rank = WaveBest::place(m);
+                        const bool give = (m >> lane) & 1ull && rank < 4;
+                        if (give) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) stage[rank * 16 + i] = x[i];
+                            s_first[w * 4 + rank] = lane;
+                        }
+                        const int have = __popcll(m) < 4 ? __popcll(m) : 4;
+                        m &= ~__ballot(give);
+                        wave_sync();
+                        const int from = s_first[w * 4 + (lane >> 4)];
+                        const float v = stage[lane];
+                        wave_sync();
+                        b.take<BITS>(v, c + tile_at<T>(from, lane & 15) + g.bg, (lane >> 4) < have);
+                    }
+                }
+            }
+            // every time the scores seen have doubled
+            if (TOP && it > 0 && (it & (it + 1)) == 0 && it + 1 < rounds) raise_floor(r.m);
         }
-        r = wave_join(r, g.c2);
-        if (lane == 0) s_stat[w] = r;
+        RowStat st = wave_stat(r, g.c2, [&](int j) {
+            // (w's scores in the order of its tiles; -1: the implicit category, seen by lane 0)
+            if (j < 0) return lane == 0 ? 0.f : kNegInf;
+            const int at = c0 + (j / TILE) * W * TILE + w * TILE + j % TILE;
+            return at < c1 ? to_f32(z[at]) : kNegInf;
+        }, back ? lane - 64 : lane, 64, rounds * TILE);
+        if (lane == 0) s_stat[w] = st;
         if (TOP) {
-            s_v[w][lane] = b.v;
-            s_i[w][lane] = b.i;
+            if (b.n > k.top) b.cut<BITS>();
+            for (int q = b.n + lane; q < 64; q += 64) b.i[q] = -1;
         }
         __syncthreads();
         if (w == 0) {
-            r = join(join(s_stat[0], s_stat[1], g.c2), join(s_stat[2], s_stat[3], g.c2), g.c2);
-            if (TOP) {
-                for (int o = 1; o < 4; ++o)
-                    for (int q = 0; q < k.top; ++q) {
-                        const float v = s_v[o][q];
-                        const int i = s_i[o][q];
-                        const float kv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(b.v), k.top - 1));
-                        const int ki = __builtin_amdgcn_readlane(b.i, k.top - 1);
-                        if (i < 0 || (ki >= 0 && !better(v, i, kv, ki))) break;  // (the other lists fall too)
-                        best_insert(b, v, i, k.top);
-                    }
-            }
+            st = s_stat[0];
+#pragma unroll
+            for (int o = 1; o < W; ++o) st = join(st, s_stat[o], g.c2);
+            float bv = kNegInf;
+            int bi = -1;
+            if (TOP) final_best<W, BITS>(s_v, s_i, k.top, bv, bi);
             if (cut.segs > 1) {
                 float *p = static_cast<float *>(k.ws) + (size_t)item * part_words(TOP ? k.top : 0);
                 if (lane == 0) {
-                    p[0] = r.m;
-                    p[1] = r.s;
-                    p[2] = r.t;
+                    p[0] = st.m;
+                    p[1] = st.s;
+                    p[2] = st.t;
                 }
                 if (TOP && lane < k.top) {
-                    p[4 + lane] = b.v;
-                    reinterpret_cast<int *>(p)[4 + k.top + lane] = b.i;
+                    p[4 + lane] = bv;
+                    reinterpret_cast<int *>(p)[4 + k.top + lane] = bi;
                 }
             } else {
-                const float ls = __builtin_amdgcn_logf(r.s) * kLn2;
-                if (TOP && lane < k.top) write_top(k, n, lane, b.v, b.i, r.m, ls);
+                const float ls = __builtin_amdgcn_logf(st.s) * kLn2;
+                if (TOP && lane < k.top) write_top(k, n, lane, bv, bi, st.m, ls);
                 if (lane == 0) {
                     int l;
                     bool has, ignored;
                     given_label(k, n, g.C + g.bg, l, has, ignored);
                     const float zl = (has && l >= g.bg) ? to_f32(z[l - g.bg]) : 0.f;
-                    write_row(k, n, r.m, r.s, r.t, has, ignored, zl);
+                    write_row(k, n, st.m, st.s, st.t, has, ignored, zl);
                 }
             }
         }
@@ -359,46 +499,58 @@ __global__ __launch_bounds__(256) void scores_block_kernel(const ScoresK k, cons
     }
 }
 
-// The segments' parts of a row together: one wave a row.
+// The segments' parts of a row together: a block a row, its waves a quarter of the segments each.
 template <typename T>
-__global__ __launch_bounds__(64) void scores_join_kernel(const ScoresK k, const Cut cut) {
+__global__ __launch_bounds__(256) void scores_join_kernel(const ScoresK k, const Cut cut) {
+    __shared__ RowStat s_stat[4];
+    __shared__ float s_v[4 * kBuf];
+    __shared__ int s_i[4 * kBuf];
+    constexpr int BITS = kKeyBits<T>;
     const LogitsK &g = k.g;
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     for (long long n = blockIdx.x; n < g.rows; n += gridDim.x) {
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
         const size_t words = part_words(k.top);
         const float *p = static_cast<const float *>(k.ws) + (size_t)n * cut.segs * words;
-        int l;
-        bool has, ignored;
-        given_label(k, n, g.C + g.bg, l, has, ignored);
-        const float zl = (has && l >= g.bg) ? to_f32(z[l - g.bg]) : 0.f;
+        int l = -1;
+        bool has = false, ignored = false;
+        float zl = 0.f;
+        if (w == 0) {
+            given_label(k, n, g.C + g.bg, l, has, ignored);
+            if (has && l >= g.bg) zl = to_f32(z[l - g.bg]);
+        }
         RowStat r = no_stat();
-        for (int q = lane; q < cut.segs; q += 64) {
+        for (int q = threadIdx.x; q < cut.segs; q += 256) {
             const float *a = p + q * words;
-            RowStat o = {a[0], reference(a[0]), a[1], a[2]};
-            r = join(r, o, g.c2);
+            r = join(r, {a[0], reference(a[0]), a[1], a[2]}, g.c2);
         }
         r = wave_join(r, g.c2);
-        if (lane == 0) write_row(k, n, r.m, r.s, r.t, has, ignored, zl);
+        if (lane == 0) s_stat[w] = r;
+        WaveBest b = {s_v + w * kBuf, s_i + w * kBuf, 0, kNegInf, 0, k.top};
         if (k.top) {
-            Best b = {kNegInf, -1, kNegInf};
-            for (int q0 = 0; q0 < cut.segs; q0 += 64) {
-                // the segments' best, a lane a segment; a segment whose list cannot add anything is passed over
-                for (int q = q0; q < cut.segs && q < q0 + 64; ++q) {
-                    const float *a = p + q * words;
-                    const float sv = lane < k.top ? a[4 + lane] : kNegInf;
-                    const int si = lane < k.top ? reinterpret_cast<const int *>(a)[4 + k.top + lane] : -1;
-                    for (int i = 0; i < k.top; ++i) {
-                        const float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sv), i));
-                        const int id = __builtin_amdgcn_readlane(si, i);
-                        if (id < 0 || !(v > b.floor)) break;  // (segments come in the order of their labels: an equal score is too late)
-                        best_insert(b, v, id, k.top);
-                    }
-                }
+            const int pairs = cut.segs * k.top;
+            for (int q0 = w * 64; q0 < pairs; q0 += 256) {
+                const int q = q0 + lane, sg = q / k.top, at = q - sg * k.top;
+                const float *a = p + sg * words + 4;
+                const bool in = q < pairs;
+                b.take<BITS>(in ? a[at] : kNegInf, in ? reinterpret_cast<const int *>(a)[k.top + at] : -1, in);
             }
-            const float ls = __builtin_amdgcn_logf(r.s) * kLn2;
-            if (lane < k.top) write_top(k, n, lane, b.v, b.i, r.m, ls);
+            if (b.n > k.top) b.cut<BITS>();
+            for (int q = b.n + lane; q < 64; q += 64) b.i[q] = -1;
         }
+        __syncthreads();
+        if (w == 0) {
+            r = join(join(s_stat[0], s_stat[1], g.c2), join(s_stat[2], s_stat[3], g.c2), g.c2);
+            if (lane == 0) write_row(k, n, r.m, r.s, r.t, has, ignored, zl);
+            if (k.top) {
+                float bv;
+                int bi;
+                final_best<4, BITS>(s_v, s_i, k.top, bv, bi);
+                const float ls = __builtin_amdgcn_logf(r.s) * kLn2;
+                if (lane < k.top) write_top(k, n, lane, bv, bi, r.m, ls);
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -477,51 +629,67 @@ __global__ __launch_bounds__(256) void scores_planes_kernel(const ScoresK k) {
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
         std::conditional_t<KEY, LaneBestKey<T, K>, LaneBest<T, K>> best;
         best.clear();
-        RowStat r = no_stat();
+        Running r = no_scores();
         if (g.bg) {
             r = {0.f, 0.f, 1.f, 0.f};
             if (K) best.take(static_cast<T>(0.f), 0.f, 0);
         }
-        for (int c = 0; c < g.C; c += 8) {
-            T raw[8];
+        auto eight = [&](const T (&raw)[8], int c) {
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) raw[i] = c + i < g.C ? z[(long long)(c + i) * g.sc] : static_cast<T>(kNegInf);
-            float x[8], cm = kNegInf;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = to_f32(raw[i]);
-                cm = maxn(cm, x[i]);
-            }
-            r.m = maxn(r.m, cm);
-            if ((cm - r.ref) * g.c2 > kSlack) rebase(r, cm, g.c2);
-            float e[8], et[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = clamp2((x[i] - r.ref) * g.c2);
-                e[i] = exp2_hw(d);
-                et[i] = e[i] * d;
-            }
-            r.s += tree_sum(e);
-            r.t += tree_sum(et);
+            for (int i = 0; i < 8; ++i) x[i] = to_f32(raw[i]);
+            add_scores(r, x, g.c2);
             if (K) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) best.take(raw[i], x[i], c + i + g.bg);
             }
+        };
+        const int whole = g.C & ~7;
+        T next[8];
+        const T *p = z;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) next[i] = p[i * g.sc];  // (more than 8 classes here)
+        for (int c = 0; c < whole; c += 8) {
+            T raw[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[i] = next[i];
+            p += 8 * g.sc;
+            if (c + 16 <= g.C) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) next[i] = p[i * g.sc];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) next[i] = c + 8 + i < g.C ? p[i * g.sc] : static_cast<T>(kNegInf);
+            }
+            eight(raw, c);
         }
-        rebase(r, reference(r.m), g.c2);
+        if (whole < g.C) eight(next, whole);
+        RowStat st = {r.m, reference(r.m), 0.f, 0.f};
+        if (far_scores(r.m, g.c2)) {
+            for (int c = -g.bg; c < g.C; ++c) {
+                const float d = clamp2(((c < 0 ? 0.f : to_f32(z[(long long)c * g.sc])) - st.ref) * g.c2), e = exp2_hw(d);
+                st.s += e;
+                st.t = fmaf(e, d, st.t);
+            }
+        } else {
+            float d;
+            const float f = to_reference(r, r.m, g.c2, d);
+            st.s = r.s * f;
+            st.t = f * fmaf(d, r.s, r.t);
+        }
         if (!live) continue;
         int l;
         bool has, ignored;
         given_label(k, n, g.C + g.bg, l, has, ignored);
         const float zl = (has && l >= g.bg) ? to_f32(z[(long long)(l - g.bg) * g.sc]) : 0.f;
-        write_row(k, n, r.m, r.s, r.t, has, ignored, zl);
+        write_row(k, n, st.m, st.s, st.t, has, ignored, zl);
         if (K) {
-            const float ls = __builtin_amdgcn_logf(r.s) * kLn2;
+            const float ls = __builtin_amdgcn_logf(st.s) * kLn2;
 #pragma unroll
             for (int q = 0; q < K; ++q)
                 if (q < k.top) {
                     const float v = best.score(q);
-                    write_top(k, n, q, v, v > kNegInf ? best.label(q) : -1, r.m, ls);
+                    write_top(k, n, q, v, v > kNegInf ? best.label(q) : -1, st.m, ls);
                 }
         }
     }
@@ -534,49 +702,47 @@ __device__ __forceinline__ float category(const LogitsK &g, const T *z, int j) {
 }
 template <typename T>
 __global__ __launch_bounds__(256) void scores_wave_kernel(const ScoresK k) {
+    __shared__ float s_v[4 * kBuf];
+    __shared__ int s_i[4 * kBuf];
+    constexpr int BITS = kKeyBits<T>;
     const LogitsK &g = k.g;
-    const int lane = threadIdx.x & 63, cats = g.C + g.bg;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, cats = g.C + g.bg;
     const long long nw = (long long)gridDim.x * 4;
-    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < g.rows; n += nw) {
+    for (long long n = (long long)blockIdx.x * 4 + w; n < g.rows; n += nw) {
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
-        RowStat r = no_stat();
-        Best b = {kNegInf, -1, kNegInf};
+        Running u = no_scores();
+        WaveBest b = {s_v + w * kBuf, s_i + w * kBuf, 0, kNegInf, 0, k.top};
+        auto score = [&](int j) { return j < cats ? category(g, z, j) : kNegInf; };
         for (int j0 = 0; j0 < cats; j0 += 256) {
-            float x[4], cm = kNegInf;
+            float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = j0 + i * 64 + lane;
-                x[i] = j < cats ? category(g, z, j) : kNegInf;
-                cm = maxn(cm, x[i]);
-            }
-            r.m = maxn(r.m, cm);
-            if ((cm - r.ref) * g.c2 > kSlack) rebase(r, cm, g.c2);
-            float e[4], et[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float d = clamp2((x[i] - r.ref) * g.c2);
-                e[i] = exp2_hw(d);
-                et[i] = e[i] * d;
-            }
-            r.s += tree_sum(e);
-            r.t += tree_sum(et);
+            for (int i = 0; i < 4; ++i) x[i] = score(j0 + i * 64 + lane);
+            add_scores(u, x, g.c2);
             if (k.top) {
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
-                    const float xv[1] = {x[i]};
-                    best_take<1>(b, xv, x[i], j0 + i * 64 + lane, k.top);
+                    const float v = i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : x[3];
+                    b.take<BITS>(v, j0 + i * 64 + lane, true);
                 }
             }
         }
-        r = wave_join(r, g.c2);
+        const RowStat r = wave_stat(u, g.c2, score, lane, 64, cats);
         if (lane == 0) {
             int l;
             bool has, ignored;
             given_label(k, n, cats, l, has, ignored);
             write_row(k, n, r.m, r.s, r.t, has, ignored, has ? category(g, z, l) : 0.f);
         }
-        const float ls = __builtin_amdgcn_logf(r.s) * kLn2;
-        if (lane < k.top) write_top(k, n, lane, b.v, b.i, r.m, ls);
+        if (k.top) {
+            b.cut<BITS>();
+            float bv = lane < b.n ? b.v[lane] : kNegInf;
+            int bi = lane < b.n ? b.i[lane] : -1;
+            const int at = rank_of(bv, bi, b.n);
+            const float ls = __builtin_amdgcn_logf(r.s) * kLn2;
+            // (lanes without a winner keep their own slot: they come behind the winners)
+            if (lane < k.top) write_top(k, n, lane < b.n ? at : lane, bv, bi, r.m, ls);
+            wave_sync();
+        }
     }
 }
 
@@ -661,10 +827,11 @@ __global__ __launch_bounds__(256) void scores_grad_group_kernel(const ScoresK k)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = (i * G + gl) * V;
+            float y[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[i].v[e] = from_f32<T>(grad_score(r, g.c2, g.invT, to_f32(x[i].v[e]), j + e + g.bg));
-            if (j + V <= g.C) __builtin_memcpy(out + j, &x[i], 16);
-            else store_part(out + j, x[i], g.C - j);
+            for (int e = 0; e < V; ++e) y[e] = grad_score(r, g.c2, g.invT, get(x[i], e), j + e + g.bg);
+            if (j + V <= g.C) store_vec(out + j, pack_vec<T>(y));
+            else store_part(out + j, y, g.C - j);
         }
     }
 }
@@ -689,10 +856,11 @@ __global__ __launch_bounds__(256) void scores_grad_block_kernel(const ScoresK k,
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = c0 + (i * 256 + threadIdx.x) * V;
+            float y[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[i].v[e] = from_f32<T>(grad_score(r, g.c2, g.invT, to_f32(x[i].v[e]), j + e + g.bg));
-            if (j + V <= g.C) __builtin_memcpy(out + j, &x[i], 16);
-            else store_part(out + j, x[i], g.C - j);
+            for (int e = 0; e < V; ++e) y[e] = grad_score(r, g.c2, g.invT, get(x[i], e), j + e + g.bg);
+            if (j + V <= g.C) store_vec(out + j, pack_vec<T>(y));
+            else store_part(out + j, y, g.C - j);
         }
     }
 }
@@ -800,11 +968,17 @@ void launch(const ScoresK &k, int num_cu, hipStream_t st) {
     if (g.C <= 256) return group<T, 16>(k, false, num_cu, st);
     if (g.C <= 512) return group<T, 32>(k, false, num_cu, st);
     if (g.C <= 1024) return group<T, 64>(k, false, num_cu, st);
-    const Cut cut = cut_rows(g, num_cu);
+    const Cut cut = cut_rows(g, num_cu, 1 << 30);
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
-    if (k.top) hipLaunchKernelGGL((scores_block_kernel<T, true>), grid, dim3(256), 0, st, k, cut);
-    else hipLaunchKernelGGL((scores_block_kernel<T, false>), grid, dim3(256), 0, st, k, cut);
-    if (cut.segs > 1) hipLaunchKernelGGL(scores_join_kernel<T>, dim3(grid_of(g.rows, num_cu, 64)), dim3(64), 0, st, k, cut);
+    // eight waves where the segments are long enough for two rounds of all of them: the loads in flight bound the rate
+    if (k.top) {
+        hipLaunchKernelGGL((scores_block_kernel<T, true, 4>), grid, dim3(256), 0, st, k, cut);
+    } else if (cut.len >= 16384) {
+        hipLaunchKernelGGL((scores_block_kernel<T, false, 8>), grid, dim3(512), 0, st, k, cut);
+    } else {
+        hipLaunchKernelGGL((scores_block_kernel<T, false, 4>), grid, dim3(256), 0, st, k, cut);
+    }
+    if (cut.segs > 1) hipLaunchKernelGGL(scores_join_kernel<T>, dim3(grid_of(g.rows, num_cu, 64)), dim3(256), 0, st, k, cut);
 }
 
 template <typename T>
@@ -841,8 +1015,8 @@ void launch_grad(const ScoresK &k, int num_cu, hipStream_t st) {
 }  // namespace
 
 size_t label_scores_workspace_bytes(const ScoresK &k, int, int num_cu) {
-    if (k.g.C <= 1024 || !contiguous(k.g)) return 0;
-    const Cut cut = cut_rows(k.g, num_cu);
+    if (k.g.C <= QMRI_SHORT_ROW || !contiguous(k.g)) return 0;
+    const Cut cut = cut_rows(k.g, num_cu, 1 << 30);
     return cut.segs > 1 ? (size_t)k.g.rows * cut.segs * (4 + 2 * (size_t)k.top) * 4 : 0;
 }
 

@@ -71,53 +71,72 @@ def _rows_of(shape, strides, dim):
 
 
 # ---- torch ---------------------------------------------------------------------------------------------------------------
+_names = {}  # torch dtype -> "float32", ..
+
+
 def _name(dtype):
-    return str(dtype)[6:]  # torch.float32 -> float32
+    name = _names.get(dtype)
+    if name is None:
+        name = _names[dtype] = str(dtype)[6:]
+    return name
 
 
 def _tensor_logits(x, dim):
+    """-> (scores, axis, shape of the rows, Rows); a copy of the scores where their rows need more than two strides."""
     if not x.is_cuda:
         raise ValueError("logits must be a tensor on the GPU or a numpy array")
     if _name(x.dtype) not in _lib.SCORE_DTYPES:
         raise ValueError(f"logits must be float32, float16 or bfloat16, got {x.dtype}")
-    dim = _check_dim(x.ndim, dim)
+    ndim = x.ndim
+    dim = _check_dim(ndim, dim)
+    if dim == ndim - 1 and x.is_contiguous():
+        C = x.shape[dim]
+        return x, dim, x.shape[:-1], _lib.Rows(x.numel() // C if C else 0, C)
     shape, rows = _rows_of(x.shape, x.stride(), dim)
-    if rows is None:  # more than two row strides: one dense copy
+    if rows is None:
         x = x.contiguous()
         shape, rows = _rows_of(x.shape, x.stride(), dim)
     return x, dim, shape, rows
 
 
-def _tensor_arg(name, t, shape, device, dtypes, last=None):
-    """A per-row argument, dense.  ``last``: size of its extra last axis."""
+def _tensor_arg(name, t, shape, device, dtypes, last=()):
+    """A per-row argument, dense.  ``last``: its extra last axis."""
     if not _is_torch(t):
         raise ValueError(f"{name} must be a tensor like the logits")
-    want = tuple(shape) + (() if last is None else (last,))
-    if tuple(t.shape) != want:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {want}")
+    if t.shape != shape + last:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape + last)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the logits are on {device}")
     if _name(t.dtype) not in dtypes:
         raise ValueError(f"{name} must be one of {', '.join(sorted(dtypes))}, got {t.dtype}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+_F32 = ("float32",)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 class _TorchCall:
     """Results and workspace from torch's allocator, work on torch's current stream of the logits' device."""
 
+    __slots__ = ("torch", "device", "index", "stream", "held")
+
     def __init__(self, x):
-        import torch
+        self.torch = torch = sys.modules["torch"]
+        self.device = x.device
+        self.index = x.get_device()
+        self.stream = torch._C._cuda_getCurrentRawStream(self.index)
 
-        self.torch, self.device = torch, x.device
-        self.stream = torch.cuda.current_stream(x.device).cuda_stream
-        self.held = []
-
-    def empty(self, shape, dtype="float32"):
-        return self.torch.empty(shape, dtype=getattr(self.torch, dtype), device=self.device)
+    def empty(self, shape, dtype=None):
+        return self.torch.empty(shape, dtype=self.torch.float32 if dtype is None else dtype, device=self.device)
 
     def workspace(self, nbytes):
-        self.held.append(self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device))
-        return self.held[-1].data_ptr()
+        # kept until the call is enqueued; torch's allocator hands it out again only to work behind this on the same stream
+        self.held = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
+        return self.held.data_ptr()
 
     def grad_like(self, x, dim):
         g = self.torch.empty_like(x)
@@ -127,72 +146,80 @@ class _TorchCall:
             rows = _rows_of(g.shape, g.stride(), dim)[1]
         return g, rows
 
-    def kw(self):
-        return {"device": self.device.index, "stream": self.stream}
-
 
 def _scores_tensor(x, labels, dim, top, norm, temperature, background, ignore_label):
     x, dim, shape, rows = _tensor_logits(x, dim)
     call = _TorchCall(x)
-    lab = None if labels is None else _tensor_arg("labels", labels, shape, x.device, _lib.L_KINDS)
-    out = LabelScores(None if lab is None else call.empty(shape), call.empty(shape), call.empty(shape + (2,)) if norm else None,
-                      call.empty(shape + (top,)) if top > 0 else None, call.empty(shape + (top,), "int32") if top > 0 else None)
-    ptr = [None if t is None else t.data_ptr() for t in out]
-    _lib.label_scores(x.data_ptr(), _name(x.dtype), rows, labels_ptr=None if lab is None else lab.data_ptr(),
-                      l_dtype=None if lab is None else _name(lab.dtype), top=top, ignore_label=ignore_label,
-                      temperature=temperature, background=background, log_prob=ptr[0], entropy=ptr[1], norm=ptr[2],
-                      top_log_prob=ptr[3], top_label=ptr[4], workspace=call.workspace, **call.kw())
+    l_dtype = None
+    if labels is not None:
+        labels = _tensor_arg("labels", labels, shape, x.device, _lib.L_KINDS)
+        l_dtype = _name(labels.dtype)
+    out = LabelScores(None if labels is None else call.empty(shape), call.empty(shape), call.empty(shape + (2,)) if norm else None,
+                      call.empty(shape + (top,)) if top > 0 else None,
+                      call.empty(shape + (top,), call.torch.int32) if top > 0 else None)
+    _lib.label_scores(x.data_ptr(), _name(x.dtype), rows, labels_ptr=_ptr(labels), l_dtype=l_dtype, top=top,
+                      ignore_label=ignore_label, temperature=temperature, background=background, log_prob=_ptr(out.log_prob),
+                      entropy=_ptr(out.entropy), norm=_ptr(out.norm), top_log_prob=_ptr(out.top_log_prob),
+                      top_label=_ptr(out.top_label), device=call.index, stream=call.stream, workspace=call.workspace)
     return out
 
 
 def _scores_grad_tensor(x, labels, norm, grad_log_prob, entropy, grad_entropy, dim, temperature, background, ignore_label):
     x, dim, shape, rows = _tensor_logits(x, dim)
     call = _TorchCall(x)
-    f32 = ("float32",)
-    lab = None if labels is None else _tensor_arg("labels", labels, shape, x.device, _lib.L_KINDS)
-    args = [_tensor_arg("norm", norm, shape, x.device, f32, 2)]
-    for name, t in (("entropy", entropy), ("grad_log_prob", grad_log_prob), ("grad_entropy", grad_entropy)):
-        args.append(None if t is None else _tensor_arg(name, t, shape, x.device, f32))
-    ptr = [None if t is None else t.data_ptr() for t in args]
+    dev = x.device
+    l_dtype = None
+    if labels is not None:
+        labels = _tensor_arg("labels", labels, shape, dev, _lib.L_KINDS)
+        l_dtype = _name(labels.dtype)
+    norm = _tensor_arg("norm", norm, shape, dev, _F32, (2,))
+    if grad_log_prob is not None:
+        grad_log_prob = _tensor_arg("grad_log_prob", grad_log_prob, shape, dev, _F32)
+    if grad_entropy is not None:
+        grad_entropy = _tensor_arg("grad_entropy", grad_entropy, shape, dev, _F32)
+        if entropy is not None:
+            entropy = _tensor_arg("entropy", entropy, shape, dev, _F32)
+    else:
+        entropy = None
     grad, grad_rows = call.grad_like(x, dim)
-    _lib.label_scores_grad(x.data_ptr(), _name(x.dtype), rows, grad.data_ptr(), grad_rows, ptr[0],
-                           labels_ptr=None if lab is None else lab.data_ptr(), l_dtype=None if lab is None else _name(lab.dtype),
-                           ignore_label=ignore_label, temperature=temperature, background=background, entropy=ptr[1],
-                           grad_log_prob=ptr[2], grad_entropy=ptr[3], **call.kw())
+    _lib.label_scores_grad(x.data_ptr(), _name(x.dtype), rows, grad.data_ptr(), grad_rows, norm.data_ptr(), labels_ptr=_ptr(labels),
+                           l_dtype=l_dtype, ignore_label=ignore_label, temperature=temperature, background=background,
+                           entropy=_ptr(entropy), grad_log_prob=_ptr(grad_log_prob), grad_entropy=_ptr(grad_entropy),
+                           device=call.index, stream=call.stream)
     return grad
+
+
+def _teacher_tensors(top_label, values, shape, device):
+    last = (top_label.shape[-1] if _is_torch(top_label) and top_label.ndim else 0,)
+    return (_tensor_arg("top_label", top_label, shape, device, ("int32", "int64"), last),
+            _tensor_arg("values", values, shape, device, _lib.SCORE_DTYPES, last))
 
 
 def _distill_tensor(x, top_label, values, dim, norm, temperature, tail, background):
     x, dim, shape, rows = _tensor_logits(x, dim)
     call = _TorchCall(x)
-    lab, val, K = _teacher_tensors(top_label, values, shape, x.device)
+    lab, val = _teacher_tensors(top_label, values, shape, x.device)
     out = DistillLoss(call.empty(shape), call.empty(shape + (2,)) if norm else None, call.empty(shape) if norm and tail else None)
-    ptr = [None if t is None else t.data_ptr() for t in out]
-    _lib.distill(x.data_ptr(), _name(x.dtype), rows, lab.data_ptr(), _name(lab.dtype), val.data_ptr(), _name(val.dtype), K,
-                 tail=tail, temperature=temperature, background=background, loss=ptr[0], norm=ptr[1], log_tail=ptr[2],
-                 workspace=call.workspace, **call.kw())
+    _lib.distill(x.data_ptr(), _name(x.dtype), rows, lab.data_ptr(), _name(lab.dtype), val.data_ptr(), _name(val.dtype),
+                 lab.shape[-1], tail=tail, temperature=temperature, background=background, loss=out.loss.data_ptr(),
+                 norm=_ptr(out.norm), log_tail=_ptr(out.log_tail), device=call.index, stream=call.stream, workspace=call.workspace)
     return out
-
-
-def _teacher_tensors(top_label, values, shape, device):
-    K = top_label.shape[-1] if _is_torch(top_label) and top_label.ndim else 0
-    return (_tensor_arg("top_label", top_label, shape, device, ("int32", "int64"), K),
-            _tensor_arg("values", values, shape, device, _lib.SCORE_DTYPES, K), K)
 
 
 def _distill_grad_tensor(x, top_label, values, norm, log_tail, grad_loss, dim, temperature, tail, background):
     x, dim, shape, rows = _tensor_logits(x, dim)
     call = _TorchCall(x)
-    f32 = ("float32",)
-    lab, val, K = _teacher_tensors(top_label, values, shape, x.device)
-    norm = _tensor_arg("norm", norm, shape, x.device, f32, 2)
-    grad_loss = _tensor_arg("grad_loss", grad_loss, shape, x.device, f32)
-    log_tail = None if log_tail is None else _tensor_arg("log_tail", log_tail, shape, x.device, f32)
+    dev = x.device
+    lab, val = _teacher_tensors(top_label, values, shape, dev)
+    norm = _tensor_arg("norm", norm, shape, dev, _F32, (2,))
+    grad_loss = _tensor_arg("grad_loss", grad_loss, shape, dev, _F32)
+    if log_tail is not None:
+        log_tail = _tensor_arg("log_tail", log_tail, shape, dev, _F32)
     grad, grad_rows = call.grad_like(x, dim)
     _lib.distill_grad(x.data_ptr(), _name(x.dtype), rows, grad.data_ptr(), grad_rows, lab.data_ptr(), _name(lab.dtype),
-                      val.data_ptr(), _name(val.dtype), K, norm.data_ptr(), grad_loss.data_ptr(),
-                      log_tail=None if log_tail is None else log_tail.data_ptr(), tail=tail, temperature=temperature,
-                      background=background, **call.kw())
+                      val.data_ptr(), _name(val.dtype), lab.shape[-1], norm.data_ptr(), grad_loss.data_ptr(),
+                      log_tail=_ptr(log_tail), tail=tail, temperature=temperature, background=background, device=call.index,
+                      stream=call.stream)
     return grad
 
 
@@ -320,10 +347,9 @@ def label_scores_grad(logits, labels, norm, *, grad_log_prob=None, entropy=None,
     if _is_torch(logits):
         return _scores_grad_tensor(logits, labels, norm, grad_log_prob, entropy, grad_entropy, **kw)
     x, dim, shape, rows = _array_logits(logits, dim)
-    f32 = ("float32",)
     lab = None if labels is None else _array_arg("labels", labels, shape, _lib.L_KINDS)
-    norm = _array_arg("norm", norm, shape, f32, 2)
-    rest = [None if a is None else _array_arg(n, a, shape, f32)
+    norm = _array_arg("norm", norm, shape, _F32, 2)
+    rest = [None if a is None else _array_arg(n, a, shape, _F32)
             for n, a in (("entropy", entropy), ("grad_log_prob", grad_log_prob), ("grad_entropy", grad_entropy))]
     g, view = _grad_array(x, dim)
     _lib.label_scores_grad(_address(x), x.dtype.name, rows, _address(g), rows, _address(norm), labels_ptr=_address(lab),
@@ -374,11 +400,10 @@ def distill_loss_grad(logits, top_label, values, norm, *, grad_loss, log_tail=No
     if _is_torch(logits):
         return _distill_grad_tensor(logits, top_label, values, norm, log_tail, grad_loss, **kw)
     x, dim, shape, rows = _array_logits(logits, dim)
-    f32 = ("float32",)
     lab, val, K = _teacher_arrays(top_label, values, shape, tail)
-    norm = _array_arg("norm", norm, shape, f32, 2)
-    grad_loss = _array_arg("grad_loss", grad_loss, shape, f32)
-    log_tail = None if log_tail is None else _array_arg("log_tail", log_tail, shape, f32)
+    norm = _array_arg("norm", norm, shape, _F32, 2)
+    grad_loss = _array_arg("grad_loss", grad_loss, shape, _F32)
+    log_tail = None if log_tail is None else _array_arg("log_tail", log_tail, shape, _F32)
     g, view = _grad_array(x, dim)
     _lib.distill_grad(_address(x), x.dtype.name, rows, _address(g), rows, _address(lab), lab.dtype.name, _address(val),
                       val.dtype.name, K, _address(norm), _address(grad_loss), log_tail=_address(log_tail), tail=tail,

@@ -419,6 +419,7 @@ typedef struct qmri_logits {
 #define QMRI_L_I16 2
 #define QMRI_L_I64 3
 #define QMRI_MAX_TOP 64 /* alternatives per row; teacher entries per row */
+#define QMRI_SHORT_ROW 1024 /* rows of up to this many classes never need a workspace */
 typedef struct qmri_label_scores_args {
     qmri_logits logits;
     const void *labels;   /* nullable [rows]: the given label of every row */

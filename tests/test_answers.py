@@ -37,7 +37,7 @@ def test_struct_layout_matches_the_c_compiler(tmp_path):
     subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)])
     assert [int(v) for v in subprocess.check_output([str(exe)]).decode().split()] == want
     head = open(os.path.join(ROOT, "include", "qmri.h")).read()
-    assert f"#define QMRI_MAX_TOP {L.MAX_TOP} " in head
+    assert f"#define QMRI_MAX_TOP {L.MAX_TOP} " in head and f"#define QMRI_SHORT_ROW {L.SHORT_ROW} " in head
 
 
 def _scores_args(**kw):
