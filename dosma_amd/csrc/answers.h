@@ -190,6 +190,43 @@ __device__ __forceinline__ Tile<T> load_tile(const T *p, int n) {
     return r;
 }
 
+// The bits of 8 scores, a class `sc` apart, `left` of them there and -inf behind.  (Bits in words of their own, and the whole eight
+// without a condition: what is packed, converted or branched upon would be waited for on the spot, and these are meant to be in
+// flight while the eight before them are worked on.)
+template <typename T>
+__device__ __forceinline__ unsigned load_bits(const T *p) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const unsigned *>(p);
+    else return *reinterpret_cast<const unsigned short *>(p);
+}
+template <typename T>
+__device__ __forceinline__ float widen(unsigned w) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else if constexpr (std::is_same_v<T, bf16_t>) return __uint_as_float(w << 16);
+    else return static_cast<float>(__builtin_bit_cast(T, (unsigned short)w));
+}
+template <typename T>
+__device__ __forceinline__ void load_classes(const T *p, long long sc, int left, unsigned (&v)[8]) {
+    if (left >= 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = load_bits(p + i * sc);
+    } else {
+        const unsigned none = bits_of(static_cast<T>(kNegInf));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? load_bits(p + i * sc) : none;
+    }
+}
+// Classes that do not lie together, a lane a row: into how many parts (of whole eights) a row is cut so that every compute unit has
+// 16 waves.  Returns the classes of a part.
+inline int cut_classes(const LogitsK &g, int num_cu, int &parts) {
+    const long long waves = (g.rows + 63) / 64;
+    long long want = (16ll * num_cu + waves - 1) / waves;
+    const int eights = (g.C + 7) / 8;
+    if (want > eights) want = eights;
+    const int len = (int)((eights + want - 1) / want) * 8;
+    parts = (g.C + len - 1) / len;
+    return len;
+}
+
 // NaN goes through a maximum here (v_maximum3_f32), so a row's NaN reaches its statistics without a test of its own
 __device__ __forceinline__ float maxn(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
@@ -326,19 +363,21 @@ __device__ __forceinline__ void raise(Running &r, float cm, float c2) {
         r.R = R;
     }
 }
-// t as the sum of exp2(d) d
+// t as the sum of exp2(d) d; returns the largest of the scores
 template <int N>
-__device__ __forceinline__ void add_scores(Running &r, const float (&x)[N], float c2) {
-    raise<true>(r, max_of(x), c2);
-    float e[N], et[N];
+__device__ __forceinline__ float add_scores(Running &r, const float (&x)[N], float c2) {
+    const float cm = max_of(x);
+    raise<true>(r, cm, c2);
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float d = clamp2(fmaf(x[i], c2, -r.R));
-        e[i] = exp2_hw(d);
-        et[i] = e[i] * d;
+        const float d = clamp2(fmaf(x[i], c2, -r.R)), e = exp2_hw(d);
+        s[i & 3] += e;
+        t[i & 3] = fmaf(e, d, t[i & 3]);
     }
-    r.s += tree_sum(e);
-    r.t += tree_sum(et);
+    r.s += tree_sum(s);
+    r.t += tree_sum(t);
+    return cm;
 }
 __device__ __forceinline__ bool far_scores(float M, float c2) { return M > kNegInf && !(fabsf(M) * c2 < kFar); }
 // factor that brings a lane's sums to reference(M), M the maximum over the lanes; d its exponent
@@ -385,6 +424,18 @@ struct Cut {
     int segs, len;
 };
 Cut cut_rows(const LogitsK &g, int num_cu, int longest);
+
+// LDS (beyond `own` bytes) that a block asks for only to be placed: the hardware fills a compute unit with as many blocks as fit
+// before it turns to the next one, so a launch of `blocks` < num_cu * limit would leave units idle while others share their vector
+// units among `limit` blocks (1024 rows of 100003 scores: 171 of 256 units at work).  With this much LDS only as many fit as each
+// unit's even share; 64 KB a block is the most a launch may ask for as it is.
+inline size_t spread_lds(long long blocks, int num_cu, int limit, int own) {
+    const long long share = (blocks + num_cu - 1) / num_cu;
+    if (share >= limit) return 0;
+    long long bytes = 160 * 1024 / share - 1024;
+    if (bytes > 65536) bytes = 65536;
+    return bytes > own ? (size_t)(bytes - own) : 0;
+}
 
 hipError_t label_scores_launch(const ScoresK &k, int dtype, int num_cu, hipStream_t st);
 size_t label_scores_workspace_bytes(const ScoresK &k, int dtype, int num_cu);

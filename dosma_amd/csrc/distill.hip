@@ -71,34 +71,6 @@ __device__ __forceinline__ Teacher teacher_of(const DistillK &k, bool any, float
 __device__ __forceinline__ float teacher_term(const DistillK &k, float v, float m) {
     return k.tail ? exp2_hw(v * kLog2e) : (m == kNegInf ? (v != v ? v : 0.f) : exp2_hw((v - m) * k.g.c2));
 }
-// by G lanes, entries q = gl, gl + G, ..
-template <int G>
-__device__ __forceinline__ Teacher teacher_group(const DistillK &k, long long n, int gl, int cats) {
-    float m = kNegInf;
-    float cnt = 0.f;
-    for (int q = gl; q < k.K; q += G) {
-        float v;
-        if (load_entry(k, n, q, cats, v) >= 0) {
-            m = maxn(m, v);
-            cnt = 1.f;
-        }
-    }
-    m = group_max<G>(m);
-    const bool any = group_max<G>(cnt) > 0.f;
-    float sum = 0.f, others = 0.f;
-    int first = 0x7fffffff;
-    for (int q = gl; q < k.K; q += G) {
-        float v;
-        if (load_entry(k, n, q, cats, v) < 0) continue;
-        const float e = teacher_term(k, v, m);
-        sum += e;
-        if (v == m && first == 0x7fffffff) first = q;
-        else others += e;
-    }
-    const int one = group_min<G>(first);
-    if (first != one && first != 0x7fffffff) others += teacher_term(k, m, m);
-    return teacher_of(k, any, m, group_sum<G>(sum), group_sum<G>(others));
-}
 // by a wave that holds an entry a lane (l < 0: none)
 __device__ __forceinline__ Teacher teacher_wave(const DistillK &k, int l, float v) {
     const bool ok = l >= 0;
@@ -108,21 +80,61 @@ __device__ __forceinline__ Teacher teacher_wave(const DistillK &k, int l, float 
     const int first = at ? __ffsll(at) - 1 : -1;
     return teacher_of(k, __ballot(ok) != 0ull, m, group_sum<64>(e), group_sum<64>((int)(threadIdx.x & 63) == first ? 0.f : e));
 }
-// K entries in registers
+// N entries of a row in registers: both loads are issued before either is looked at.
+template <int N, typename L, typename V, int K>
+__device__ __forceinline__ void load_pairs(const void *labels, const void *values, long long n, int cats, int (&l)[K], float (&v)[K]) {
+    struct {
+        L v[N];
+    } rl;
+    struct {
+        V v[N];
+    } rv;
+    __builtin_memcpy(&rl, static_cast<const L *>(labels) + n * N, sizeof(rl));
+    __builtin_memcpy(&rv, static_cast<const V *>(values) + n * N, sizeof(rv));
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        l[q] = rl.v[q] >= 0 && rl.v[q] < (L)cats ? (int)rl.v[q] : -1;
+        v[q] = to_f32(rv.v[q]);
+    }
+}
+template <int N, int K>
+__device__ __forceinline__ void load_exactly(const DistillK &k, long long n, int cats, int (&l)[K], float (&v)[K]) {
+    if (k.l_kind == QMRI_L_I32) {
+        if (k.v_dtype == QMRI_F32) load_pairs<N, int, float>(k.labels, k.values, n, cats, l, v);
+        else if (k.v_dtype == QMRI_F16) load_pairs<N, int, f16_t>(k.labels, k.values, n, cats, l, v);
+        else load_pairs<N, int, bf16_t>(k.labels, k.values, n, cats, l, v);
+    } else {
+        if (k.v_dtype == QMRI_F32) load_pairs<N, long long, float>(k.labels, k.values, n, cats, l, v);
+        else if (k.v_dtype == QMRI_F16) load_pairs<N, long long, f16_t>(k.labels, k.values, n, cats, l, v);
+        else load_pairs<N, long long, bf16_t>(k.labels, k.values, n, cats, l, v);
+    }
+}
 template <int K>
 __device__ __forceinline__ void load_entries(const DistillK &k, long long n, int cats, int (&l)[K], float (&v)[K]) {
+    // (the usual case by itself and first: of the ways below each gives its registers to a common set in the end, which waits)
     if (k.K == K && k.l_kind == QMRI_L_I32 && k.v_dtype == QMRI_F32) {
         __builtin_memcpy(&l, static_cast<const int *>(k.labels) + n * K, sizeof(l));
         __builtin_memcpy(&v, static_cast<const float *>(k.values) + n * K, sizeof(v));
 #pragma unroll
         for (int q = 0; q < K; ++q) l[q] = (unsigned)l[q] < (unsigned)cats ? l[q] : -1;
-    } else {
+        return;
+    }
 #pragma unroll
-        for (int q = 0; q < K; ++q) {
-            l[q] = -1;
-            v[q] = 0.f;
-            if (q < k.K) l[q] = load_entry(k, n, q, cats, v[q]);
-        }
+    for (int q = 0; q < K; ++q) {
+        l[q] = -1;
+        v[q] = 0.f;
+    }
+    if constexpr (K == 2) {
+        if (k.K == 2) load_exactly<2>(k, n, cats, l, v);
+        else load_exactly<1>(k, n, cats, l, v);
+    } else if constexpr (K == 4) {
+        if (k.K == 4) load_exactly<4>(k, n, cats, l, v);
+        else load_exactly<3>(k, n, cats, l, v);
+    } else {
+        if (k.K == 8) load_exactly<8>(k, n, cats, l, v);
+        else if (k.K == 7) load_exactly<7>(k, n, cats, l, v);
+        else if (k.K == 6) load_exactly<6>(k, n, cats, l, v);
+        else load_exactly<5>(k, n, cats, l, v);
     }
 }
 template <int K>
@@ -145,8 +157,8 @@ __device__ __forceinline__ Teacher teacher_lane(const DistillK &k, const int (&l
     }
     return teacher_of(k, any, m, sum, others);
 }
-template <>
-__device__ __forceinline__ Teacher teacher_group<1>(const DistillK &k, long long n, int, int cats) {
+// by one lane, the entries read from memory
+__device__ __forceinline__ Teacher teacher_read(const DistillK &k, long long n, int cats) {
     float m = kNegInf;
     bool any = false;
     for (int q = 0; q < k.K; ++q) {
@@ -235,7 +247,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillK k) {
         int el[K > 0 ? K : 1];
         float ev[K > 0 ? K : 1];
         if (K) load_entries(k, n, cats, el, ev);
-        const Teacher t = K ? teacher_lane(k, el, ev) : teacher_group<1>(k, n, 0, cats);
+        const Teacher t = K ? teacher_lane(k, el, ev) : teacher_read(k, n, cats);
         // x[0]: the implicit category, or one that is not offered; x[j + 1]: class j
         float x[N + 1], e[N + 1], s = 0.f, so = 0.f;
         x[0] = g.bg ? 0.f : kNegInf;
@@ -317,7 +329,7 @@ __global__ __launch_bounds__(256) void distill_grad_small_kernel(const DistillK 
         int el[K > 0 ? K : 1];
         float ev[K > 0 ? K : 1];
         if (K) load_entries(k, n, cats, el, ev);
-        const Teacher t = K ? teacher_lane(k, el, ev) : teacher_group<1>(k, n, 0, cats);
+        const Teacher t = K ? teacher_lane(k, el, ev) : teacher_read(k, n, cats);
         const GradRow r = grad_row(k, n, t);
         unsigned in = 0u;
         float qs[N];
@@ -355,86 +367,142 @@ __global__ __launch_bounds__(256) void distill_grad_small_kernel(const DistillK 
 }
 
 // ---- group: G lanes a row, 16 scores a lane ------------------------------------------------------------------------------------
-// The labels of the entries are marked in LDS, one 16-bit word for each lane's scores.
+// The labels of the entries are marked in LDS, one 16-bit word for each lane's scores.  A lane holds every G-th entry: E of them
+// in registers, or (E 0) read again where they are needed.
 template <int G, int V>
-__device__ __forceinline__ void mark(unsigned *bits, int c) {  // bits: the block's words, two lanes a word
-    const int vec = c / V, owner = (int)(threadIdx.x / G) * G + vec % G, bit = (vec / G) * V + c % V;
-    atomicOr(&bits[owner >> 1], 1u << ((owner & 1) * 16 + bit));
+__device__ __forceinline__ void place_of(int c, int &owner, int &bit) {
+    const int vec = c / V;
+    owner = (int)(threadIdx.x / G) * G + vec % G;
+    bit = (vec / G) * V + c % V;
 }
-template <typename T, int G>
+template <int G, int E>
+struct GroupEntries {
+    int l[E > 0 ? E : 1];
+    float v[E > 0 ? E : 1];
+    const DistillK &k;
+    long long n;
+    int gl, cats;
+    __device__ __forceinline__ GroupEntries(const DistillK &k_, long long n_, int gl_, int cats_) : k(k_), n(n_), gl(gl_), cats(cats_) {
+        if constexpr (E > 0) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int q = gl + e * G;
+                l[e] = -1;
+                v[e] = 0.f;
+                if (q < k.K) l[e] = load_entry(k, n, q, cats, v[e]);
+            }
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        if constexpr (E > 0) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (l[e] >= 0) f(l[e], v[e]);
+        } else {
+            for (int q = gl; q < k.K; q += G) {
+                float x;
+                const int i = load_entry(k, n, q, cats, x);
+                if (i >= 0) f(i, x);
+            }
+        }
+    }
+    __device__ __forceinline__ Teacher teacher() const {
+        float m = kNegInf, cnt = 0.f, sum = 0.f, others = 0.f;
+        each([&](int, float x) {
+            m = maxn(m, x);
+            cnt = 1.f;
+        });
+        m = group_max<G>(m);
+        const bool any = group_max<G>(cnt) > 0.f;
+        bool left_out = false;
+        each([&](int, float x) {
+            const float e = teacher_term(k, x, m);
+            sum += e;
+            if (x == m && !left_out) left_out = true;
+            else others += e;
+        });
+        // one entry of the largest value is left out, not one a lane
+        const int one = group_min<G>(left_out ? gl : 0x7fffffff);
+        if (left_out && one != gl) others += teacher_term(k, m, m);
+        return teacher_of(k, any, m, group_sum<G>(sum), group_sum<G>(others));
+    }
+};
+template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
     __shared__ unsigned s_bits[128];
     const LogitsK &g = k.g;
     constexpr int V = kVec<T>, NV = 16 / V, ROWS = 256 / G;
     const int gl = threadIdx.x % G, cats = g.C + g.bg;
     for (long long n0 = (long long)blockIdx.x * ROWS; n0 < g.rows; n0 += (long long)gridDim.x * ROWS) {
+        // (groups behind the last row work on it too and write nothing: the lane exchanges want whole waves)
         const long long nr = n0 + threadIdx.x / G;
         const bool live = nr < g.rows;
         const long long n = live ? nr : g.rows - 1;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
-        float x[17];
+        Vec<T> raw[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = (i * G + gl) * V;
-            const Vec<T> r = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[i * V + e] = get(r, e);
+            raw[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
         }
-        x[16] = (g.bg && gl == 0) ? 0.f : kNegInf;
+        const GroupEntries<G, E> entries(k, n, gl, cats);
         unsigned in = 0u;
         float back_in = 0.f;  // 1: the implicit category is an entry
         if (k.tail) {
             if ((threadIdx.x & 1) == 0) s_bits[threadIdx.x >> 1] = 0u;
             wave_sync();
-            for (int q = gl; q < k.K; q += G) {
-                float v;
-                const int c = load_entry(k, n, q, cats, v) - g.bg;
-                if (c >= 0) mark<G, V>(s_bits, c);
-                else if (g.bg && c == -1) back_in = 1.f;
-            }
+            entries.each([&](int l, float) {
+                if (l < g.bg) {
+                    back_in = 1.f;
+                } else {
+                    int owner, bit;
+                    place_of<G, V>(l - g.bg, owner, bit);
+                    atomicOr(&s_bits[owner >> 1], 1u << ((owner & 1) * 16 + bit));
+                }
+            });
             wave_sync();
             in = s_bits[threadIdx.x >> 1] >> ((threadIdx.x & 1) * 16) & 0xffffu;
             wave_sync();
-            // (an empty slot is -1 - bg: with the background it is -2, without it the flag is not read)
             back_in = group_max<G>(back_in);
         }
-        const Teacher t = teacher_group<G>(k, n, gl, cats);
-        float M = x[16];
+        const Teacher t = entries.teacher();
+        float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) M = maxn(M, x[i]);
-        M = group_max<G>(M);
-        const float ref = reference(M);
-        float e[16], eo[16];
+        for (int i = 0; i < 16; ++i) x[i] = get(raw[i / V], i % V);
+        const float xb = (g.bg && gl == 0) ? 0.f : kNegInf;
+        const float M = group_max<G>(maxn(max_of(x), xb)), ref = reference(M);
+        float e[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            e[i] = exp2_hw((x[i] - ref) * g.c2);
-            eo[i] = (in >> i) & 1u ? 0.f : e[i];
-        }
-        const float eb = exp2_hw((x[16] - ref) * g.c2);
+        for (int i = 0; i < 16; ++i) e[i] = exp2_hw((x[i] - ref) * g.c2);
+        const float eb = exp2_hw((xb - ref) * g.c2);
         const float s = group_sum<G>(tree_sum(e) + eb);
-        const float so = k.tail ? group_sum<G>(tree_sum(eo) + (back_in > 0.f ? 0.f : eb)) : 0.f;
+        float so = 0.f;
+        if (k.tail) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) e[i] = (in >> i) & 1u ? 0.f : e[i];
+            so = group_sum<G>(tree_sum(e) + (back_in > 0.f ? 0.f : eb));
+        }
         const Student p = student_of(M, s);
         float loss = 0.f;
-        for (int q = gl; q < k.K; q += G) {
-            float v;
-            const int l = load_entry(k, n, q, cats, v);
-            if (l >= 0) loss += entry_loss(k, t, p, v, l < g.bg ? 0.f : to_f32(z[l - g.bg]));
-        }
+        entries.each([&](int l, float v) { loss += entry_loss(k, t, p, v, gather(g, z, l)); });
         loss = group_sum<G>(loss);
         const float lso = log_outside<G>(k, n, z, gl, cats, p, t, so);
         if (live && gl == 0) write_row(k, n, M, lso, p, t, loss);
     }
 }
 
-template <typename T, int G>
+template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK k) {
     __shared__ unsigned s_bits[128];
-    __shared__ T s_val[256 * 16];  // what an entry's lane has worked out for its label
+    __shared__ float s_val[256 * 16];  // what an entry's lane has worked out for its label
+    __shared__ int s_l[E > 0 ? 256 * E : 1];
+    __shared__ float s_q[E > 0 ? 256 * E : 1];
     const LogitsK &g = k.g;
     constexpr int V = kVec<T>, NV = 16 / V, ROWS = 256 / G;
-    const int gl = threadIdx.x % G, cats = g.C + g.bg;
+    const int gl = threadIdx.x % G, cats = g.C + g.bg, row = threadIdx.x / G;
     for (long long n0 = (long long)blockIdx.x * ROWS; n0 < g.rows; n0 += (long long)gridDim.x * ROWS) {
-        const long long nr = n0 + threadIdx.x / G;
+        const long long nr = n0 + row;
         const bool live = nr < g.rows;
         const long long n = live ? nr : g.rows - 1;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
@@ -445,24 +513,36 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
             const int j = (i * G + gl) * V;
             x[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
         }
-        const Teacher t = teacher_group<G>(k, n, gl, cats);
+        const GroupEntries<G, E> entries(k, n, gl, cats);
+        const Teacher t = entries.teacher();
         const GradRow r = grad_row(k, n, t);
         if ((threadIdx.x & 1) == 0) s_bits[threadIdx.x >> 1] = 0u;
+        if constexpr (E > 0) {  // entry q of the row at row * G E + q
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                s_l[row * G * E + gl + e * G] = entries.l[e];
+                s_q[row * G * E + gl + e * G] = entries.l[e] >= 0 ? weight(t, entries.v[e]) : 0.f;
+            }
+        }
         wave_sync();
-        for (int q = gl; q < k.K; q += G) {
-            float v;
-            const int l = load_entry(k, n, q, cats, v), c = l - g.bg;
-            if (l < 0 || c < 0) continue;
+        entries.each([&](int l, float) {
+            const int c = l - g.bg;
+            if (c < 0) return;
             // the same label twice: every one of its entries sums all of them, in the order of the entries, and writes the same value
             float qs = 0.f;
             for (int o = 0; o < k.K; ++o) {
-                float vo;
-                if (load_entry(k, n, o, cats, vo) == l) qs += weight(t, vo);
+                if constexpr (E > 0) {
+                    qs += s_l[row * G * E + o] == l ? s_q[row * G * E + o] : 0.f;
+                } else {
+                    float v;
+                    if (load_entry(k, n, o, cats, v) == l) qs += weight(t, v);
+                }
             }
-            const int vec = c / V, owner = (int)(threadIdx.x / G) * G + vec % G, bit = (vec / G) * V + c % V;
-            s_val[owner * 16 + bit] = from_f32<T>(grad_inside(r, g.c2, to_f32(z[c]), qs));
-            mark<G, V>(s_bits, c);
-        }
+            int owner, bit;
+            place_of<G, V>(c, owner, bit);
+            s_val[owner * 16 + bit] = grad_inside(r, g.c2, to_f32(z[c]), qs);
+            atomicOr(&s_bits[owner >> 1], 1u << ((owner & 1) * 16 + bit));
+        });
         wave_sync();
         const unsigned in = s_bits[threadIdx.x >> 1] >> ((threadIdx.x & 1) * 16) & 0xffffu;
 #pragma unroll
@@ -473,8 +553,7 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
             for (int e = 0; e < V; ++e) y[e] = grad_outside(r, g.c2, get(x[i], e));
             if ((in >> (i * V)) & ((1u << V) - 1u)) {
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if ((in >> (i * V + e)) & 1u) y[e] = to_f32(s_val[threadIdx.x * 16 + i * V + e]);
+                for (int e = 0; e < V; ++e) y[e] = (in >> (i * V + e)) & 1u ? s_val[threadIdx.x * 16 + i * V + e] : y[e];
             }
             if (!live) continue;
             if (j + V <= g.C) store_vec(out + j, pack_vec<T>(y));
@@ -703,48 +782,75 @@ __global__ __launch_bounds__(256) void distill_grad_block_kernel(const DistillK 
 }
 
 // ---- planes: one lane a row, more than 8 classes that do not lie together ------------------------------------------------------
-// Which of the 32 categories from c are entries: the row's labels are read again for each 32 (they stay in the caches).
-__device__ __forceinline__ unsigned marks(const DistillK &k, long long n, int c, int cats) {
-    unsigned in = 0u;
-    for (int q = 0; q < k.K; ++q) {
-        const long long l = load_label(k.labels, k.l_kind, n * k.K + q) - c;
-        if (l >= 0 && l < 32 && l + c < cats) in |= 1u << (int)l;
+// K: entries in registers, as in small; 0: read again.
+template <int K>
+struct LaneEntries {
+    int l[K > 0 ? K : 1];
+    float v[K > 0 ? K : 1];
+    const DistillK &k;
+    long long n;
+    int cats;
+    __device__ __forceinline__ LaneEntries(const DistillK &k_, long long n_, int cats_) : k(k_), n(n_), cats(cats_) {
+        if constexpr (K > 0) load_entries(k, n, cats, l, v);
     }
-    return in;
-}
-template <typename T>
+    // f(label, value) for every entry that counts
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        if constexpr (K > 0) {
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+                if (l[q] >= 0) f(l[q], v[q]);
+        } else {
+            for (int q = 0; q < k.K; ++q) {
+                float x;
+                const int i = load_entry(k, n, q, cats, x);
+                if (i >= 0) f(i, x);
+            }
+        }
+    }
+    __device__ __forceinline__ Teacher teacher() const {
+        if constexpr (K > 0) return teacher_lane(k, l, v);
+        else return teacher_read(k, n, cats);
+    }
+    // which of the 32 categories from c are entries
+    __device__ __forceinline__ unsigned marks(int c) const {
+        unsigned in = 0u;
+        each([&](int i, float) { in |= (unsigned)(i - c) < 32u ? 1u << (i - c) : 0u; });
+        return in;
+    }
+};
+template <typename T, int K>
 __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillK k) {
     const LogitsK &g = k.g;
     const int cats = g.C + g.bg;
     const long long stride = (long long)gridDim.x * 256;
     for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < g.rows; n += stride) {
-        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
+        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si), *p = z;
+        unsigned next[8];
+        load_classes(p, g.sc, g.C, next);
+        const LaneEntries<K> entries(k, n, cats);
         Running r = no_scores();  // (t: the sum outside the entries)
-        for (int c0 = 0; c0 < cats; c0 += 32) {
-            const unsigned in = k.tail ? marks(k, n, c0, cats) : 0u;
+        if (g.bg) {
+            const float x[1] = {0.f};
+            add_outside(r, x, g.c2, k.tail ? entries.marks(0) & 1u : 0u);
+        }
+        unsigned in = 0u;
+        for (int c = 0; c < g.C; c += 8) {
+            if (k.tail && (c & 31) == 0) in = entries.marks(c + g.bg);
+            float x[8];
 #pragma unroll
-            for (int i0 = 0; i0 < 32; i0 += 8) {
-                if (c0 + i0 >= cats) break;
-                float x[8];
-                if (c0 + i0 >= g.bg && c0 + i0 + 8 <= cats) {
-                    const T *p = z + (long long)(c0 + i0 - g.bg) * g.sc;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i * g.sc]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = c0 + i0 + i < cats ? gather(g, z, c0 + i0 + i) : kNegInf;
-                }
-                add_outside(r, x, g.c2, (in >> i0) & 0xffu);
-            }
+            for (int i = 0; i < 8; ++i) x[i] = widen<T>(next[i]);
+            p += 8 * g.sc;
+            if (c + 8 < g.C) load_classes(p, g.sc, g.C - c - 8, next);
+            add_outside(r, x, g.c2, (in >> (c & 31)) & 0xffu);
         }
         float sum = 0.f, so = 0.f;
         if (far_scores(r.m, g.c2)) {  // (see answers.h)
-            unsigned in = 0u;
             for (int j = 0; j < cats; ++j) {
-                if (k.tail && (j & 31) == 0) in = marks(k, n, j, cats);
+                if (k.tail && (j & 31) == 0) in = entries.marks(j);
                 const float e = exp2_hw((gather(g, z, j) - reference(r.m)) * g.c2);
                 sum += e;
-                so += (in >> (j & 31)) & 1u ? 0.f : e;
+                so += k.tail && (in >> (j & 31)) & 1u ? 0.f : e;
             }
         } else {
             float d;
@@ -752,15 +858,11 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillK k) {
             sum = r.s * f;
             so = r.t * f;
         }
-        const Student p = student_of(r.m, sum);
-        const Teacher t = teacher_group<1>(k, n, 0, cats);
+        const Student st = student_of(r.m, sum);
+        const Teacher t = entries.teacher();
         float loss = 0.f;
-        for (int q = 0; q < k.K; ++q) {
-            float v;
-            const int l = load_entry(k, n, q, cats, v);
-            if (l >= 0) loss += entry_loss(k, t, p, v, gather(g, z, l));
-        }
-        write_row(k, n, r.m, log_outside<1>(k, n, z, 0, cats, p, t, so), p, t, loss);
+        entries.each([&](int l, float v) { loss += entry_loss(k, t, st, v, gather(g, z, l)); });
+        write_row(k, n, r.m, log_outside<1>(k, n, z, 0, cats, st, t, so), st, t, loss);
     }
 }
 
@@ -816,50 +918,45 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(const DistillK k) {
     }
 }
 
-// a block 256 rows and 32 classes
-template <typename T>
-__global__ __launch_bounds__(256) void distill_grad_planes_kernel(const DistillK k, int parts) {
+// A block takes 256 rows and `len` classes of them, as if none of these were an entry's; the entries' classes are written over in
+// the end (by the lane that wrote them before, so in order).
+template <typename T, int K>
+__global__ __launch_bounds__(256) void distill_grad_planes_kernel(const DistillK k, int parts, int len) {
     const LogitsK &g = k.g;
     const int cats = g.C + g.bg;
     const long long blocks = (g.rows + 255) / 256;
     for (long long item = blockIdx.x; item < blocks * parts; item += gridDim.x) {
-        const long long rb = item / parts;
-        const int c0 = (int)(item - rb * parts) * 32, c1 = c0 + 32 < g.C ? c0 + 32 : g.C;
+        const long long rb = parts == 1 ? item : item / parts;
+        const int c0 = (int)(item - rb * parts) * len, c1 = c0 + len < g.C ? c0 + len : g.C;
         const long long n = rb * 256 + threadIdx.x;
         if (n >= g.rows) continue;
-        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
-        T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi);
-        const Teacher t = teacher_group<1>(k, n, 0, cats);
+        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si), *p = z + c0 * g.sc;
+        T *grad = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi), *out = grad + c0 * k.gsc;
+        unsigned next[8];
+        load_classes(p, g.sc, c1 - c0, next);
+        const LaneEntries<K> entries(k, n, cats);
+        const Teacher t = entries.teacher();
         const GradRow r = grad_row(k, n, t);
-        const unsigned in = marks(k, n, c0 + g.bg, cats);
+        for (int c = c0; c < c1; c += 8) {
+            float y[8];
 #pragma unroll
-        for (int i0 = 0; i0 < 32; i0 += 8) {
-            const int c = c0 + i0;
-            if (c >= c1) break;
-            T raw[8];
+            for (int i = 0; i < 8; ++i) y[i] = widen<T>(next[i]);
+            p += 8 * g.sc;
+            if (c + 8 < c1) load_classes(p, g.sc, c1 - c - 8, next);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < c1) raw[i] = z[(long long)(c + i) * g.sc];
-            float qs[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) qs[i] = 0.f;
-            if ((in >> i0) & 0xffu) {
-                for (int q = 0; q < k.K; ++q) {
-                    float v;
-                    const int at = load_entry(k, n, q, cats, v) - g.bg - c;
-                    const float wq = weight(t, v);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) qs[i] += at == i ? wq : 0.f;
-                }
-            }
+            for (int i = 0; i < 8; ++i) y[i] = grad_outside(r, g.c2, y[i]);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (c + i < c1) {
-                    const float v = to_f32(raw[i]);
-                    out[(long long)(c + i) * k.gsc] =
-                        from_f32<T>((in >> (i0 + i)) & 1u ? grad_inside(r, g.c2, v, qs[i]) : grad_outside(r, g.c2, v));
-                }
+                if (c + i < c1) out[i * k.gsc] = from_f32<T>(y[i]);
+            out += 8 * k.gsc;
         }
+        entries.each([&](int l, float) {
+            const int c = l - g.bg;
+            if (c < c0 || c >= c1) return;
+            float qs = 0.f;  // (the same label twice: each time the sum of all its entries, in their order)
+            entries.each([&](int o, float v) { qs += o == l ? weight(t, v) : 0.f; });
+            grad[c * k.gsc] = from_f32<T>(grad_inside(r, g.c2, to_f32(z[c * g.sc]), qs));
+        });
     }
 }
 
@@ -901,8 +998,33 @@ void small_of(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
 template <typename T, int G>
 void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of((k.g.rows + 256 / G - 1) / (256 / G), num_cu, 64)), block(256);
-    if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G>), grid, block, 0, st, k);
-    else hipLaunchKernelGGL((distill_group_kernel<T, G>), grid, block, 0, st, k);
+    // entries of a lane in registers: as many as 16 a row, or 64 where the lanes of a row are that many
+    constexpr int E = G >= 16 ? 64 / G : 16 / G > 4 ? 4 : 16 / G;
+    if (k.K <= G * E) {
+        if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, E>), grid, block, 0, st, k);
+        else hipLaunchKernelGGL((distill_group_kernel<T, G, E>), grid, block, 0, st, k);
+    } else {
+        if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, 0>), grid, block, 0, st, k);
+        else hipLaunchKernelGGL((distill_group_kernel<T, G, 0>), grid, block, 0, st, k);
+    }
+}
+template <typename T>
+void planes(const DistillK &k, int num_cu, hipStream_t st) {
+    const dim3 grid(grid_of((k.g.rows + 255) / 256, num_cu, 64)), block(256);
+    if (k.K <= 2) hipLaunchKernelGGL((distill_planes_kernel<T, 2>), grid, block, 0, st, k);
+    else if (k.K <= 4) hipLaunchKernelGGL((distill_planes_kernel<T, 4>), grid, block, 0, st, k);
+    else if (k.K <= 8) hipLaunchKernelGGL((distill_planes_kernel<T, 8>), grid, block, 0, st, k);
+    else hipLaunchKernelGGL((distill_planes_kernel<T, 0>), grid, block, 0, st, k);
+}
+template <typename T>
+void planes_grad(const DistillK &k, int num_cu, hipStream_t st) {
+    int parts;
+    const int len = cut_classes(k.g, num_cu, parts);
+    const dim3 grid(grid_of((k.g.rows + 255) / 256 * parts, num_cu, 64)), block(256);
+    if (k.K <= 2) hipLaunchKernelGGL((distill_grad_planes_kernel<T, 2>), grid, block, 0, st, k, parts, len);
+    else if (k.K <= 4) hipLaunchKernelGGL((distill_grad_planes_kernel<T, 4>), grid, block, 0, st, k, parts, len);
+    else if (k.K <= 8) hipLaunchKernelGGL((distill_grad_planes_kernel<T, 8>), grid, block, 0, st, k, parts, len);
+    else hipLaunchKernelGGL((distill_grad_planes_kernel<T, 0>), grid, block, 0, st, k, parts, len);
 }
 
 template <typename T>
@@ -913,7 +1035,7 @@ void launch(const DistillK &k, int num_cu, hipStream_t st) {
     if (!contig) {
         // (as in label_scores.hip: a lane a row from 64 rows a compute unit on, or where rows are short)
         if (g.C <= 64 || g.rows >= 64ll * num_cu)
-            hipLaunchKernelGGL(distill_planes_kernel<T>, dim3(grid_of((g.rows + 255) / 256, num_cu, 64)), dim3(256), 0, st, k);
+            planes<T>(k, num_cu, st);
         else
             hipLaunchKernelGGL(distill_wave_kernel<T>, dim3(grid_of((g.rows + 3) / 4, num_cu, 32)), dim3(256), 0, st, k);
         return;
@@ -943,9 +1065,7 @@ void launch_grad(const DistillK &k, int num_cu, hipStream_t st) {
     const bool contig = contiguous(g) && (k.gsc == 1 || g.C == 1);
     if (g.C <= 8) return small_of<T>(k, true, num_cu, st);
     if (!contig) {
-        const int parts = (g.C + 31) / 32;
-        hipLaunchKernelGGL(distill_grad_planes_kernel<T>, dim3(grid_of((g.rows + 255) / 256 * parts, num_cu, 64)), dim3(256), 0, st, k, parts);
-        return;
+        return planes_grad<T>(k, num_cu, st);
     }
     if (g.C <= 32) return group<T, 2>(k, true, num_cu, st);
     if (g.C <= 64) return group<T, 4>(k, true, num_cu, st);

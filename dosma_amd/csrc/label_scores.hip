@@ -15,9 +15,9 @@
 namespace qmri {
 
 Cut cut_rows(const LogitsK &g, int num_cu, int longest) {
-    // enough blocks for every compute unit twice over, but at least 2048 scores (two rounds of a block's loads) for each
+    // enough blocks for every compute unit twice over, but at least 4096 scores (a round of a block's loads) for each
     long long want = g.rows >= 2ll * num_cu ? 1 : (2ll * num_cu + g.rows - 1) / g.rows;
-    const long long most = (g.C + 2047) / 2048, least = (g.C + longest - 1) / longest;
+    const long long most = (g.C + 4095) / 4096, least = (g.C + longest - 1) / longest;
     if (want > most) want = most;
     if (want < least) want = least;
     Cut c;
@@ -58,6 +58,23 @@ __device__ __forceinline__ void given_label(const ScoresK &k, long long n, int c
     has = v >= 0 && v < cats;
     if (has) l = (int)v;
 }
+
+// ---- scores as keys -----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned ordered(float f) {  // the order of floats as that of unsigned integers; -0 ranks as +0
+    const int u = __float_as_int(f + 0.f);
+    return (unsigned)(u ^ ((u >> 31) | (int)0x80000000));
+}
+__device__ __forceinline__ float unordered(unsigned o) {
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+constexpr unsigned kKeyNegInf = 0x007fffffu;  // ordered(-inf)
+// significant bits of a widened score's key: the lower ones are all alike
+template <typename T>
+constexpr int kKeyBits = 32;
+template <>
+constexpr int kKeyBits<f16_t> = 19;
+template <>
+constexpr int kKeyBits<bf16_t> = 16;
 
 // ---- small: one lane a row ----------------------------------------------------------------------------------------------------
 // Bound by memory and, right behind, by the vector unit: a row of 4 scores in 32 bits is 16 bytes in and up to 32 out.
@@ -156,22 +173,47 @@ __global__ __launch_bounds__(256) void scores_group_kernel(const ScoresK k) {
         if (live && gl == 0) write_row(k, n, M, s, t, has, ignored, zl);
         if (k.top == 0) continue;
         const float ls = __builtin_amdgcn_logf(s) * kLn2;
-        for (int q = 0; q < k.top; ++q) {
-            // the largest of this lane's 16 (the first of equals: its labels rise with i only within a vector and from vector to vector)
-            float bv = x[16];
-            int bi = 0;
+        auto label_of = [&](int i) { return ((i / V) * G + gl) * V + i % V + g.bg; };
+        if constexpr (sizeof(T) == 2) {
+            // the significant bits of a score over the complement of its label (11 bits: up to 1024 classes), below 2^31: of the
+            // differences key - last those of the keys already taken are small, the others wrap around, in their order
+            constexpr int DOWN = 32 - kKeyBits<T>;
+            auto key_of = [&](float v, int label) { return ((ordered(v) >> DOWN) << 11) | (2047u - (unsigned)label); };
+            unsigned key[17];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const bool c = x[i] > bv;
-                bv = c ? x[i] : bv;
-                bi = c ? ((i / V) * G + gl) * V + i % V + g.bg : bi;
+            for (int i = 0; i < 16; ++i) key[i] = key_of(x[i], label_of(i));
+            key[16] = key_of(x[16], 0);
+            unsigned last = 0x80000000u;
+            for (int q = 0; q < k.top; ++q) {
+                unsigned m = key[16] - last;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const unsigned d = key[i] - last;
+                    m = d > m ? d : m;
+                }
+                last += group_maxu<G>(m);
+                const unsigned o = (last >> 11) << DOWN;
+                const float v = unordered(o & 0x80000000u ? o : o | ((1u << DOWN) - 1u));
+                if (live && gl == 0) write_top(k, n, q, v, v > kNegInf ? (int)(2047u - (last & 2047u)) : -1, M, ls);
             }
-            const float best = group_max<G>(bv);
-            const int at = group_min<G>(bv == best ? bi : 0x7fffffff);
-            if (live && gl == 0) write_top(k, n, q, best, best > kNegInf ? at : -1, M, ls);
+        } else {
+            for (int q = 0; q < k.top; ++q) {
+                float bv = x[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = ((i / V) * G + gl) * V + i % V + g.bg == at ? kNegInf : x[i];
-            if (at == 0 && g.bg) x[16] = kNegInf;
+                for (int i = 0; i < 16; ++i) bv = fmaxf(bv, x[i]);
+                const float best = group_max<G>(bv);
+                int bi = x[16] == best ? 0 : 0x7fffffff;
+#pragma unroll
+                for (int i = 15; i >= 0; --i) {
+                    const int l = label_of(i);
+                    bi = x[i] == best && l < bi ? l : bi;
+                }
+                const int at = group_min<G>(bi);
+                if (live && gl == 0) write_top(k, n, q, best, best > kNegInf ? at : -1, M, ls);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = label_of(i) == at ? kNegInf : x[i];
+                if (at == 0 && g.bg) x[16] = kNegInf;
+            }
         }
     }
 }
@@ -180,22 +222,6 @@ __global__ __launch_bounds__(256) void scores_group_kernel(const ScoresK k) {
 // A score can belong to the k best only if it is above a floor for which k others are known.  What passes the floor goes into a
 // buffer of the wave's in LDS; a full buffer is cut down to its k best, whose last is the new floor.  The order is (score falling,
 // label rising), so the result does not depend on who came first.
-__device__ __forceinline__ unsigned ordered(float f) {  // the order of floats as that of unsigned integers; -0 ranks as +0
-    const int u = __float_as_int(f + 0.f);
-    return (unsigned)(u ^ ((u >> 31) | (int)0x80000000));
-}
-__device__ __forceinline__ float unordered(unsigned o) {
-    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
-}
-constexpr unsigned kKeyNegInf = 0x007fffffu;  // ordered(-inf)
-// significant bits of a widened score's key: the lower ones are all alike
-template <typename T>
-constexpr int kKeyBits = 32;
-template <>
-constexpr int kKeyBits<f16_t> = 19;
-template <>
-constexpr int kKeyBits<bf16_t> = 16;
-
 // Which of the wave's 64 N (key, label) pairs are its k best; key 0: none.  The k-th largest key is found bit by bit.
 template <int N, int BITS>
 __device__ __forceinline__ unsigned select_best(const unsigned (&key)[N], const int (&id)[N], int k, bool (&win)[N]) {
@@ -206,6 +232,7 @@ __device__ __forceinline__ unsigned select_best(const unsigned (&key)[N], const 
         return c;
     };
     unsigned t = 0u;
+#pragma unroll 1
     for (int bit = 31; bit >= 32 - BITS; --bit) {
         const unsigned at = t | (1u << bit);
         if (count([&](int i) { return key[i] >= at; }) >= k) t = at;
@@ -216,6 +243,7 @@ __device__ __forceinline__ unsigned select_best(const unsigned (&key)[N], const 
     int last = 0x7fffffff;
     if (t != 0u && above + count([&](int i) { return (key[i] & top) == t; }) > k) {
         last = 0;
+#pragma unroll 1
         for (int bit = 30; bit >= 0; --bit) {  // the largest label of which fewer than k - above equals lie below
             const int at = last | (1 << bit);
             if (count([&](int i) { return (key[i] & top) == t && id[i] < at; }) < k - above) last = at;
@@ -296,26 +324,29 @@ struct WaveBest {
 
 // The floor that 64 N values (N a lane) give: k of them are at least as large as the k-th, so only what is above a lower value
 // can be among the best.
-template <int N>
+template <int N, int BITS>
 __device__ __forceinline__ float first_floor(const float *m, int k) {
     const int lane = threadIdx.x & 63;
     unsigned key[N];
 #pragma unroll
     for (int q = 0; q < N; ++q) key[q] = ordered(m[q * 64 + lane]);
     unsigned t = 0u;
-    for (int bit = 31; bit >= 12; --bit) {  // (the upper 20 bits will do: a floor that is a little low only lets more through)
+    constexpr int LOW = BITS < 20 ? 32 - BITS : 12;  // (the upper 20 bits will do: a floor that is a little low only lets more through)
+#pragma unroll 1
+    for (int bit = 31; bit >= LOW; --bit) {
         const unsigned at = t | (1u << bit);
         int c = 0;
 #pragma unroll
         for (int q = 0; q < N; ++q) c += __popcll(__ballot(key[q] >= at));
         if (c >= k) t = at;
     }
-    return t > kKeyNegInf + 0x1000u ? unordered(t - 0x1000u) : kNegInf;  // (the next lower of these 20-bit keys)
+    return t > kKeyNegInf + (1u << LOW) ? unordered(t - (1u << LOW)) : kNegInf;  // (the next lower of these keys)
 }
 
 // Up to 64 winners, one a lane (i < 0: none), into falling order: every lane counts the better ones.
 __device__ __forceinline__ int rank_of(float v, int i, int k) {
     int r = 0;
+#pragma unroll 1
     for (int o = 0; o < k; ++o) {
         const float ov = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), o));
         const int oi = __builtin_amdgcn_readlane(i, o);
@@ -332,18 +363,24 @@ __device__ __forceinline__ size_t part_words(int k) { return 4 + 2 * (size_t)k; 
 template <int W, int BITS>
 __device__ __forceinline__ void final_best(float *tv, int *ti, int k, float &bv, int &bi) {
     const int lane = threadIdx.x & 63;
-    unsigned key[W];
     int id[W];
     float sv[W];
     bool win[W];
+    int all = 0;
 #pragma unroll
     for (int q = 0; q < W; ++q) {
         id[q] = ti[q * kBuf + lane];
         sv[q] = tv[q * kBuf + lane];
-        key[q] = id[q] < 0 ? 0u : ordered(sv[q]);
+        win[q] = id[q] >= 0;
+        all += __popcll(__ballot(win[q]));
     }
     wave_sync();
-    select_best<W, BITS>(key, id, k, win);
+    if (all > 64) {  // (up to 64 are put in order as they are)
+        unsigned key[W];
+#pragma unroll
+        for (int q = 0; q < W; ++q) key[q] = win[q] ? ordered(sv[q]) : 0u;
+        select_best<W, BITS>(key, id, k, win);
+    }
     int n = 0;
 #pragma unroll
     for (int q = 0; q < W; ++q) {
@@ -372,10 +409,9 @@ __device__ __forceinline__ void final_best(float *tv, int *ti, int k, float &bv,
 // Per score: widen, half a maximum, one fused multiply, clamp, exp2 (two slots), one and a half sums -- about 8 issue slots, of
 // the 14 that a 2-byte score has at 5.5 TB/s: memory first, the vector unit close behind.
 template <typename T, bool TOP, int W>
-__global__ __launch_bounds__(64 * W, TOP ? 5 : 8) void scores_block_kernel(const ScoresK k, const Cut cut) {
+__global__ __launch_bounds__(64 * W, TOP ? 6 : sizeof(T) == 4 ? 6 : 8) void scores_block_kernel(const ScoresK k, const Cut cut) {
     __shared__ RowStat s_stat[W];
-    __shared__ float s_max[TOP ? 64 * W : 1];  // the lanes' largest, or the scores of up to four lanes of each wave
-    __shared__ int s_first[TOP ? 4 * W : 1];
+    __shared__ float s_max[TOP ? 64 * W : 1];  // the lanes' largest
     __shared__ float s_v[TOP ? W * kBuf : 1];
     __shared__ int s_i[TOP ? W * kBuf : 1];
     const LogitsK &g = k.g;
@@ -388,19 +424,28 @@ __global__ __launch_bounds__(64 * W, TOP ? 5 : 8) void scores_block_kernel(const
         const int c0 = seg * cut.len, c1 = c0 + cut.len < g.C ? c0 + cut.len : g.C;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
         const bool back = g.bg && seg == 0 && w == 0;
+        // the given label's score, needed last, is on its way from the start
+        int l = -1;
+        bool has = false, ignored = false;
+        float zl = 0.f;
+        if (w == 0 && cut.segs == 1) {
+            given_label(k, n, g.C + g.bg, l, has, ignored);
+            if (has && l >= g.bg) zl = to_f32(z[l - g.bg]);
+        }
         Running r = no_scores();
         if (back && lane == 0) r = {0.f, 0.f, 1.f, 0.f};  // the implicit category: lane 0 has seen a score of 0
         WaveBest b = {s_v + (TOP ? w * kBuf : 0), s_i + (TOP ? w * kBuf : 0), 0, kNegInf, 0, k.top};
-        // the best k of the lanes' largest so far: nothing below the last of them can be among the best of the row
+        // the best k of the lanes' largest so far: nothing below the last of them can be among the best of the row.  (What the
+        // other waves have written meanwhile does not matter: older maxima are scores of the row as well.)
         auto raise_floor = [&](float m) {
+            wave_sync();
             s_max[threadIdx.x] = m;
-            __syncthreads();
-            const float f = first_floor<W>(s_max, k.top);
+            wave_sync();
+            const float f = first_floor<W, BITS>(s_max, k.top);
             if (f > b.floor) {
                 b.floor = f;
                 b.bound = 0;
             }
-            __syncthreads();
         };
         const int rounds = (c1 - c0 + W * TILE - 1) / (W * TILE);
         int c = c0 + w * TILE;
@@ -417,6 +462,8 @@ __global__ __launch_bounds__(64 * W, TOP ? 5 : 8) void scores_block_kernel(const
             if (TOP && it == 0) {
                 float cm = back && lane == 0 ? 0.f : kNegInf;
                 if (mine) cm = fmaxf(cm, max_of(x));
+                s_max[threadIdx.x] = cm;
+                __syncthreads();
                 raise_floor(cm);
                 if (back && b.passes(0.f, 0)) {
                     if (lane == 0) {
@@ -427,31 +474,27 @@ __global__ __launch_bounds__(64 * W, TOP ? 5 : 8) void scores_block_kernel(const
                 }
             }
             if (mine) {
-                add_scores(r, x, g.c2);
+                const float cm = add_scores(r, x, g.c2);
                 if (TOP) {
-                    // lanes that hold something for the list hand their 16 scores over through LDS, four lanes at a time, so that
-                    // all 64 lanes look at one each
-                    float *stage = s_max + w * 64;
-                    for (unsigned long long m = __ballot(max_of(x) >= b.floor); m != 0ull;) {
-                        const int rank = WaveBest::place(m);
-                        const bool give = (m >> lane) & 1ull && rank < 4;
-                        if (give) {
+                    // the 16 scores of lanes that hold something for the list are read again, four lanes' at a time, one a lane
+                    for (unsigned long long m = __ballot(cm >= b.floor); m != 0ull;) {
+                        int from = 0, have = 0;
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) stage[rank * 16 + i] = x[i];
-                            s_first[w * 4 + rank] = lane;
-                        }
-                        const int have = __popcll(m) < 4 ? __popcll(m) : 4;
-                        m &= ~__ballot(give);
-                        wave_sync();
-                        const int from = s_first[w * 4 + (lane >> 4)];
-                        const float v = stage[lane];
-                        wave_sync();
-                        b.take<BITS>(v, c + tile_at<T>(from, lane & 15) + g.bg, (lane >> 4) < have);
+                        for (int q = 0; q < 4; ++q)
+                            if (m != 0ull) {
+                                const int l = __ffsll(m) - 1;
+                                from = (lane >> 4) == q ? l : from;
+                                m &= m - 1;
+                                have = q + 1;
+                            }
+                        const int j = c + tile_at<T>(from, lane & 15);
+                        const bool in = (lane >> 4) < have && j < c1;
+                        b.take<BITS>(in ? to_f32(z[j]) : kNegInf, j + g.bg, in);
                     }
                 }
             }
-            // every time the scores seen have doubled
-            if (TOP && it > 0 && (it & (it + 1)) == 0 && it + 1 < rounds) raise_floor(r.m);
+            // every time the scores seen have quadrupled
+            if (TOP && (it == 3 || it == 15 || it == 63) && it + 1 < rounds) raise_floor(r.m);
         }
         RowStat st = wave_stat(r, g.c2, [&](int j) {
             // (w's scores in the order of its tiles; -1: the implicit category, seen by lane 0)
@@ -461,17 +504,17 @@ __global__ __launch_bounds__(64 * W, TOP ? 5 : 8) void scores_block_kernel(const
         }, back ? lane - 64 : lane, 64, rounds * TILE);
         if (lane == 0) s_stat[w] = st;
         if (TOP) {
-            if (b.n > k.top) b.cut<BITS>();
+            if (b.n > 64) b.cut<BITS>();
             for (int q = b.n + lane; q < 64; q += 64) b.i[q] = -1;
         }
         __syncthreads();
         if (w == 0) {
-            st = s_stat[0];
-#pragma unroll
-            for (int o = 1; o < W; ++o) st = join(st, s_stat[o], g.c2);
             float bv = kNegInf;
             int bi = -1;
             if (TOP) final_best<W, BITS>(s_v, s_i, k.top, bv, bi);
+            st = s_stat[0];
+#pragma unroll
+            for (int o = 1; o < W; ++o) st = join(st, s_stat[o], g.c2);
             if (cut.segs > 1) {
                 float *p = static_cast<float *>(k.ws) + (size_t)item * part_words(TOP ? k.top : 0);
                 if (lane == 0) {
@@ -486,13 +529,7 @@ __global__ __launch_bounds__(64 * W, TOP ? 5 : 8) void scores_block_kernel(const
             } else {
                 const float ls = __builtin_amdgcn_logf(st.s) * kLn2;
                 if (TOP && lane < k.top) write_top(k, n, lane, bv, bi, st.m, ls);
-                if (lane == 0) {
-                    int l;
-                    bool has, ignored;
-                    given_label(k, n, g.C + g.bg, l, has, ignored);
-                    const float zl = (has && l >= g.bg) ? to_f32(z[l - g.bg]) : 0.f;
-                    write_row(k, n, st.m, st.s, st.t, has, ignored, zl);
-                }
+                if (lane == 0) write_row(k, n, st.m, st.s, st.t, has, ignored, zl);
             }
         }
         __syncthreads();
@@ -503,6 +540,7 @@ __global__ __launch_bounds__(64 * W, TOP ? 5 : 8) void scores_block_kernel(const
 template <typename T>
 __global__ __launch_bounds__(256) void scores_join_kernel(const ScoresK k, const Cut cut) {
     __shared__ RowStat s_stat[4];
+    __shared__ float s_max[256];
     __shared__ float s_v[4 * kBuf];
     __shared__ int s_i[4 * kBuf];
     constexpr int BITS = kKeyBits<T>;
@@ -529,13 +567,19 @@ __global__ __launch_bounds__(256) void scores_join_kernel(const ScoresK k, const
         WaveBest b = {s_v + w * kBuf, s_i + w * kBuf, 0, kNegInf, 0, k.top};
         if (k.top) {
             const int pairs = cut.segs * k.top;
+            // (the segments' first: k of them are at least as large as the k-th)
+            if (cut.segs >= k.top) {
+                s_max[threadIdx.x] = (int)threadIdx.x < cut.segs ? p[threadIdx.x * words + 4] : kNegInf;
+                __syncthreads();
+                b.floor = first_floor<4, BITS>(s_max, k.top);
+            }
             for (int q0 = w * 64; q0 < pairs; q0 += 256) {
                 const int q = q0 + lane, sg = q / k.top, at = q - sg * k.top;
                 const float *a = p + sg * words + 4;
                 const bool in = q < pairs;
                 b.take<BITS>(in ? a[at] : kNegInf, in ? reinterpret_cast<const int *>(a)[k.top + at] : -1, in);
             }
-            if (b.n > k.top) b.cut<BITS>();
+            if (b.n > 64) b.cut<BITS>();
             for (int q = b.n + lane; q < 64; q += 64) b.i[q] = -1;
         }
         __syncthreads();
@@ -555,17 +599,14 @@ __global__ __launch_bounds__(256) void scores_join_kernel(const ScoresK k, const
 }
 
 // ---- planes: one lane a row, more than 8 classes ---------------------------------------------------------------------------
-// Neighbouring lanes read neighbouring rows.  The best are a sorted list in registers.  Of 2-byte scores a key of 32 bits, the
-// ordered score over the complement of the label, enters it with one v_med3 a level; 4-byte scores carry the label beside.
-__device__ __forceinline__ unsigned score_key(unsigned short u, int label) {
-    const unsigned hi = (u == 0x8000u) ? 0u : (unsigned)u << 16;  // -0 ranks as +0
-    const unsigned ordered = hi ^ ((unsigned)((int)hi >> 31) | 0x80000000u);
-    return (ordered & 0xffff0000u) | (0xffffu - (unsigned)label);
-}
-__device__ __forceinline__ unsigned med3u(unsigned a, unsigned b, unsigned c) {
-    const unsigned lo = a < b ? a : b, hi = a < b ? b : a;
-    return hi < c ? hi : (lo > c ? lo : c);
-}
+// Neighbouring lanes read neighbouring rows.  The best are a sorted list in registers.  A widened 2-byte score leaves the lower
+// bits of its 32 unused: with the label's complement there, score and label are one unsigned key, and a key enters the list with
+// one v_med3 a level; 4-byte scores carry the label beside.
+template <typename T>
+constexpr int kLabelBits = 32 - kKeyBits<T>;
+__device__ __forceinline__ unsigned minu(unsigned a, unsigned b) { return a < b ? a : b; }
+__device__ __forceinline__ unsigned maxu(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned med3u(unsigned a, unsigned b, unsigned c) { return maxu(minu(a, b), minu(maxu(a, b), c)); }
 template <typename T, int K>
 struct LaneBest {  // any type: score and label side by side
     float v[K > 0 ? K : 1];
@@ -577,8 +618,8 @@ struct LaneBest {  // any type: score and label side by side
             i[q] = -1;
         }
     }
-    __device__ void take(T, float x, int label) {
-        if (K > 4 && __ballot(x > v[K - 1]) == 0ull) return;
+    __device__ void take(float x, int label) {
+        if (K > 4 && __ballot(x > v[K > 0 ? K - 1 : 0]) == 0ull) return;
 #pragma unroll
         for (int q = K - 1; q >= 0; --q) {
             const bool above = q > 0 && x > v[q > 0 ? q - 1 : 0], here = x > v[q];
@@ -590,31 +631,26 @@ struct LaneBest {  // any type: score and label side by side
     __device__ int label(int q) const { return i[q]; }
 };
 template <typename T, int K>
-struct LaneBestKey {  // 2-byte scores, labels below 65536 (those of the last, partly filled step of 8 included)
+struct LaneBestKey {  // 2-byte scores, labels that fit the unused bits
+    static constexpr unsigned MASK = kLabelBits<T> < 32 ? (1u << (kLabelBits<T> % 32)) - 1u : 0u;
     unsigned key[K > 0 ? K : 1];
     __device__ void clear() {
 #pragma unroll
         for (int q = 0; q < K; ++q) key[q] = 0u;
     }
-    __device__ void take(T raw, float, int label) {
-        unsigned short u;
-        __builtin_memcpy(&u, &raw, 2);
-        const unsigned x = score_key(u, label);
-        if (K > 4 && __ballot(x > key[K - 1]) == 0ull) return;
+    __device__ void take(float x, int label) {
+        const unsigned k = (ordered(x) & ~MASK) | (MASK - (unsigned)label);
+        if (K > 4 && __ballot(k > key[K > 0 ? K - 1 : 0]) == 0ull) return;
 #pragma unroll
-        for (int q = K - 1; q > 0; --q) key[q] = med3u(key[q - 1], key[q], x);
-        if (K > 0) key[0] = key[0] > x ? key[0] : x;
+        for (int q = K - 1; q > 0; --q) key[q] = med3u(key[q - 1], key[q], k);
+        if (K > 0) key[0] = maxu(key[0], k);
     }
     __device__ float score(int q) const {
-        const unsigned o = key[q] & 0xffff0000u;
-        unsigned hi = (o & 0x80000000u) ? o ^ 0x80000000u : ~o & 0xffff0000u;
-        if (key[q] == 0u) return kNegInf;
-        const unsigned short u = (unsigned short)(hi >> 16);
-        T r;
-        __builtin_memcpy(&r, &u, 2);
-        return to_f32(r);
+        // (below the significant bits a negative score's key has ones)
+        const unsigned o = key[q] & 0x80000000u ? key[q] & ~MASK : key[q] | MASK;
+        return (key[q] & ~MASK) <= (kKeyNegInf & ~MASK) ? kNegInf : unordered(o);
     }
-    __device__ int label(int q) const { return score(q) > kNegInf ? (int)(0xffffu - (key[q] & 0xffffu)) : -1; }
+    __device__ int label(int q) const { return (int)(MASK - (key[q] & MASK)); }
 };
 
 template <typename T, int K, bool KEY>
@@ -632,38 +668,23 @@ __global__ __launch_bounds__(256) void scores_planes_kernel(const ScoresK k) {
         Running r = no_scores();
         if (g.bg) {
             r = {0.f, 0.f, 1.f, 0.f};
-            if (K) best.take(static_cast<T>(0.f), 0.f, 0);
+            if (K) best.take(0.f, 0);
         }
-        auto eight = [&](const T (&raw)[8], int c) {
+        unsigned next[8];
+        load_classes(z, g.sc, g.C, next);
+        const T *p = z;
+        for (int c = 0; c < g.C; c += 8) {
             float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = to_f32(raw[i]);
+            for (int i = 0; i < 8; ++i) x[i] = widen<T>(next[i]);
+            p += 8 * g.sc;
+            if (c + 8 < g.C) load_classes(p, g.sc, g.C - c - 8, next);
             add_scores(r, x, g.c2);
             if (K) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) best.take(raw[i], x[i], c + i + g.bg);
+                for (int i = 0; i < 8; ++i) best.take(x[i], c + i + g.bg);
             }
-        };
-        const int whole = g.C & ~7;
-        T next[8];
-        const T *p = z;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) next[i] = p[i * g.sc];  // (more than 8 classes here)
-        for (int c = 0; c < whole; c += 8) {
-            T raw[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) raw[i] = next[i];
-            p += 8 * g.sc;
-            if (c + 16 <= g.C) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) next[i] = p[i * g.sc];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) next[i] = c + 8 + i < g.C ? p[i * g.sc] : static_cast<T>(kNegInf);
-            }
-            eight(raw, c);
         }
-        if (whole < g.C) eight(next, whole);
         RowStat st = {r.m, reference(r.m), 0.f, 0.f};
         if (far_scores(r.m, g.c2)) {
             for (int c = -g.bg; c < g.C; ++c) {
@@ -865,27 +886,33 @@ __global__ __launch_bounds__(256) void scores_grad_block_kernel(const ScoresK k,
     }
 }
 
-// Classes that do not lie together: neighbouring lanes take neighbouring rows (planes), a block 256 rows and 32 classes.
+// Classes that do not lie together: neighbouring lanes take neighbouring rows, a block 256 rows and `len` classes of them.
 template <typename T>
-__global__ __launch_bounds__(256) void scores_grad_planes_kernel(const ScoresK k, int parts) {
+__global__ __launch_bounds__(256) void scores_grad_planes_kernel(const ScoresK k, int parts, int len) {
     const LogitsK &g = k.g;
     const long long blocks = (g.rows + 255) / 256;
     for (long long item = blockIdx.x; item < blocks * parts; item += gridDim.x) {
-        const long long rb = item / parts;
-        const int c0 = (int)(item - rb * parts) * 32, c1 = c0 + 32 < g.C ? c0 + 32 : g.C;
+        const long long rb = parts == 1 ? item : item / parts;
+        const int c0 = (int)(item - rb * parts) * len, c1 = c0 + len < g.C ? c0 + len : g.C;
         const long long n = rb * 256 + threadIdx.x;
         if (n >= g.rows) continue;
-        const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
-        T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi);
+        const T *p = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si) + c0 * g.sc;
+        T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi) + c0 * k.gsc;
+        unsigned next[8];
+        load_classes(p, g.sc, c1 - c0, next);
         const GradRow r = grad_row(k, n, g.C + g.bg);
         for (int c = c0; c < c1; c += 8) {
-            T raw[8];
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = widen<T>(next[i]);
+            p += 8 * g.sc;
+            if (c + 8 < c1) load_classes(p, g.sc, c1 - c - 8, next);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = grad_score(r, g.c2, g.invT, y[i], c + i + g.bg);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (c + i < c1) raw[i] = z[(long long)(c + i) * g.sc];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < c1) out[(long long)(c + i) * k.gsc] = from_f32<T>(grad_score(r, g.c2, g.invT, to_f32(raw[i]), c + i + g.bg));
+                if (c + i < c1) out[i * k.gsc] = from_f32<T>(y[i]);
+            out += 8 * k.gsc;
         }
     }
 }
@@ -925,7 +952,8 @@ void group(const ScoresK &k, bool grad, int num_cu, hipStream_t st) {
 template <typename T, int K>
 void planes(const ScoresK &k, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of((k.g.rows + 255) / 256, num_cu, 64)), block(256);
-    if (sizeof(T) == 2 && k.g.C <= 65528) hipLaunchKernelGGL((scores_planes_kernel<T, K, sizeof(T) == 2>), grid, block, 0, st, k);
+    // (the last eight classes may reach 7 labels beyond the last)
+    if (sizeof(T) == 2 && k.g.C + k.g.bg + 7 <= (1 << kLabelBits<T>)) hipLaunchKernelGGL((scores_planes_kernel<T, K, sizeof(T) == 2>), grid, block, 0, st, k);
     else hipLaunchKernelGGL((scores_planes_kernel<T, K, false>), grid, block, 0, st, k);
 }
 
@@ -970,9 +998,12 @@ void launch(const ScoresK &k, int num_cu, hipStream_t st) {
     if (g.C <= 1024) return group<T, 64>(k, false, num_cu, st);
     const Cut cut = cut_rows(g, num_cu, 1 << 30);
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
-    // eight waves where the segments are long enough for two rounds of all of them: the loads in flight bound the rate
-    if (k.top) {
-        hipLaunchKernelGGL((scores_block_kernel<T, true, 4>), grid, dim3(256), 0, st, k, cut);
+    if (g.C <= 16384 && g.rows >= 16ll * num_cu) {
+        if (k.top) hipLaunchKernelGGL((scores_block_kernel<T, true, 1>), grid, dim3(64), 0, st, k, cut);
+        else hipLaunchKernelGGL((scores_block_kernel<T, false, 1>), grid, dim3(64), 0, st, k, cut);
+    } else if (k.top) {
+        const size_t pad = spread_lds(g.rows * cut.segs, num_cu, 5, 4 * (kBuf * 8 + 64 * 4 + (int)sizeof(RowStat)));
+        hipLaunchKernelGGL((scores_block_kernel<T, true, 4>), grid, dim3(256), pad, st, k, cut);
     } else if (cut.len >= 16384) {
         hipLaunchKernelGGL((scores_block_kernel<T, false, 8>), grid, dim3(512), 0, st, k, cut);
     } else {
@@ -998,8 +1029,9 @@ void launch_grad(const ScoresK &k, int num_cu, hipStream_t st) {
         }
     }
     if (!contig) {
-        const int parts = (g.C + 31) / 32;
-        hipLaunchKernelGGL(scores_grad_planes_kernel<T>, dim3(grid_of((g.rows + 255) / 256 * parts, num_cu, 64)), dim3(256), 0, st, k, parts);
+        int parts;
+        const int len = cut_classes(g, num_cu, parts);
+        hipLaunchKernelGGL(scores_grad_planes_kernel<T>, dim3(grid_of((g.rows + 255) / 256 * parts, num_cu, 64)), dim3(256), 0, st, k, parts, len);
         return;
     }
     if (g.C <= 32) return group<T, 2>(k, true, num_cu, st);
