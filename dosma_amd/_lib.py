@@ -179,6 +179,16 @@ class QmriDistillArgs(ctypes.Structure):
     ]
 
 
+class QmriUnet2dScoreArgs(ctypes.Structure):
+    _fields_ = [
+        ("vol_hws", ctypes.c_void_p), ("S", ctypes.c_int32), ("whiten", ctypes.c_int32), ("whiten_eps", ctypes.c_double),
+        ("temperature", ctypes.c_double), ("labels_hws", ctypes.c_void_p), ("log_prob_hws", ctypes.c_void_p),
+        ("entropy_hws", ctypes.c_void_p), ("top", ctypes.c_int32), ("entries", ctypes.c_int32), ("top_label", ctypes.c_void_p),
+        ("top_log_prob", ctypes.c_void_p), ("teacher_label", ctypes.c_void_p), ("teacher_log_prob", ctypes.c_void_p),
+        ("divergence_hws", ctypes.c_void_p), ("stream", ctypes.c_void_p),
+    ]
+
+
 L_KINDS = {"int32": 0, "uint8": 1, "int16": 2, "int64": 3}
 SCORE_DTYPES = {"float32": QMRI_F32, "float16": QMRI_F16, "bfloat16": QMRI_BF16}
 MAX_TOP = 64
@@ -201,7 +211,7 @@ EXPORTS = (
     "qmri_region_stats_device", "qmri_host_alloc", "qmri_host_free", "qmri_device_mem_info", "qmri_selftest_fp64",
     "qmri_label_scores_device", "qmri_label_scores_host", "qmri_label_scores_grad_device", "qmri_label_scores_grad_host",
     "qmri_label_scores_workspace", "qmri_distill_device", "qmri_distill_host", "qmri_distill_grad_device",
-    "qmri_distill_grad_host", "qmri_distill_workspace",
+    "qmri_distill_grad_host", "qmri_distill_workspace", "qmri_unet2d_score_volume",
 )
 
 _lib = None
@@ -317,6 +327,8 @@ def load():
         lib.qmri_unet2d_segment_volume.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
                                                    ctypes.c_double, ctypes.c_void_p, ctypes.c_void_p]
         lib.qmri_unet2d_segment_volume.restype = ctypes.c_int
+        lib.qmri_unet2d_score_volume.argtypes = [ctypes.c_void_p, ctypes.POINTER(QmriUnet2dScoreArgs)]
+        lib.qmri_unet2d_score_volume.restype = ctypes.c_int
         lib.qmri_unet2d_destroy.argtypes = [ctypes.c_void_p]
         lib.qmri_unet2d_destroy.restype = ctypes.c_int
         lib.qmri_conv2d_nhwc_host.argtypes = [
@@ -742,6 +754,45 @@ class Unet2dEngine:
         out = _hostpool.empty((self.n_classes, self.H, self.W, S), np.uint8)
         check(self._lib.qmri_unet2d_segment_volume(self._handle, _ptr(v), S, 1 if whiten else 0, float(eps),
                                                    _ptr(out), None))
+        return out
+
+    def score_volume(self, vol_hws, *, whiten=False, eps=0.0, temperature=1.0, labels=None, entropy=False, top=0, teacher=None):
+        """What the network's answers say on a (H, W, S) volume (``qmri_unet2d_score_volume``), the background as category 0:
+        dict of ``log_prob`` (of the uint8 ``labels``, 255 = none), ``entropy``, ``top_label`` uint8 / ``top_log_prob``
+        (top, H, W, S), and ``divergence`` from ``teacher`` = (labels uint8, log probabilities float32), (entries, H, W, S)."""
+        v = np.ascontiguousarray(vol_hws, dtype=np.float32)
+        if v.ndim != 3 or v.shape[:2] != (self.H, self.W):
+            raise ValueError(f"volume is {v.shape}, model was built for slices of {(self.H, self.W)}")
+        a = QmriUnet2dScoreArgs()
+        a.vol_hws, a.S = _ptr(v), v.shape[2]
+        a.whiten, a.whiten_eps, a.temperature = 1 if whiten else 0, float(eps), float(temperature)
+        out, keep = {}, [v]
+        if labels is not None:
+            labels = np.ascontiguousarray(labels)
+            if labels.shape != v.shape or labels.dtype != np.uint8:
+                raise ValueError(f"labels must be uint8 of shape {v.shape}, got {labels.dtype} {labels.shape}")
+            keep.append(labels)
+            out["log_prob"] = _hostpool.empty(v.shape, np.float32)
+            a.labels_hws, a.log_prob_hws = _ptr(labels), _ptr(out["log_prob"])
+        if entropy:
+            out["entropy"] = _hostpool.empty(v.shape, np.float32)
+            a.entropy_hws = _ptr(out["entropy"])
+        a.top = int(top)
+        if a.top > 0:
+            out["top_label"] = _hostpool.empty((a.top,) + v.shape, np.uint8)
+            out["top_log_prob"] = _hostpool.empty((a.top,) + v.shape, np.float32)
+            a.top_label, a.top_log_prob = _ptr(out["top_label"]), _ptr(out["top_log_prob"])
+        if teacher is not None:
+            t_lab, t_lp = np.ascontiguousarray(teacher[0]), np.ascontiguousarray(teacher[1])
+            if (t_lab.dtype != np.uint8 or t_lp.dtype != np.float32 or t_lab.shape != t_lp.shape or t_lab.ndim != 4
+                    or t_lab.shape[1:] != v.shape or t_lab.shape[0] < 1):
+                raise ValueError(f"teacher must be uint8 labels and float32 log probabilities of shape (entries, *{v.shape})")
+            keep += [t_lab, t_lp]
+            out["divergence"] = _hostpool.empty(v.shape, np.float32)
+            a.entries, a.teacher_label, a.teacher_log_prob = t_lab.shape[0], _ptr(t_lab), _ptr(t_lp)
+            a.divergence_hws = _ptr(out["divergence"])
+        check(self._lib.qmri_unet2d_score_volume(self._handle, ctypes.byref(a)))
+        del keep
         return out
 
     def forward_device(self, x_ptr, S, logits_ptr, mask_ptr, *, whiten=False, eps=0.0, stream=None):

@@ -18,6 +18,7 @@
 #include <string>
 #include <vector>
 
+#include "answers.h"
 #include "qmri_internal.h"
 
 namespace {
@@ -1340,6 +1341,121 @@ int qmri_unet2d_segment_volume(void *handle, const float *vol_hws, int32_t S, in
     U_TRY(hipMemcpyAsync(mask_chws, U->mask_planes.p, (size_t)n * U->ncls, hipMemcpyDeviceToHost, st));
     U_TRY(hipStreamSynchronize(st));
     return QMRI_OK;
+}
+
+// The network's answers on a whole volume: label scores and the divergence from a teacher's, in the same layouts.
+int qmri_unet2d_score_volume(void *handle, const qmri_unet2d_score_args *a) {
+    if (!handle || !a || (a->S != 0 && !a->vol_hws)) return ufail(QMRI_ERR_ARG, "handle / args / volume is NULL");
+    Unet *U = static_cast<Unet *>(handle);
+    const int S = a->S, cats = U->ncls + 1;
+    if (S < 0) return ufail(QMRI_ERR_ARG, "S < 0");
+    if (!(a->temperature >= 1e-30 && a->temperature <= 1e30)) return ufail(QMRI_ERR_ARG, "temperature must be in [1e-30, 1e30]");
+    if (a->top < 0 || a->top > cats) return ufail(QMRI_ERR_ARG, "top = %d, but there are %d categories", a->top, cats);
+    if (a->entries < 0 || a->entries > cats) return ufail(QMRI_ERR_ARG, "entries = %d, but there are %d categories", a->entries, cats);
+    if (a->top > 0 && (!a->top_label || !a->top_log_prob)) return ufail(QMRI_ERR_ARG, "top_label / top_log_prob is NULL");
+    if (a->entries > 0 && (!a->teacher_label || !a->teacher_log_prob || !a->divergence_hws))
+        return ufail(QMRI_ERR_ARG, "teacher_label / teacher_log_prob / divergence is NULL");
+    if (a->log_prob_hws && !a->labels_hws) return ufail(QMRI_ERR_ARG, "log_prob needs labels");
+    if (S == 0) return QMRI_OK;
+    hipStream_t st = static_cast<hipStream_t>(a->stream);
+    U_TRY(hipSetDevice(U->device));
+    int num_cu = 0;
+    U_TRY(hipDeviceGetAttribute(&num_cu, hipDeviceAttributeMultiprocessorCount, U->device));
+    const long long P = (long long)U->H * U->W, n = (long long)S * P;
+    const int K = a->top, E = a->entries, most = K > E ? (K > 1 ? K : 1) : (E > 1 ? E : 1);
+    // staging (planes as the caller's arrays, one at a time) and the rows the kernels work on
+    DevBuf planes, lab, lp, ent, tl, tv, el, ev, div;
+    U_TRY(planes.alloc((size_t)n * 4 * most));
+    if (a->log_prob_hws) {
+        U_TRY(lab.alloc((size_t)n));
+        U_TRY(lp.alloc((size_t)n * 4));
+        U_TRY(hipMemcpyAsync(planes.p, a->labels_hws, (size_t)n, hipMemcpyHostToDevice, st));
+        U_TRY(qmri::planes_to_rows_launch(planes.p, 1, P, S, 1, lab.p, st));
+    }
+    if (a->entropy_hws) U_TRY(ent.alloc((size_t)n * 4));
+    if (K) {
+        U_TRY(tl.alloc((size_t)n * K * 4));
+        U_TRY(tv.alloc((size_t)n * K * 4));
+    }
+    if (E) {
+        U_TRY(el.alloc((size_t)n * E * 4));
+        U_TRY(ev.alloc((size_t)n * E * 4));
+        U_TRY(div.alloc((size_t)n * 4));
+        U_TRY(hipMemcpyAsync(planes.p, a->teacher_label, (size_t)n * E, hipMemcpyHostToDevice, st));
+        U_TRY(qmri::planes_to_rows_launch(planes.p, 2, P, S, E, el.p, st));
+        U_TRY(hipMemcpyAsync(planes.p, a->teacher_log_prob, (size_t)n * E * 4, hipMemcpyHostToDevice, st));
+        U_TRY(qmri::planes_to_rows_launch(planes.p, 0, P, S, E, ev.p, st));
+    }
+    if (U->vol_cap < n) {
+        U_TRY(U->vol.alloc((size_t)n * 4));
+        U->vol_cap = n;
+    }
+    U_TRY(hipMemcpyAsync(planes.p, a->vol_hws, (size_t)n * 4, hipMemcpyHostToDevice, st));
+    U_TRY(qmri::transpose_ps_launch(planes.as<float>(), P, S, U->vol.as<float>(), st));
+    if (a->whiten) U_TRY(qmri::whiten_launch(U->vol.as<float>(), n, a->whiten_eps, U->stats.as<double>(), U->vol.as<float>(), st));
+    if (!U->logits.p) U_TRY(U->logits.alloc((size_t)U->maxB * P * U->ncls * 4));
+    auto body = [&]() -> int {
+        for (int s0 = 0; s0 < S; s0 += U->maxB) {
+            const int Bt = (S - s0) < U->maxB ? (S - s0) : U->maxB;
+            U_TRY(load_batch(U, U->vol.as<float>() + (long long)s0 * P, (long long)Bt * P, st));
+            const int rc = forward_batch(U, Bt, U->logits.as<float>(), nullptr, st);
+            if (rc != QMRI_OK) return rc;
+            const long long r0 = (long long)s0 * P;
+            qmri::LogitsK g;
+            std::memset(&g, 0, sizeof(g));
+            g.z = U->logits.p;
+            g.rows = g.inner = (long long)Bt * P;
+            g.si = U->ncls;
+            g.sc = 1;
+            g.C = U->ncls;
+            g.bg = 1;
+            g.c2 = (float)(1.4426950408889634074 / a->temperature);
+            g.invT = (float)(1.0 / a->temperature);
+            if (lp.p || ent.p || K) {
+                qmri::ScoresK k;
+                std::memset(&k, 0, sizeof(k));
+                k.g = g;
+                k.labels = lp.p ? lab.as<unsigned char>() + r0 : nullptr;
+                k.l_kind = QMRI_L_U8;
+                k.ignore = 255;
+                k.top = K;
+                k.log_prob = lp.p ? lp.as<float>() + r0 : nullptr;
+                k.entropy = ent.p ? ent.as<float>() + r0 : nullptr;
+                k.top_log_prob = K ? tv.as<float>() + r0 * K : nullptr;
+                k.top_label = K ? tl.as<int>() + r0 * K : nullptr;
+                U_TRY(qmri::label_scores_launch(k, QMRI_F32, num_cu, st));
+            }
+            if (E) {
+                qmri::DistillK k;
+                std::memset(&k, 0, sizeof(k));
+                k.g = g;
+                k.labels = el.as<int>() + r0 * E;
+                k.values = ev.as<float>() + r0 * E;
+                k.l_kind = QMRI_L_I32;
+                k.v_dtype = QMRI_F32;
+                k.K = E;
+                k.tail = 1;
+                k.loss = div.as<float>() + r0;
+                U_TRY(qmri::distill_launch(k, QMRI_F32, num_cu, st));
+            }
+        }
+        return QMRI_OK;
+    };
+    const int rc = run_in_range(U, U->vol.as<float>(), n, a->whiten != 0, st, body);
+    if (rc != QMRI_OK) return rc;
+    auto give = [&](const void *rows, int is_label, int k, void *out) -> int {
+        U_TRY(qmri::rows_to_planes_launch(rows, is_label, P, S, k, planes.p, st));
+        U_TRY(hipMemcpyAsync(out, planes.p, (size_t)n * k * (is_label ? 1 : 4), hipMemcpyDeviceToHost, st));
+        return QMRI_OK;
+    };
+    int ok = QMRI_OK;
+    if (ok == QMRI_OK && a->log_prob_hws) ok = give(lp.p, 0, 1, a->log_prob_hws);
+    if (ok == QMRI_OK && a->entropy_hws) ok = give(ent.p, 0, 1, a->entropy_hws);
+    if (ok == QMRI_OK && K) ok = give(tl.p, 1, K, a->top_label);
+    if (ok == QMRI_OK && K) ok = give(tv.p, 0, K, a->top_log_prob);
+    if (ok == QMRI_OK && E) ok = give(div.p, 0, 1, a->divergence_hws);
+    U_TRY(hipStreamSynchronize(st));
+    return ok;
 }
 
 // Single-layer entry for unit tests and for users who want the operators alone: host NHWC fp32 in/out.

@@ -7,6 +7,7 @@ preprocessing and ``generate_mask`` plumbing (deepcopy, reformat to SAGITTAL, (s
 ``libqmri_hip.so`` (conv / transposed conv / BN affine on MFMA).
 """
 import os
+from collections import namedtuple
 from copy import deepcopy
 
 import numpy as np
@@ -15,7 +16,12 @@ from dosma_amd.med_volume import MedicalVolume
 from dosma_amd.models.seg_model import HipSegModel, whiten_volume  # noqa: F401
 from dosma_amd.orientation import SAGITTAL
 
-__all__ = ["OAIUnet2D", "IWOAIOAIUnet2D", "IWOAIOAIUnet2DNormalized"]
+__all__ = ["OAIUnet2D", "IWOAIOAIUnet2D", "IWOAIOAIUnet2DNormalized", "AnswerMaps"]
+
+#: What a model answers besides its masks (``generate_scores``): ``top_labels`` / ``top_log_probs``, lists of uint8 / float32
+#: MedicalVolumes, the best label of every voxel first (0: background, i + 1: the model's class i) with the log probability;
+#: ``entropy`` in nats; ``log_prob`` of the labels that were given (None without)
+AnswerMaps = namedtuple("AnswerMaps", "top_labels top_log_probs entropy log_prob")
 
 
 class OAIUnet2D(HipSegModel):
@@ -95,6 +101,58 @@ class OAIUnet2D(HipSegModel):
         # any other threshold: the reference's own sequence, step by step (:140-170)
         vol_sag, v = self._to_network_input(volume)
         return self._from_network_output(self._predict_probabilities(v), vol_sag, volume.orientation)
+
+    # ---- beyond the reference, which keeps the masks only: what else the answer says -------------------------------------
+    def _single_volume(self, volume):
+        """The 3D volume the network sees of what the caller passes."""
+        return volume
+
+    def _label_planes(self, labels: MedicalVolume, vol_sag: MedicalVolume) -> np.ndarray:
+        if not isinstance(labels, MedicalVolume):
+            raise ValueError("`labels` must be a MedicalVolume")
+        lab = labels.reformat(SAGITTAL).volume
+        if lab.shape != vol_sag.volume.shape:
+            raise ValueError(f"`labels` has shape {lab.shape}, the volume {vol_sag.volume.shape} (sagittal)")
+        if lab.dtype == np.uint8:
+            return lab
+        if lab.dtype.kind not in "iub":
+            raise ValueError(f"`labels` must be integers, got {lab.dtype}")
+        if lab.size and (lab.min() < -1 or lab.max() > 255):
+            raise ValueError("`labels` must be -1 (none) .. 255")
+        return np.where(lab == -1, 255, lab).astype(np.uint8)
+
+    def generate_scores(self, volume: MedicalVolume, top: int = 1, temperature: float = 1.0, labels: MedicalVolume = None):
+        """How sure the model is, and what it would have said instead -> :data:`AnswerMaps`, in the volume's orientation.
+
+        The network's classes have sigmoid heads; under the condition that a voxel carries at most one tissue its label has the
+        distribution ``softmax([0, logits] / temperature)``, 0 being the background (``models.label_scores``).  ``top``: labels
+        wanted per voxel (at most the number of classes + 1); ``top_labels[0]`` is a label map as ``to_metrics`` takes it.
+        ``labels``: a label map to score, e.g. a manual segmentation (255 or -1: none); its log probability is ``log_prob``."""
+        top = int(top)
+        if not 1 <= top <= self._n_classes() + 1:
+            raise ValueError(f"`top` must be 1 .. {self._n_classes() + 1}, got {top}")
+        volume = self._single_volume(volume)
+        vol_sag = self._to_sagittal(volume)
+        given = None if labels is None else self._label_planes(labels, vol_sag)
+        r = self.seg_model.score_volume(vol_sag.volume, whiten=self._WHITEN, eps=self._WHITEN_EPS, temperature=temperature,
+                                        labels=given, entropy=True, top=top)
+        wrap = lambda plane: self._wrap_mask(vol_sag, plane, volume.orientation)  # noqa: E731
+        return AnswerMaps([wrap(p) for p in r["top_label"]], [wrap(p) for p in r["top_log_prob"]], wrap(r["entropy"]),
+                          wrap(r["log_prob"]) if given is not None else None)
+
+    def divergence(self, volume: MedicalVolume, answers: AnswerMaps, temperature: float = 1.0) -> MedicalVolume:
+        """Kullback-Leibler divergence (nats, per voxel) of this model's answers from those of another one, ``answers`` =
+        its ``generate_scores`` at the same ``temperature``: what a faster precision or other weights change, voxel by voxel.
+        The labels beyond the stored ones are compared as one (``models.distill_loss`` with ``tail=True``)."""
+        if not answers.top_labels or len(answers.top_labels) != len(answers.top_log_probs):
+            raise ValueError("`answers` holds no labels")
+        volume = self._single_volume(volume)
+        vol_sag = self._to_sagittal(volume)
+        labels = np.stack([self._label_planes(m, vol_sag) for m in answers.top_labels])
+        probs = np.stack([m.reformat(SAGITTAL).volume for m in answers.top_log_probs]).astype(np.float32)
+        r = self.seg_model.score_volume(vol_sag.volume, whiten=self._WHITEN, eps=self._WHITEN_EPS, temperature=temperature,
+                                        teacher=(labels, probs))
+        return self._wrap_mask(vol_sag, r["divergence"], volume.orientation)
 
     def __preprocess_volume__(self, volume: np.ndarray):
         return whiten_volume(volume, eps=1e-8)

@@ -486,6 +486,29 @@ int qmri_distill_workspace(const qmri_distill_args *args, uint64_t *bytes);
 int qmri_distill_host(const qmri_distill_args *args);
 int qmri_distill_grad_host(const qmri_distill_args *args);
 
+/* The answers of a U-Net on a whole volume in the reference's array layouts (as qmri_unet2d_segment_volume, host pointers,
+ * synchronous; one upload, one download per result): the network, then the operators above on its logits with the background as
+ * category 0 (class c is category c + 1), and the transposes on the GPU.  In label volumes 255 stands for "none". */
+typedef struct qmri_unet2d_score_args {
+    const float *vol_hws;       /* [H][W][S] */
+    int32_t S;
+    int32_t whiten;             /* as in qmri_unet2d_forward */
+    double whiten_eps;
+    double temperature;
+    const uint8_t *labels_hws;  /* nullable [H][W][S]: given labels */
+    float *log_prob_hws;        /* nullable [H][W][S]: their log probability (0 where the label is 255) */
+    float *entropy_hws;         /* nullable [H][W][S] */
+    int32_t top;                /* best labels wanted: 0 .. n_classes + 1 */
+    int32_t entries;            /* labels of the teacher: 0 .. n_classes + 1 */
+    uint8_t *top_label;         /* [top][H][W][S] */
+    float *top_log_prob;        /* [top][H][W][S] */
+    const uint8_t *teacher_label;    /* [entries][H][W][S]: top_label / top_log_prob of another network at this temperature */
+    const float *teacher_log_prob;   /* [entries][H][W][S] */
+    float *divergence_hws;      /* [H][W][S], entries > 0: qmri_distill's loss with the tail */
+    void *stream;
+} qmri_unet2d_score_args;
+int qmri_unet2d_score_volume(void *handle, const qmri_unet2d_score_args *args);
+
 /* Mean kernel time in ms of the last qmri_monoexp_fit_device call on this thread that was issued
  * with timing enabled (qmri_set_timing(1)); measured with hipEvents on the launch stream. */
 void qmri_set_timing(int enable);

@@ -23,7 +23,8 @@ def lib():
 
 
 def test_struct_layout_matches_the_c_compiler(tmp_path):
-    fields = {"qmri_logits": L.QmriLogits, "qmri_label_scores_args": L.QmriLabelScoresArgs, "qmri_distill_args": L.QmriDistillArgs}
+    fields = {"qmri_logits": L.QmriLogits, "qmri_label_scores_args": L.QmriLabelScoresArgs, "qmri_distill_args": L.QmriDistillArgs,
+              "qmri_unet2d_score_args": L.QmriUnet2dScoreArgs}
     lines, want = [], []
     for name, cls in fields.items():
         lines.append(f'printf("%zu\\n", sizeof({name}));')
