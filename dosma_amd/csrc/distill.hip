@@ -368,7 +368,53 @@ __global__ __launch_bounds__(256) void distill_grad_small_kernel(const DistillK 
 
 // ---- group: G lanes a row, 16 scores a lane ------------------------------------------------------------------------------------
 // The labels of the entries are marked in LDS, one 16-bit word for each lane's scores.  A lane holds every G-th entry: E of them
-// in registers, or (E 0) read again where they are needed.
+// in registers, or (E 0) any number in LDS.
+// More entries than registers are given to lie in LDS: those of a block's rows are one piece of memory, read side by side.  A row
+// every K | 1 words (lanes that walk through rows of their own do not meet in a bank), rows behind the last are empty.
+struct StagedEntries {
+    int *l;
+    float *v;
+    __device__ __forceinline__ void to_row(int row, int K) {
+        l += row * (K | 1);
+        v += row * (K | 1);
+    }
+    // the sum of the weights (v holds them then) of all entries with label x, in their order
+    __device__ __forceinline__ float weights_of(int x, int K) const {
+        float s = 0.f;
+        int o = 0;
+        for (; o + 4 <= K; o += 4) {
+            int i[4];
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                i[e] = l[o + e];
+                w[e] = v[o + e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += i[e] == x ? w[e] : 0.f;
+        }
+        for (; o < K; ++o) s += l[o] == x ? v[o] : 0.f;
+        return s;
+    }
+};
+inline size_t staged_bytes(int rows, int K) { return (size_t)rows * (K | 1) * 8; }
+template <int THREADS>
+__device__ __forceinline__ StagedEntries stage_entries(const DistillK &k, void *lds, long long n0, int rows, int cats) {
+    const int stride = k.K | 1, all = rows * k.K;
+    StagedEntries s = {static_cast<int *>(lds), static_cast<float *>(lds) + rows * stride};
+    const long long left = (k.g.rows - n0) * k.K;
+    __syncthreads();  // (the block's last rows have been worked on)
+    for (int i = threadIdx.x; i < all; i += THREADS) {
+        int l = -1;
+        float v = 0.f;
+        if (i < left) l = load_entry(k, n0, i, cats, v);  // (entry i from the first row on)
+        const int r = (unsigned)i / (unsigned)k.K, at = r * stride + i - r * k.K;
+        s.l[at] = l;
+        s.v[at] = v;
+    }
+    __syncthreads();
+    return s;
+}
 template <int G, int V>
 __device__ __forceinline__ void place_of(int c, int &owner, int &bit) {
     const int vec = c / V;
@@ -380,9 +426,9 @@ struct GroupEntries {
     int l[E > 0 ? E : 1];
     float v[E > 0 ? E : 1];
     const DistillK &k;
-    long long n;
-    int gl, cats;
-    __device__ __forceinline__ GroupEntries(const DistillK &k_, long long n_, int gl_, int cats_) : k(k_), n(n_), gl(gl_), cats(cats_) {
+    StagedEntries at;  // E 0: the row's
+    int gl;
+    __device__ __forceinline__ GroupEntries(const DistillK &k_, long long n, int gl_, int cats, StagedEntries at_) : k(k_), at(at_), gl(gl_) {
         if constexpr (E > 0) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -400,10 +446,33 @@ struct GroupEntries {
             for (int e = 0; e < E; ++e)
                 if (l[e] >= 0) f(l[e], v[e]);
         } else {
-            for (int q = gl; q < k.K; q += G) {
-                float x;
-                const int i = load_entry(k, n, q, cats, x);
-                if (i >= 0) f(i, x);
+            for (int q = gl; q < k.K; q += G)
+                if (at.l[q] >= 0) f(at.l[q], at.v[q]);
+        }
+    }
+    // f(label, value, score): the scores of the entries in registers, or of 4, are under way together
+    template <typename T, typename F>
+    __device__ __forceinline__ void each_score(const T *z, F f) const {
+        const int bg = k.g.bg;
+        if constexpr (E > 0) {
+            unsigned w[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = load_bits(z + (l[e] > bg ? l[e] - bg : 0));
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (l[e] >= 0) f(l[e], v[e], l[e] < bg ? 0.f : widen<T>(w[e]));
+        } else {
+            for (int q0 = gl; q0 < k.K; q0 += 4 * G) {
+                unsigned w[4];
+                int i[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    i[e] = q0 + e * G < k.K ? at.l[q0 + e * G] : -1;
+                    w[e] = load_bits(z + (i[e] > bg ? i[e] - bg : 0));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i[e] >= 0) f(i[e], at.v[q0 + e * G], i[e] < bg ? 0.f : widen<T>(w[e]));
             }
         }
     }
@@ -430,6 +499,7 @@ struct GroupEntries {
 };
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
+    extern __shared__ float s_entries[];  // E 0
     __shared__ unsigned s_bits[128];
     const LogitsK &g = k.g;
     constexpr int V = kVec<T>, NV = 16 / V, ROWS = 256 / G;
@@ -446,7 +516,12 @@ __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
             const int j = (i * G + gl) * V;
             raw[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
         }
-        const GroupEntries<G, E> entries(k, n, gl, cats);
+        StagedEntries staged = {nullptr, nullptr};
+        if constexpr (E == 0) {
+            staged = stage_entries<256>(k, s_entries, n0, ROWS, cats);
+            staged.to_row(threadIdx.x / G, k.K);
+        }
+        const GroupEntries<G, E> entries(k, n, gl, cats, staged);
         unsigned in = 0u;
         float back_in = 0.f;  // 1: the implicit category is an entry
         if (k.tail) {
@@ -485,19 +560,20 @@ __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
         }
         const Student p = student_of(M, s);
         float loss = 0.f;
-        entries.each([&](int l, float v) { loss += entry_loss(k, t, p, v, gather(g, z, l)); });
+        entries.each_score(z, [&](int, float v, float zl) { loss += entry_loss(k, t, p, v, zl); });
         loss = group_sum<G>(loss);
         const float lso = log_outside<G>(k, n, z, gl, cats, p, t, so);
         if (live && gl == 0) write_row(k, n, M, lso, p, t, loss);
     }
 }
 
+// As if none of the scores were an entry's label; those are written over by the entries' lanes, when the wave's other stores have
+// arrived.
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK k) {
-    __shared__ unsigned s_bits[128];
-    __shared__ float s_val[256 * 16];  // what an entry's lane has worked out for its label
-    __shared__ int s_l[E > 0 ? 256 * E : 1];
-    __shared__ float s_q[E > 0 ? 256 * E : 1];
+    extern __shared__ float s_entries[];  // E 0
+    __shared__ int s_l[E > 0 ? 256 / G * ((G * E) | 1) : 1];  // entry q of a row at row * (G E | 1) + q
+    __shared__ float s_q[E > 0 ? 256 / G * ((G * E) | 1) : 1];
     const LogitsK &g = k.g;
     constexpr int V = kVec<T>, NV = 16 / V, ROWS = 256 / G;
     const int gl = threadIdx.x % G, cats = g.C + g.bg, row = threadIdx.x / G;
@@ -513,52 +589,44 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
             const int j = (i * G + gl) * V;
             x[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
         }
-        const GroupEntries<G, E> entries(k, n, gl, cats);
+        StagedEntries at = {nullptr, nullptr};
+        if constexpr (E == 0) {
+            at = stage_entries<256>(k, s_entries, n0, ROWS, cats);
+            at.to_row(row, k.K);
+        }
+        const GroupEntries<G, E> entries(k, n, gl, cats, at);
         const Teacher t = entries.teacher();
         const GradRow r = grad_row(k, n, t);
-        if ((threadIdx.x & 1) == 0) s_bits[threadIdx.x >> 1] = 0u;
-        if constexpr (E > 0) {  // entry q of the row at row * G E + q
+        // what follows wants the weights of a row's entries in one place
+        if constexpr (E > 0) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                s_l[row * G * E + gl + e * G] = entries.l[e];
-                s_q[row * G * E + gl + e * G] = entries.l[e] >= 0 ? weight(t, entries.v[e]) : 0.f;
+                s_l[row * ((G * E) | 1) + gl + e * G] = entries.l[e];
+                s_q[row * ((G * E) | 1) + gl + e * G] = entries.l[e] >= 0 ? weight(t, entries.v[e]) : 0.f;
             }
+            at = {s_l + row * ((G * E) | 1), s_q + row * ((G * E) | 1)};
+        } else {
+            for (int q = gl; q < k.K; q += G) at.v[q] = at.l[q] >= 0 ? weight(t, at.v[q]) : 0.f;
         }
         wave_sync();
-        entries.each([&](int l, float) {
-            const int c = l - g.bg;
-            if (c < 0) return;
-            // the same label twice: every one of its entries sums all of them, in the order of the entries, and writes the same value
-            float qs = 0.f;
-            for (int o = 0; o < k.K; ++o) {
-                if constexpr (E > 0) {
-                    qs += s_l[row * G * E + o] == l ? s_q[row * G * E + o] : 0.f;
-                } else {
-                    float v;
-                    if (load_entry(k, n, o, cats, v) == l) qs += weight(t, v);
-                }
-            }
-            int owner, bit;
-            place_of<G, V>(c, owner, bit);
-            s_val[owner * 16 + bit] = grad_inside(r, g.c2, to_f32(z[c]), qs);
-            atomicOr(&s_bits[owner >> 1], 1u << ((owner & 1) * 16 + bit));
-        });
-        wave_sync();
-        const unsigned in = s_bits[threadIdx.x >> 1] >> ((threadIdx.x & 1) * 16) & 0xffffu;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = (i * G + gl) * V;
             float y[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) y[e] = grad_outside(r, g.c2, get(x[i], e));
-            if ((in >> (i * V)) & ((1u << V) - 1u)) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) y[e] = (in >> (i * V + e)) & 1u ? s_val[threadIdx.x * 16 + i * V + e] : y[e];
-            }
             if (!live) continue;
             if (j + V <= g.C) store_vec(out + j, pack_vec<T>(y));
             else store_part(out + j, y, g.C - j);
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        entries.each_score(z, [&](int l, float, float zl) {
+            const int c = l - g.bg;
+            if (c < 0 || !live) return;
+            // the same label twice: every one of its entries sums all of them, in the order of the entries, and writes the same value
+            const float qs = at.weights_of(l, k.K);
+            out[c] = from_f32<T>(grad_inside(r, g.c2, zl, qs));
+        });
         wave_sync();
     }
 }
@@ -782,15 +850,14 @@ __global__ __launch_bounds__(256) void distill_grad_block_kernel(const DistillK 
 }
 
 // ---- planes: one lane a row, more than 8 classes that do not lie together ------------------------------------------------------
-// K: entries in registers, as in small; 0: read again.
+// K: entries in registers, as in small; 0: any number in LDS (blocks of one wave then).
 template <int K>
 struct LaneEntries {
     int l[K > 0 ? K : 1];
     float v[K > 0 ? K : 1];
     const DistillK &k;
-    long long n;
-    int cats;
-    __device__ __forceinline__ LaneEntries(const DistillK &k_, long long n_, int cats_) : k(k_), n(n_), cats(cats_) {
+    StagedEntries at;  // K 0: the row's
+    __device__ __forceinline__ LaneEntries(const DistillK &k_, long long n, int cats, StagedEntries at_) : k(k_), at(at_) {
         if constexpr (K > 0) load_entries(k, n, cats, l, v);
     }
     // f(label, value) for every entry that counts
@@ -801,16 +868,54 @@ struct LaneEntries {
             for (int q = 0; q < K; ++q)
                 if (l[q] >= 0) f(l[q], v[q]);
         } else {
-            for (int q = 0; q < k.K; ++q) {
-                float x;
-                const int i = load_entry(k, n, q, cats, x);
-                if (i >= 0) f(i, x);
+            for (int q = 0; q < k.K; ++q)
+                if (at.l[q] >= 0) f(at.l[q], at.v[q]);
+        }
+    }
+    // f(label, value, score): the scores of up to 8 entries are under way together (an empty slot reads the first class's)
+    template <typename T, typename F>
+    __device__ __forceinline__ void each_score(const T *z, F f) const {
+        const LogitsK &g = k.g;
+        if constexpr (K > 0) {
+            unsigned w[K];
+#pragma unroll
+            for (int q = 0; q < K; ++q) w[q] = load_bits(z + (l[q] > g.bg ? l[q] - g.bg : 0) * g.sc);
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+                if (l[q] >= 0) f(l[q], v[q], l[q] < g.bg ? 0.f : widen<T>(w[q]));
+        } else {
+            for (int q0 = 0; q0 < k.K; q0 += 8) {
+                unsigned w[8];
+                int i[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    i[q] = q0 + q < k.K ? at.l[q0 + q] : -1;
+                    w[q] = load_bits(z + (i[q] > g.bg ? i[q] - g.bg : 0) * g.sc);
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (i[q] >= 0) f(i[q], at.v[q0 + q], i[q] < g.bg ? 0.f : widen<T>(w[q]));
             }
         }
     }
     __device__ __forceinline__ Teacher teacher() const {
-        if constexpr (K > 0) return teacher_lane(k, l, v);
-        else return teacher_read(k, n, cats);
+        if constexpr (K > 0) {
+            return teacher_lane(k, l, v);
+        } else {
+            float m = kNegInf, sum = 0.f, others = 0.f;
+            bool any = false, left_out = false;
+            each([&](int, float x) {
+                m = maxn(m, x);
+                any = true;
+            });
+            each([&](int, float x) {
+                const float e = teacher_term(k, x, m);
+                sum += e;
+                if (x == m && !left_out) left_out = true;
+                else others += e;
+            });
+            return teacher_of(k, any, m, sum, others);
+        }
     }
     // which of the 32 categories from c are entries
     __device__ __forceinline__ unsigned marks(int c) const {
@@ -819,16 +924,26 @@ struct LaneEntries {
         return in;
     }
 };
+template <int K>
+constexpr int kPlaneThreads = K > 0 ? 256 : 64;
 template <typename T, int K>
-__global__ __launch_bounds__(256) void distill_planes_kernel(const DistillK k) {
+__global__ __launch_bounds__(kPlaneThreads<K>) void distill_planes_kernel(const DistillK k) {
+    extern __shared__ float s_entries[];  // K 0
+    constexpr int B = kPlaneThreads<K>;
     const LogitsK &g = k.g;
     const int cats = g.C + g.bg;
-    const long long stride = (long long)gridDim.x * 256;
-    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < g.rows; n += stride) {
+    for (long long n0 = (long long)blockIdx.x * B; n0 < g.rows; n0 += (long long)gridDim.x * B) {
+        const long long n = n0 + threadIdx.x;
+        StagedEntries at = {nullptr, nullptr};
+        if constexpr (K == 0) {
+            at = stage_entries<B>(k, s_entries, n0, B, cats);
+            at.to_row(threadIdx.x, k.K);
+        }
+        if (n >= g.rows) continue;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si), *p = z;
         unsigned next[8];
         load_classes(p, g.sc, g.C, next);
-        const LaneEntries<K> entries(k, n, cats);
+        const LaneEntries<K> entries(k, n, cats, at);
         Running r = no_scores();  // (t: the sum outside the entries)
         if (g.bg) {
             const float x[1] = {0.f};
@@ -861,7 +976,7 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillK k) {
         const Student st = student_of(r.m, sum);
         const Teacher t = entries.teacher();
         float loss = 0.f;
-        entries.each([&](int l, float v) { loss += entry_loss(k, t, st, v, gather(g, z, l)); });
+        entries.each_score(z, [&](int, float v, float zl) { loss += entry_loss(k, t, st, v, zl); });
         write_row(k, n, r.m, log_outside<1>(k, n, z, 0, cats, st, t, so), st, t, loss);
     }
 }
@@ -921,22 +1036,32 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(const DistillK k) {
 // A block takes 256 rows and `len` classes of them, as if none of these were an entry's; the entries' classes are written over in
 // the end (by the lane that wrote them before, so in order).
 template <typename T, int K>
-__global__ __launch_bounds__(256) void distill_grad_planes_kernel(const DistillK k, int parts, int len) {
+__global__ __launch_bounds__(kPlaneThreads<K>) void distill_grad_planes_kernel(const DistillK k, int parts, int len) {
+    extern __shared__ float s_entries[];  // K 0
+    constexpr int B = kPlaneThreads<K>;
     const LogitsK &g = k.g;
     const int cats = g.C + g.bg;
-    const long long blocks = (g.rows + 255) / 256;
+    const long long blocks = (g.rows + B - 1) / B;
     for (long long item = blockIdx.x; item < blocks * parts; item += gridDim.x) {
         const long long rb = parts == 1 ? item : item / parts;
         const int c0 = (int)(item - rb * parts) * len, c1 = c0 + len < g.C ? c0 + len : g.C;
-        const long long n = rb * 256 + threadIdx.x;
+        const long long n = rb * B + threadIdx.x;
+        StagedEntries at = {nullptr, nullptr};
+        if constexpr (K == 0) {
+            at = stage_entries<B>(k, s_entries, rb * B, B, cats);
+            at.to_row(threadIdx.x, k.K);
+        }
         if (n >= g.rows) continue;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si), *p = z + c0 * g.sc;
         T *grad = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi), *out = grad + c0 * k.gsc;
         unsigned next[8];
         load_classes(p, g.sc, c1 - c0, next);
-        const LaneEntries<K> entries(k, n, cats);
+        const LaneEntries<K> entries(k, n, cats, at);
         const Teacher t = entries.teacher();
         const GradRow r = grad_row(k, n, t);
+        if constexpr (K == 0) {  // (weights_of)
+            for (int q = 0; q < k.K; ++q) at.v[q] = weight(t, at.v[q]);
+        }
         for (int c = c0; c < c1; c += 8) {
             float y[8];
 #pragma unroll
@@ -950,12 +1075,13 @@ __global__ __launch_bounds__(256) void distill_grad_planes_kernel(const DistillK
                 if (c + i < c1) out[i * k.gsc] = from_f32<T>(y[i]);
             out += 8 * k.gsc;
         }
-        entries.each([&](int l, float) {
+        entries.each_score(z, [&](int l, float, float zl) {
             const int c = l - g.bg;
             if (c < c0 || c >= c1) return;
             float qs = 0.f;  // (the same label twice: each time the sum of all its entries, in their order)
-            entries.each([&](int o, float v) { qs += o == l ? weight(t, v) : 0.f; });
-            grad[c * k.gsc] = from_f32<T>(grad_inside(r, g.c2, to_f32(z[c * g.sc]), qs));
+            if constexpr (K > 0) entries.each([&](int o, float v) { qs += o == l ? weight(t, v) : 0.f; });
+            else qs = at.weights_of(l, k.K);
+            grad[c * k.gsc] = from_f32<T>(grad_inside(r, g.c2, zl, qs));
         });
     }
 }
@@ -998,14 +1124,19 @@ void small_of(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
 template <typename T, int G>
 void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of((k.g.rows + 256 / G - 1) / (256 / G), num_cu, 64)), block(256);
-    // entries of a lane in registers: as many as 16 a row, or 64 where the lanes of a row are that many
+    // up to 16 entries a row in registers, or 64 where a row has that many lanes; 256 / G rows of more in LDS (G 2: at most 64 KB)
     constexpr int E = G >= 16 ? 64 / G : 16 / G > 4 ? 4 : 16 / G;
     if (k.K <= G * E) {
         if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, E>), grid, block, 0, st, k);
         else hipLaunchKernelGGL((distill_group_kernel<T, G, E>), grid, block, 0, st, k);
-    } else {
-        if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, 0>), grid, block, 0, st, k);
-        else hipLaunchKernelGGL((distill_group_kernel<T, G, 0>), grid, block, 0, st, k);
+    } else if constexpr (G < 16) {
+        const size_t lds = staged_bytes(256 / G, k.K);
+        if (lds > 48 * 1024) {
+            (void)hipFuncSetAttribute(reinterpret_cast<const void *>(distill_grad_group_kernel<T, G, 0>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            (void)hipFuncSetAttribute(reinterpret_cast<const void *>(distill_group_kernel<T, G, 0>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        }
+        if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, 0>), grid, block, lds, st, k);
+        else hipLaunchKernelGGL((distill_group_kernel<T, G, 0>), grid, block, lds, st, k);
     }
 }
 template <typename T>
@@ -1014,7 +1145,7 @@ void planes(const DistillK &k, int num_cu, hipStream_t st) {
     if (k.K <= 2) hipLaunchKernelGGL((distill_planes_kernel<T, 2>), grid, block, 0, st, k);
     else if (k.K <= 4) hipLaunchKernelGGL((distill_planes_kernel<T, 4>), grid, block, 0, st, k);
     else if (k.K <= 8) hipLaunchKernelGGL((distill_planes_kernel<T, 8>), grid, block, 0, st, k);
-    else hipLaunchKernelGGL((distill_planes_kernel<T, 0>), grid, block, 0, st, k);
+    else hipLaunchKernelGGL((distill_planes_kernel<T, 0>), dim3(grid_of((k.g.rows + 63) / 64, num_cu, 64)), dim3(64), staged_bytes(64, k.K), st, k);
 }
 template <typename T>
 void planes_grad(const DistillK &k, int num_cu, hipStream_t st) {
@@ -1024,7 +1155,8 @@ void planes_grad(const DistillK &k, int num_cu, hipStream_t st) {
     if (k.K <= 2) hipLaunchKernelGGL((distill_grad_planes_kernel<T, 2>), grid, block, 0, st, k, parts, len);
     else if (k.K <= 4) hipLaunchKernelGGL((distill_grad_planes_kernel<T, 4>), grid, block, 0, st, k, parts, len);
     else if (k.K <= 8) hipLaunchKernelGGL((distill_grad_planes_kernel<T, 8>), grid, block, 0, st, k, parts, len);
-    else hipLaunchKernelGGL((distill_grad_planes_kernel<T, 0>), grid, block, 0, st, k, parts, len);
+    else hipLaunchKernelGGL((distill_grad_planes_kernel<T, 0>), dim3(grid_of((k.g.rows + 63) / 64 * parts, num_cu, 64)), dim3(64),
+                            staged_bytes(64, k.K), st, k, parts, len);
 }
 
 template <typename T>
