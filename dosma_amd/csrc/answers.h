@@ -425,18 +425,6 @@ struct Cut {
 };
 Cut cut_rows(const LogitsK &g, int num_cu, int longest);
 
-// LDS (beyond `own` bytes) that a block asks for only to be placed: the hardware fills a compute unit with as many blocks as fit
-// before it turns to the next one, so a launch of `blocks` < num_cu * limit would leave units idle while others share their vector
-// units among `limit` blocks (1024 rows of 100003 scores: 171 of 256 units at work).  With this much LDS only as many fit as each
-// unit's even share; 64 KB a block is the most a launch may ask for as it is.
-inline size_t spread_lds(long long blocks, int num_cu, int limit, int own) {
-    const long long share = (blocks + num_cu - 1) / num_cu;
-    if (share >= limit) return 0;
-    long long bytes = 160 * 1024 / share - 1024;
-    if (bytes > 65536) bytes = 65536;
-    return bytes > own ? (size_t)(bytes - own) : 0;
-}
-
 hipError_t label_scores_launch(const ScoresK &k, int dtype, int num_cu, hipStream_t st);
 size_t label_scores_workspace_bytes(const ScoresK &k, int dtype, int num_cu);
 hipError_t label_scores_grad_launch(const ScoresK &k, int dtype, int num_cu, hipStream_t st);

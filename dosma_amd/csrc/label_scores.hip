@@ -45,9 +45,12 @@ __device__ __forceinline__ void write_row(const ScoresK &k, long long n, float M
         k.log_prob[n] = ignored ? 0.f : lp;
     }
 }
+__device__ __forceinline__ float top_value(const ScoresK &k, float v, int i, float M, float ls) {
+    return i < 0 ? (ls != ls ? ls : kNegInf) : (v - reference(M)) * k.g.invT - ls;
+}
 __device__ __forceinline__ void write_top(const ScoresK &k, long long n, int q, float v, int i, float M, float ls) {
     k.top_label[n * k.top + q] = i;
-    k.top_log_prob[n * k.top + q] = i < 0 ? (ls != ls ? ls : kNegInf) : (v - reference(M)) * k.g.invT - ls;
+    k.top_log_prob[n * k.top + q] = top_value(k, v, i, M, ls);
 }
 __device__ __forceinline__ void given_label(const ScoresK &k, long long n, int cats, int &l, bool &has, bool &ignored) {
     l = -1;
@@ -653,12 +656,19 @@ struct LaneBestKey {  // 2-byte scores, labels that fit the unused bits
     __device__ int label(int q) const { return (int)(MASK - (key[q] & MASK)); }
 };
 
+//
+// Long lists go out through LDS: 64 lanes that write each its own row ask for 64 lines a store.  A wave's rows lie one behind the
+// other, so from LDS (a row every top | 1 words) they are written as one piece.
+template <int K>
+constexpr int kPlaneThreads = K > 32 ? 64 : 256;
 template <typename T, int K, bool KEY>
-__global__ __launch_bounds__(256) void scores_planes_kernel(const ScoresK k) {
+__global__ __launch_bounds__(kPlaneThreads<K>) void scores_planes_kernel(const ScoresK k) {
+    constexpr int B = kPlaneThreads<K>;
+    extern __shared__ int s_top[];  // K > 4
     const LogitsK &g = k.g;
-    const long long stride = (long long)gridDim.x * 256;
+    const long long stride = (long long)gridDim.x * B;
     // (whole waves walk on together: the lists ask all lanes whether a score is worth entering)
-    for (long long n0 = (long long)blockIdx.x * 256 + (threadIdx.x & ~63); n0 < g.rows; n0 += stride) {
+    for (long long n0 = (long long)blockIdx.x * B + (threadIdx.x & ~63); n0 < g.rows; n0 += stride) {
         const long long nr = n0 + (threadIdx.x & 63);
         const bool live = nr < g.rows;
         const long long n = live ? nr : g.rows - 1;
@@ -698,20 +708,41 @@ __global__ __launch_bounds__(256) void scores_planes_kernel(const ScoresK k) {
             st.s = r.s * f;
             st.t = f * fmaf(d, r.s, r.t);
         }
-        if (!live) continue;
         int l;
         bool has, ignored;
         given_label(k, n, g.C + g.bg, l, has, ignored);
         const float zl = (has && l >= g.bg) ? to_f32(z[(long long)(l - g.bg) * g.sc]) : 0.f;
-        write_row(k, n, st.m, st.s, st.t, has, ignored, zl);
+        if (live) write_row(k, n, st.m, st.s, st.t, has, ignored, zl);
         if (K) {
             const float ls = __builtin_amdgcn_logf(st.s) * kLn2;
+            if (K <= 4) {
 #pragma unroll
-            for (int q = 0; q < K; ++q)
-                if (q < k.top) {
+                for (int q = 0; q < K; ++q) {
                     const float v = best.score(q);
-                    write_top(k, n, q, v, v > kNegInf ? best.label(q) : -1, st.m, ls);
+                    if (live) write_top(k, n, q, v, v > kNegInf ? best.label(q) : -1, st.m, ls);
                 }
+            } else {
+                const int lane = threadIdx.x & 63, step = k.top | 1;
+                int *s = s_top + (threadIdx.x & ~63) * step;
+                const long long left = g.rows - n0;
+                const int all = (left < 64 ? (int)left : 64) * k.top;
+                const float per = 1.f / (float)k.top;
+                auto write_all = [&](auto value, auto out) {
+#pragma unroll
+                    for (int q = 0; q < K; ++q)
+                        if (q < k.top) s[lane * step + q] = value(q);
+                    wave_sync();
+                    for (int i = lane; i < all; i += 64) {
+                        const int r = (int)((i + 0.5f) * per);  // (i < 4096: exact)
+                        out(n0 * k.top + i, s[r * step + i - r * k.top]);
+                    }
+                    wave_sync();
+                };
+                auto label = [&](int q) { return best.score(q) > kNegInf ? best.label(q) : -1; };
+                write_all(label, [&](long long at, int v) { k.top_label[at] = v; });
+                write_all([&](int q) { return __float_as_int(top_value(k, best.score(q), label(q), st.m, ls)); },
+                          [&](long long at, int v) { k.top_log_prob[at] = __int_as_float(v); });
+            }
         }
     }
 }
@@ -951,10 +982,12 @@ void group(const ScoresK &k, bool grad, int num_cu, hipStream_t st) {
 }
 template <typename T, int K>
 void planes(const ScoresK &k, int num_cu, hipStream_t st) {
-    const dim3 grid(grid_of((k.g.rows + 255) / 256, num_cu, 64)), block(256);
+    constexpr int B = kPlaneThreads<K>;
+    const dim3 grid(grid_of((k.g.rows + B - 1) / B, num_cu, 64 * (256 / B))), block(B);
+    const size_t lds = K > 4 ? (size_t)B * (k.top | 1) * 4 : 0;
     // (the last eight classes may reach 7 labels beyond the last)
-    if (sizeof(T) == 2 && k.g.C + k.g.bg + 7 <= (1 << kLabelBits<T>)) hipLaunchKernelGGL((scores_planes_kernel<T, K, sizeof(T) == 2>), grid, block, 0, st, k);
-    else hipLaunchKernelGGL((scores_planes_kernel<T, K, false>), grid, block, 0, st, k);
+    if (sizeof(T) == 2 && k.g.C + k.g.bg + 7 <= (1 << kLabelBits<T>)) hipLaunchKernelGGL((scores_planes_kernel<T, K, sizeof(T) == 2>), grid, block, lds, st, k);
+    else hipLaunchKernelGGL((scores_planes_kernel<T, K, false>), grid, block, lds, st, k);
 }
 
 template <typename T>
@@ -1002,8 +1035,7 @@ void launch(const ScoresK &k, int num_cu, hipStream_t st) {
         if (k.top) hipLaunchKernelGGL((scores_block_kernel<T, true, 1>), grid, dim3(64), 0, st, k, cut);
         else hipLaunchKernelGGL((scores_block_kernel<T, false, 1>), grid, dim3(64), 0, st, k, cut);
     } else if (k.top) {
-        const size_t pad = spread_lds(g.rows * cut.segs, num_cu, 5, 4 * (kBuf * 8 + 64 * 4 + (int)sizeof(RowStat)));
-        hipLaunchKernelGGL((scores_block_kernel<T, true, 4>), grid, dim3(256), pad, st, k, cut);
+        hipLaunchKernelGGL((scores_block_kernel<T, true, 4>), grid, dim3(256), 0, st, k, cut);
     } else if (cut.len >= 16384) {
         hipLaunchKernelGGL((scores_block_kernel<T, false, 8>), grid, dim3(512), 0, st, k, cut);
     } else {
