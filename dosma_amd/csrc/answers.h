@@ -126,19 +126,35 @@ __device__ __forceinline__ Vec<T> load_vec(const T *p) {
     __builtin_memcpy(&r, p, 16);
     return r;
 }
-// the first n scores of a vector that ends behind its row, the rest -inf
+// the vector without its first n scores, -inf behind the others
+template <typename T>
+__device__ __forceinline__ Vec<T> drop_front(Vec<T> r, int n) {
+    constexpr unsigned fill = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, bf16_t> ? 0xff80ff80u : 0xfc00fc00u;
+    int words = n;
+    if constexpr (sizeof(T) == 2) {
+        words = n >> 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = n & 1 ? __builtin_amdgcn_alignbit(i < 3 ? r.w[i < 3 ? i + 1 : 3] : fill, r.w[i], 16) : r.w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = words & 1 ? (i < 3 ? r.w[i < 3 ? i + 1 : 3] : fill) : r.w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = words & 2 ? (i < 2 ? r.w[i < 2 ? i + 2 : 3] : fill) : r.w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = words >= 4 ? fill : r.w[i];
+    return r;
+}
+// The vector at p of a row with n scores (any number, also none) from there on, -inf behind: where it would end behind the row, the
+// row's last vector without what lies before p.  (One load for all lanes: the scores one by one in a branch cost a third of the
+// time of rows that end inside a vector.)  The row has at least kVec<T> scores.
+template <typename T>
+__device__ __forceinline__ int vec_back(int n) {  // by how many scores the load is moved to the front
+    return n < kVec<T> ? kVec<T> - n : 0;
+}
 template <typename T>
 __device__ __forceinline__ Vec<T> load_part(const T *p, int n) {
-    Vec<T> r;
-    unsigned b[kVec<T>];
-#pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) b[i] = bits_of(i < n ? p[i] : static_cast<T>(kNegInf));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) r.w[i] = b[i];
-        else r.w[i] = b[2 * i] | (b[2 * i + 1] << 16);
-    }
-    return r;
+    const int back = vec_back<T>(n);
+    return drop_front(load_vec(p - back), back < kVec<T> ? back : kVec<T>);
 }
 // values rounded to T
 template <typename T>
@@ -184,7 +200,7 @@ __device__ __forceinline__ Tile<T> load_tile(const T *p, int n) {
 #pragma unroll
         for (int u = 0; u < 16 / V; ++u) {
             const int j = u * 64 * V + lane * V;
-            r.v[u] = j + V <= n ? load_vec(p + j) : load_part(p + j, n - j);
+            r.v[u] = load_part(p + j, n - j);
         }
     }
     return r;

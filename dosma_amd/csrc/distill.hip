@@ -514,7 +514,7 @@ __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = (i * G + gl) * V;
-            raw[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
+            raw[i] = load_vec(z + j - vec_back<T>(g.C - j));
         }
         StagedEntries staged = {nullptr, nullptr};
         if constexpr (E == 0) {
@@ -544,7 +544,13 @@ __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
         const Teacher t = entries.teacher();
         float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = get(raw[i / V], i % V);
+        for (int i = 0; i < NV; ++i) {
+            const int back = vec_back<T>(g.C - (i * G + gl) * V);
+            // (with more than 8 G scores in a row the first half of the vectors is whole)
+            const Vec<T> v = G > 2 && 2 * i < NV ? raw[i] : drop_front(raw[i], back < V ? back : V);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[i * V + e] = get(v, e);
+        }
         const float xb = (g.bg && gl == 0) ? 0.f : kNegInf;
         const float M = group_max<G>(maxn(max_of(x), xb)), ref = reference(M);
         float e[16];
@@ -587,7 +593,7 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = (i * G + gl) * V;
-            x[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
+            x[i] = load_vec(z + j - vec_back<T>(g.C - j));
         }
         StagedEntries at = {nullptr, nullptr};
         if constexpr (E == 0) {
@@ -611,13 +617,12 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
         wave_sync();
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            // (a vector moved to the front: scores that another lane has too get the same value from both)
             const int j = (i * G + gl) * V;
             float y[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) y[e] = grad_outside(r, g.c2, get(x[i], e));
-            if (!live) continue;
-            if (j + V <= g.C) store_vec(out + j, pack_vec<T>(y));
-            else store_part(out + j, y, g.C - j);
+            if (live && j < g.C) store_vec(out + j - vec_back<T>(g.C - j), pack_vec<T>(y));
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         entries.each_score(z, [&](int l, float, float zl) {

@@ -150,7 +150,8 @@ __global__ __launch_bounds__(256) void scores_group_kernel(const ScoresK k) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = (i * G + gl) * V;
-            const Vec<T> r = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
+            // (with more than 8 G scores in a row the first half of the vectors is whole)
+            const Vec<T> r = G > 2 && 2 * i < NV ? load_vec(z + j) : load_part(z + j, g.C - j);
 #pragma unroll
             for (int e = 0; e < V; ++e) x[i * V + e] = get(r, e);
         }
@@ -873,17 +874,17 @@ __global__ __launch_bounds__(256) void scores_grad_group_kernel(const ScoresK k)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = (i * G + gl) * V;
-            x[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
+            x[i] = load_vec(z + j - vec_back<T>(g.C - j));
         }
         const GradRow r = grad_row(k, n, g.C + g.bg);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int j = (i * G + gl) * V;
+            // (the vector moved to the front: scores that another lane has too get the same value from both)
+            const int j = (i * G + gl) * V, at = j - vec_back<T>(g.C - j);
             float y[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = grad_score(r, g.c2, g.invT, get(x[i], e), j + e + g.bg);
-            if (j + V <= g.C) store_vec(out + j, pack_vec<T>(y));
-            else store_part(out + j, y, g.C - j);
+            for (int e = 0; e < V; ++e) y[e] = grad_score(r, g.c2, g.invT, get(x[i], e), at + e + g.bg);
+            if (j < g.C) store_vec(out + at, pack_vec<T>(y));
         }
     }
 }
@@ -902,7 +903,7 @@ __global__ __launch_bounds__(256) void scores_grad_block_kernel(const ScoresK k,
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int j = c0 + (i * 256 + threadIdx.x) * V;
-            x[i] = j + V <= g.C ? load_vec(z + j) : load_part(z + j, g.C - j);
+            x[i] = load_part(z + j, g.C - j);
         }
         const GradRow r = grad_row(k, n, g.C + g.bg);
 #pragma unroll
