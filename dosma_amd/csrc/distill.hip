@@ -181,6 +181,11 @@ __device__ __forceinline__ Teacher teacher_read(const DistillK &k, long long n, 
     return teacher_of(k, any, m, sum, others);
 }
 
+// v, or 0 where bit i of `marks` is set (two instructions: a sign extended from the bit, and a mask)
+__device__ __forceinline__ float unless(float v, unsigned marks, int i) {
+    return __int_as_float(__float_as_int(v) & __builtin_amdgcn_sbfe((int)~marks, i, 1));
+}
+
 // ---- results of a row -----------------------------------------------------------------------------------------------------------
 // s: of all categories, so: of those outside the entries, both relative to reference(M)
 struct Student {
@@ -285,7 +290,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillK k) {
             }
         }
 #pragma unroll
-        for (int j = 0; j <= N; ++j) so += (in >> j) & 1u ? 0.f : e[j];
+        for (int j = 0; j <= N; ++j) so += unless(e[j], in, j);
         write_row(k, n, M, log_outside<1>(k, n, z, 0, cats, p, t, so), p, t, loss);
     }
 }
@@ -367,8 +372,9 @@ __global__ __launch_bounds__(256) void distill_grad_small_kernel(const DistillK 
 }
 
 // ---- group: G lanes a row, 16 scores a lane ------------------------------------------------------------------------------------
-// The labels of the entries are marked in LDS, one 16-bit word for each lane's scores.  A lane holds every G-th entry: E of them
-// in registers, or (E 0) any number in LDS.
+// E > 0: a lane holds E entries in registers, every G-th of the row; the labels are marked in LDS, a 16-bit word for each lane's
+// scores.  E 0: the same with any number of entries, in LDS.  E < 0: up to -E entries, all of them in every lane -- the exponents
+// and logarithms of a few entries, worked out by all lanes alike, are less than the exchanges between them.
 // More entries than registers are given to lie in LDS: those of a block's rows are one piece of memory, read side by side.  A row
 // every K | 1 words (lanes that walk through rows of their own do not meet in a bank), rows behind the last are empty.
 struct StagedEntries {
@@ -450,6 +456,27 @@ struct GroupEntries {
                 if (at.l[q] >= 0) f(at.l[q], at.v[q]);
         }
     }
+    // which of the lane's scores are entries' (bits: LDS), and whether the implicit category is one
+    template <int V>
+    __device__ __forceinline__ unsigned marks(unsigned *bits, bool &back) const {
+        float b = 0.f;
+        if ((threadIdx.x & 1) == 0) bits[threadIdx.x >> 1] = 0u;
+        wave_sync();
+        each([&](int i, float) {
+            if (i < k.g.bg) {
+                b = 1.f;
+            } else {
+                int owner, bit;
+                place_of<G, V>(i - k.g.bg, owner, bit);
+                atomicOr(&bits[owner >> 1], 1u << ((owner & 1) * 16 + bit));
+            }
+        });
+        wave_sync();
+        const unsigned in = bits[threadIdx.x >> 1] >> ((threadIdx.x & 1) * 16) & 0xffffu;
+        wave_sync();
+        back = group_max<G>(b) > 0.f;
+        return in;
+    }
     // f(label, value, score): the scores of the entries in registers, or of 4, are under way together
     template <typename T, typename F>
     __device__ __forceinline__ void each_score(const T *z, F f) const {
@@ -496,7 +523,43 @@ struct GroupEntries {
         if (left_out && one != gl) others += teacher_term(k, m, m);
         return teacher_of(k, any, m, group_sum<G>(sum), group_sum<G>(others));
     }
+    __device__ __forceinline__ float total(float part) const { return group_sum<G>(part); }  // of what each gave
 };
+template <int G, int K>
+struct AllEntries {
+    int l[K];
+    float v[K];
+    const DistillK &k;
+    __device__ __forceinline__ AllEntries(const DistillK &k_, long long n, int, int cats, StagedEntries) : k(k_) { load_entries(k, n, cats, l, v); }
+    template <int V>
+    __device__ __forceinline__ unsigned marks(unsigned *, bool &back) const {
+        unsigned in = 0u;
+        back = false;
+#pragma unroll
+        for (int q = 0; q < K; ++q) {
+            int owner, bit;
+            place_of<G, V>(l[q] - k.g.bg, owner, bit);
+            const bool there = l[q] >= k.g.bg;
+            back |= l[q] == 0 && !there;
+            in |= there && owner == (int)threadIdx.x ? 1u << bit : 0u;
+        }
+        return in;
+    }
+    template <typename T, typename F>
+    __device__ __forceinline__ void each_score(const T *z, F f) const {
+        const int bg = k.g.bg;
+        unsigned w[K];
+#pragma unroll
+        for (int q = 0; q < K; ++q) w[q] = load_bits(z + (l[q] > bg ? l[q] - bg : 0));
+#pragma unroll
+        for (int q = 0; q < K; ++q)
+            if (l[q] >= 0) f(l[q], v[q], l[q] < bg ? 0.f : widen<T>(w[q]));
+    }
+    __device__ __forceinline__ Teacher teacher() const { return teacher_lane(k, l, v); }
+    __device__ __forceinline__ float total(float part) const { return part; }
+};
+template <int G, int E>
+using EntriesOf = std::conditional_t<(E < 0), AllEntries<G, E < 0 ? -E : 1>, GroupEntries<G, E < 0 ? 1 : E>>;
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
     extern __shared__ float s_entries[];  // E 0
@@ -521,26 +584,10 @@ __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
             staged = stage_entries<256>(k, s_entries, n0, ROWS, cats);
             staged.to_row(threadIdx.x / G, k.K);
         }
-        const GroupEntries<G, E> entries(k, n, gl, cats, staged);
+        const EntriesOf<G, E> entries(k, n, gl, cats, staged);
         unsigned in = 0u;
-        float back_in = 0.f;  // 1: the implicit category is an entry
-        if (k.tail) {
-            if ((threadIdx.x & 1) == 0) s_bits[threadIdx.x >> 1] = 0u;
-            wave_sync();
-            entries.each([&](int l, float) {
-                if (l < g.bg) {
-                    back_in = 1.f;
-                } else {
-                    int owner, bit;
-                    place_of<G, V>(l - g.bg, owner, bit);
-                    atomicOr(&s_bits[owner >> 1], 1u << ((owner & 1) * 16 + bit));
-                }
-            });
-            wave_sync();
-            in = s_bits[threadIdx.x >> 1] >> ((threadIdx.x & 1) * 16) & 0xffffu;
-            wave_sync();
-            back_in = group_max<G>(back_in);
-        }
+        bool back_in = false;  // the implicit category is an entry
+        if (k.tail) in = entries.template marks<V>(s_bits, back_in);
         const Teacher t = entries.teacher();
         float x[16];
 #pragma unroll
@@ -561,13 +608,13 @@ __global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
         float so = 0.f;
         if (k.tail) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) e[i] = (in >> i) & 1u ? 0.f : e[i];
-            so = group_sum<G>(tree_sum(e) + (back_in > 0.f ? 0.f : eb));
+            for (int i = 0; i < 16; ++i) e[i] = unless(e[i], in, i);
+            so = group_sum<G>(tree_sum(e) + (back_in ? 0.f : eb));
         }
         const Student p = student_of(M, s);
         float loss = 0.f;
         entries.each_score(z, [&](int, float v, float zl) { loss += entry_loss(k, t, p, v, zl); });
-        loss = group_sum<G>(loss);
+        loss = entries.total(loss);
         const float lso = log_outside<G>(k, n, z, gl, cats, p, t, so);
         if (live && gl == 0) write_row(k, n, M, lso, p, t, loss);
     }
@@ -600,7 +647,7 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
             at = stage_entries<256>(k, s_entries, n0, ROWS, cats);
             at.to_row(row, k.K);
         }
-        const GroupEntries<G, E> entries(k, n, gl, cats, at);
+        const EntriesOf<G, E> entries(k, n, gl, cats, at);
         const Teacher t = entries.teacher();
         const GradRow r = grad_row(k, n, t);
         // what follows wants the weights of a row's entries in one place
@@ -611,7 +658,7 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
                 s_q[row * ((G * E) | 1) + gl + e * G] = entries.l[e] >= 0 ? weight(t, entries.v[e]) : 0.f;
             }
             at = {s_l + row * ((G * E) | 1), s_q + row * ((G * E) | 1)};
-        } else {
+        } else if constexpr (E == 0) {
             for (int q = gl; q < k.K; q += G) at.v[q] = at.l[q] >= 0 ? weight(t, at.v[q]) : 0.f;
         }
         wave_sync();
@@ -625,13 +672,25 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
             if (live && j < g.C) store_vec(out + j - vec_back<T>(g.C - j), pack_vec<T>(y));
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        entries.each_score(z, [&](int l, float, float zl) {
-            const int c = l - g.bg;
-            if (c < 0 || !live) return;
-            // the same label twice: every one of its entries sums all of them, in the order of the entries, and writes the same value
-            const float qs = at.weights_of(l, k.K);
-            out[c] = from_f32<T>(grad_inside(r, g.c2, zl, qs));
-        });
+        // the same label twice: every one of its entries sums all of them, in the order of the entries, and writes the same value
+        if constexpr (E < 0) {
+            float w[-E];
+#pragma unroll
+            for (int q = 0; q < -E; ++q) w[q] = entries.l[q] >= 0 ? weight(t, entries.v[q]) : 0.f;
+            entries.each_score(z, [&](int l, float, float zl) {
+                const int c = l - g.bg;
+                float qs = 0.f;
+#pragma unroll
+                for (int q = 0; q < -E; ++q) qs += entries.l[q] == l ? w[q] : 0.f;
+                if (c >= 0 && live && gl == (c & (G - 1))) out[c] = from_f32<T>(grad_inside(r, g.c2, zl, qs));
+            });
+        } else {
+            entries.each_score(z, [&](int l, float, float zl) {
+                const int c = l - g.bg;
+                if (c < 0 || !live) return;
+                out[c] = from_f32<T>(grad_inside(r, g.c2, zl, at.weights_of(l, k.K)));
+            });
+        }
         wave_sync();
     }
 }
@@ -666,7 +725,7 @@ __device__ __forceinline__ void add_outside(Running &r, const float (&x)[N], flo
     r.s += s;
     if (in) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) e[i] = (in >> i) & 1u ? 0.f : e[i];
+        for (int i = 0; i < N; ++i) e[i] = unless(e[i], in, i);
         r.t += tree_sum(e);
     } else {
         r.t += s;
@@ -1131,6 +1190,20 @@ void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of((k.g.rows + 256 / G - 1) / (256 / G), num_cu, 64)), block(256);
     // up to 16 entries a row in registers, or 64 where a row has that many lanes; 256 / G rows of more in LDS (G 2: at most 64 KB)
     constexpr int E = G >= 16 ? 64 / G : 16 / G > 4 ? 4 : 16 / G;
+    // One or two entries: all of them in every lane (1000 classes: 74 us instead of 83); with more it pays only where two lanes share a
+    // row (20 classes, three entries: 135 and 149 us; 500 classes: 85 and 81)
+    if (k.K <= 2) {
+        if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, -2>), grid, block, 0, st, k);
+        else hipLaunchKernelGGL((distill_group_kernel<T, G, -2>), grid, block, 0, st, k);
+        return;
+    }
+    if constexpr (G == 2) {
+        if (k.K <= 4) {
+            if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, -4>), grid, block, 0, st, k);
+            else hipLaunchKernelGGL((distill_group_kernel<T, G, -4>), grid, block, 0, st, k);
+            return;
+        }
+    }
     if (k.K <= G * E) {
         if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, E>), grid, block, 0, st, k);
         else hipLaunchKernelGGL((distill_group_kernel<T, G, E>), grid, block, 0, st, k);
@@ -1186,7 +1259,10 @@ void launch(const DistillK &k, int num_cu, hipStream_t st) {
     const Cut cut = cut_rows(g, num_cu, k.tail ? kLongest : 1 << 30);
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
     const unsigned marks = (unsigned)(cut.len + 31) / 32 * 4;
-    if (cut.len >= 16384) {  // (as in label_scores.hip)
+    if (g.C <= 16384 && g.rows >= 16ll * num_cu) {  // (as in label_scores.hip)
+        if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true, 1>), grid, dim3(64), marks, st, k, cut);
+        else hipLaunchKernelGGL((distill_block_kernel<T, false, 1>), grid, dim3(64), 0, st, k, cut);
+    } else if (cut.len >= 16384) {
         if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true, 8>), grid, dim3(512), marks, st, k, cut);
         else hipLaunchKernelGGL((distill_block_kernel<T, false, 8>), grid, dim3(512), 0, st, k, cut);
     } else {
