@@ -561,7 +561,7 @@ struct AllEntries {
 template <int G, int E>
 using EntriesOf = std::conditional_t<(E < 0), AllEntries<G, E < 0 ? -E : 1>, GroupEntries<G, E < 0 ? 1 : E>>;
 template <typename T, int G, int E>
-__global__ __launch_bounds__(256) void distill_group_kernel(const DistillK k) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 || E == 0 ? 6 : 8) void distill_group_kernel(const DistillK k) {
     extern __shared__ float s_entries[];  // E 0
     __shared__ unsigned s_bits[128];
     const LogitsK &g = k.g;
@@ -846,11 +846,11 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillK k, cons
     }
 }
 
-// A block takes a segment of a row, 256 lanes x 16 scores at a time, as if none of them were an entry's label; those few are
+// W waves take a segment of a row, 16 scores a lane at a time, as if none of them were an entry's label; those few are
 // written over at the end, when the block's other stores have arrived.
-template <typename T>
-__global__ __launch_bounds__(256) void distill_grad_block_kernel(const DistillK k, const Cut cut) {
-    constexpr int V = kVec<T>, NV = 16 / V, TILE = 256 * 16;
+template <typename T, int W>
+__global__ __launch_bounds__(64 * W) void distill_grad_block_kernel(const DistillK k, const Cut cut) {
+    constexpr int V = kVec<T>, NV = 16 / V, TILE = 1024 * W;
     __shared__ GradRow s_row;
     const LogitsK &g = k.g;
     for (long long item = blockIdx.x; item < g.rows * cut.segs; item += gridDim.x) {
@@ -862,8 +862,8 @@ __global__ __launch_bounds__(256) void distill_grad_block_kernel(const DistillK 
         auto fetch = [&](int c) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int j = c + (i * 256 + threadIdx.x) * V;
-                nx[i] = j + V <= c1 ? load_vec(z + j) : load_part(z + j, c1 - j);
+                const int j = c + (i * 64 * W + (int)threadIdx.x) * V;
+                nx[i] = load_vec(z + j - vec_back<T>(g.C - j));  // (lanes behind the row: its last vector)
             }
         };
         fetch(c0);
@@ -898,13 +898,14 @@ __global__ __launch_bounds__(256) void distill_grad_block_kernel(const DistillK 
             if (c + TILE < c1) fetch(c + TILE);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int j = c + (i * 256 + threadIdx.x) * V;
+                const int j = c + (i * 64 * W + (int)threadIdx.x) * V, back = vec_back<T>(g.C - j);
                 if (j >= c1) continue;
                 float y[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) y[e] = grad_outside(r, g.c2, get(now[i], e));
-                if (j + V <= c1) store_vec(out + j, pack_vec<T>(y));
-                else store_part(out + j, y, c1 - j);
+                // (the row's last vector, moved to the front: what lies before j is another lane's)
+                if (back == 0) store_vec(out + j, pack_vec<T>(y));
+                else store_end(out + j - back, y, back);
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1259,7 +1260,7 @@ void launch(const DistillK &k, int num_cu, hipStream_t st) {
     const Cut cut = cut_rows(g, num_cu, k.tail ? kLongest : 1 << 30);
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
     const unsigned marks = (unsigned)(cut.len + 31) / 32 * 4;
-    if (g.C <= 16384 && g.rows >= 16ll * num_cu) {  // (as in label_scores.hip)
+    if (wave_rows(g, num_cu)) {
         if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true, 1>), grid, dim3(64), marks, st, k, cut);
         else hipLaunchKernelGGL((distill_block_kernel<T, false, 1>), grid, dim3(64), 0, st, k, cut);
     } else if (cut.len >= 16384) {
@@ -1286,14 +1287,16 @@ void launch_grad(const DistillK &k, int num_cu, hipStream_t st) {
     if (g.C <= 256) return group<T, 16>(k, true, num_cu, st);
     if (g.C <= 512) return group<T, 32>(k, true, num_cu, st);
     if (g.C <= 1024) return group<T, 64>(k, true, num_cu, st);
-    // a row's setup (its teacher) is worth several tiles; eight blocks on every compute unit hide it
+    // a row's setup (its teacher) is worth several rounds of loads; eight blocks on every compute unit hide it
     const long long most = (g.C + 4095) / 4096;
     long long want = (8ll * num_cu + g.rows - 1) / g.rows;
     if (want > most) want = most;
     Cut cut;
     cut.len = (int)(((g.C + want - 1) / want + 4095) / 4096 * 4096);
     cut.segs = (g.C + cut.len - 1) / cut.len;
-    hipLaunchKernelGGL(distill_grad_block_kernel<T>, dim3(grid_of(g.rows * cut.segs, num_cu, 64)), dim3(256), 0, st, k, cut);
+    const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
+    if (wave_rows_grad<T>(g, num_cu)) hipLaunchKernelGGL((distill_grad_block_kernel<T, 1>), grid, dim3(64), 0, st, k, cut);
+    else hipLaunchKernelGGL((distill_grad_block_kernel<T, 4>), grid, dim3(256), 0, st, k, cut);
 }
 
 }  // namespace

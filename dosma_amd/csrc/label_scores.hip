@@ -25,7 +25,6 @@ Cut cut_rows(const LogitsK &g, int num_cu, int longest) {
     c.segs = (g.C + c.len - 1) / c.len;
     return c;
 }
-
 namespace {
 
 // ---- results of a row -------------------------------------------------------------------------------------------------------
@@ -135,8 +134,9 @@ __global__ __launch_bounds__(256) void scores_small_kernel(const ScoresK k) {
 }
 
 // ---- group: G lanes a row, 16 scores a lane -----------------------------------------------------------------------------------
-template <typename T, int G>
-__global__ __launch_bounds__(256) void scores_group_kernel(const ScoresK k) {
+// Without the best: 64 registers, eight waves a SIMD (500 classes in bf16, 200000 rows: 51 us instead of 55 with the code of both).
+template <typename T, int G, bool TOP>
+__global__ __launch_bounds__(256, TOP ? 4 : 8) void scores_group_kernel(const ScoresK k) {
     const LogitsK &g = k.g;
     constexpr int V = kVec<T>, NV = 16 / V, ROWS = 256 / G;
     const int gl = threadIdx.x % G, cats = g.C + g.bg;
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void scores_group_kernel(const ScoresK k) {
         const float db = clamp2((x[16] - ref) * g.c2), eb = exp2_hw(db);
         const float s = group_sum<G>(tree_sum(e) + eb), t = group_sum<G>(tree_sum(et) + eb * db);
         if (live && gl == 0) write_row(k, n, M, s, t, has, ignored, zl);
-        if (k.top == 0) continue;
+        if (!TOP) continue;
         const float ls = __builtin_amdgcn_logf(s) * kLn2;
         auto label_of = [&](int i) { return ((i / V) * G + gl) * V + i % V + g.bg; };
         if constexpr (sizeof(T) == 2) {
@@ -889,31 +889,42 @@ __global__ __launch_bounds__(256) void scores_grad_group_kernel(const ScoresK k)
     }
 }
 
-// A block takes 256 lanes x 16 scores of a row at a time.
-template <typename T>
-__global__ __launch_bounds__(256) void scores_grad_block_kernel(const ScoresK k, long long tiles) {
+// W waves a segment of a row, 16 scores a lane at a time and the next 16 in flight.
+template <typename T, int W>
+__global__ __launch_bounds__(64 * W) void scores_grad_block_kernel(const ScoresK k, const Cut cut) {
     const LogitsK &g = k.g;
-    constexpr int V = kVec<T>, NV = 16 / V, TILE = 256 * 16;
-    for (long long item = blockIdx.x; item < g.rows * tiles; item += gridDim.x) {
-        const long long n = item / tiles;
-        const int c0 = (int)(item - n * tiles) * TILE;
+    constexpr int V = kVec<T>, NV = 16 / V, TILE = 1024 * W;
+    for (long long item = blockIdx.x; item < g.rows * cut.segs; item += gridDim.x) {
+        const long long n = cut.segs == 1 ? item : item / cut.segs;
+        const int c0 = (int)(item - n * cut.segs) * cut.len, c1 = c0 + cut.len < g.C ? c0 + cut.len : g.C;
         const T *z = static_cast<const T *>(g.z) + row_base(g, n, g.so, g.si);
         T *out = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi);
-        Vec<T> x[NV];
+        Vec<T> nx[NV];
+        auto fetch = [&](int c) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = c0 + (i * 256 + threadIdx.x) * V;
-            x[i] = load_part(z + j, g.C - j);
-        }
+            for (int i = 0; i < NV; ++i) {
+                const int j = c + (i * 64 * W + (int)threadIdx.x) * V;
+                nx[i] = load_vec(z + j - vec_back<T>(g.C - j));  // (lanes behind the row: its last vector)
+            }
+        };
+        fetch(c0);
         const GradRow r = grad_row(k, n, g.C + g.bg);
+        for (int c = c0; c < c1; c += TILE) {
+            Vec<T> now[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = c0 + (i * 256 + threadIdx.x) * V;
-            float y[V];
+            for (int i = 0; i < NV; ++i) now[i] = nx[i];
+            if (c + TILE < c1) fetch(c + TILE);
 #pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = grad_score(r, g.c2, g.invT, get(x[i], e), j + e + g.bg);
-            if (j + V <= g.C) store_vec(out + j, pack_vec<T>(y));
-            else store_part(out + j, y, g.C - j);
+            for (int i = 0; i < NV; ++i) {
+                const int j = c + (i * 64 * W + (int)threadIdx.x) * V, back = vec_back<T>(g.C - j);
+                if (j >= c1) continue;
+                float y[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = grad_score(r, g.c2, g.invT, get(now[i], e), j - back + e + g.bg);
+                // (the row's last vector, moved to the front: what lies before j is another lane's)
+                if (back == 0) store_vec(out + j, pack_vec<T>(y));
+                else store_end(out + j - back, y, back);
+            }
         }
     }
 }
@@ -979,7 +990,8 @@ template <typename T, int G>
 void group(const ScoresK &k, bool grad, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of((k.g.rows + 256 / G - 1) / (256 / G), num_cu, 64)), block(256);
     if (grad) hipLaunchKernelGGL((scores_grad_group_kernel<T, G>), grid, block, 0, st, k);
-    else hipLaunchKernelGGL((scores_group_kernel<T, G>), grid, block, 0, st, k);
+    else if (k.top) hipLaunchKernelGGL((scores_group_kernel<T, G, true>), grid, block, 0, st, k);
+    else hipLaunchKernelGGL((scores_group_kernel<T, G, false>), grid, block, 0, st, k);
 }
 template <typename T, int K>
 void planes(const ScoresK &k, int num_cu, hipStream_t st) {
@@ -1032,7 +1044,7 @@ void launch(const ScoresK &k, int num_cu, hipStream_t st) {
     if (g.C <= 1024) return group<T, 64>(k, false, num_cu, st);
     const Cut cut = cut_rows(g, num_cu, 1 << 30);
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
-    if (g.C <= 16384 && g.rows >= 16ll * num_cu) {
+    if (wave_rows(g, num_cu)) {
         if (k.top) hipLaunchKernelGGL((scores_block_kernel<T, true, 1>), grid, dim3(64), 0, st, k, cut);
         else hipLaunchKernelGGL((scores_block_kernel<T, false, 1>), grid, dim3(64), 0, st, k, cut);
     } else if (k.top) {
@@ -1073,8 +1085,12 @@ void launch_grad(const ScoresK &k, int num_cu, hipStream_t st) {
     if (g.C <= 256) return group<T, 16>(k, true, num_cu, st);
     if (g.C <= 512) return group<T, 32>(k, true, num_cu, st);
     if (g.C <= 1024) return group<T, 64>(k, true, num_cu, st);
-    const long long tiles = (g.C + 4095) / 4096;
-    hipLaunchKernelGGL(scores_grad_block_kernel<T>, dim3(grid_of(g.rows * tiles, num_cu, 256)), dim3(256), 0, st, k, tiles);
+    // a block a piece of 4096 scores, one round of its loads (4-byte scores: 8192 x 16384 in 190 us, by blocks that go on to the next
+    // pieces 228); a wave a row where that leaves lanes without scores (50000 x 1999 in bf16: 92 us, in pieces 146)
+    const bool wave = wave_rows_grad<T>(g, num_cu);
+    const Cut cut = {wave ? 1 : (g.C + 4095) / 4096, wave ? g.C : 4096};
+    if (wave) hipLaunchKernelGGL((scores_grad_block_kernel<T, 1>), dim3(grid_of(g.rows, num_cu, 64)), dim3(64), 0, st, k, cut);
+    else hipLaunchKernelGGL((scores_grad_block_kernel<T, 4>), dim3(grid_of(g.rows * cut.segs, num_cu, 256)), dim3(256), 0, st, k, cut);
 }
 
 }  // namespace
