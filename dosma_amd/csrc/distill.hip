@@ -317,6 +317,12 @@ __device__ __forceinline__ float grad_outside(const GradRow &r, float c2, float 
     const float o = v == kNegInf ? 0.f : exp2_hw(d + r.share);  // (the share of a row with nothing outside is infinite)
     return r.zero ? 0.f : r.f * fmaf(r.total, p, -o);
 }
+// q: the sum of the weights of the score's entries, negative where it has none
+__device__ __forceinline__ float grad_either(const GradRow &r, float c2, float v, float q) {
+    const float d = (v - r.M) * c2 - r.l2s, p = exp2_hw(d);
+    const float o = v == kNegInf ? 0.f : exp2_hw(d + r.share);
+    return r.zero ? 0.f : r.f * fmaf(r.total, p, -(q < 0.f ? o : q));
+}
 __device__ __forceinline__ float grad_inside(const GradRow &r, float c2, float v, float qs) {
     const float p = exp2_hw((v - r.M) * c2 - r.l2s);
     return r.zero ? 0.f : r.f * fmaf(r.total, p, -qs);
@@ -388,36 +394,55 @@ struct StagedEntries {
     __device__ __forceinline__ float weights_of(int x, int K) const {
         float s = 0.f;
         int o = 0;
-        for (; o + 4 <= K; o += 4) {
-            int i[4];
-            float w[4];
+        for (; o + 8 <= K; o += 8) {
+            int i[8];
+            float w[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 8; ++e) {
                 i[e] = l[o + e];
                 w[e] = v[o + e];
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s += i[e] == x ? w[e] : 0.f;
+            for (int e = 0; e < 8; ++e) s += i[e] == x ? w[e] : 0.f;
         }
         for (; o < K; ++o) s += l[o] == x ? v[o] : 0.f;
         return s;
     }
 };
 inline size_t staged_bytes(int rows, int K) { return (size_t)rows * (K | 1) * 8; }
+template <int THREADS, typename L, typename V>
+__device__ __forceinline__ void stage_from(const StagedEntries &s, const L *labels, const V *values, int K, int all, long long left, int cats) {
+    for (int i0 = threadIdx.x; i0 < all; i0 += 8 * THREADS) {  // (eight of each under way together)
+        L l[8];
+        V v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const long long i = i0 + e * THREADS, at = i < left ? i : left - 1;
+            l[e] = labels[at];
+            v[e] = values[at];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int i = i0 + e * THREADS, r = (unsigned)i / (unsigned)K, at = r * (K | 1) + i - r * K;
+            if (i >= all) continue;
+            s.l[at] = i < left && l[e] >= 0 && l[e] < (L)cats ? (int)l[e] : -1;
+            s.v[at] = to_f32(v[e]);
+        }
+    }
+}
 template <int THREADS>
 __device__ __forceinline__ StagedEntries stage_entries(const DistillK &k, void *lds, long long n0, int rows, int cats) {
-    const int stride = k.K | 1, all = rows * k.K;
-    StagedEntries s = {static_cast<int *>(lds), static_cast<float *>(lds) + rows * stride};
-    const long long left = (k.g.rows - n0) * k.K;
+    const StagedEntries s = {static_cast<int *>(lds), static_cast<float *>(lds) + rows * (k.K | 1)};
+    const long long first = n0 * k.K, left = (k.g.rows - n0) * k.K;
     __syncthreads();  // (the block's last rows have been worked on)
-    for (int i = threadIdx.x; i < all; i += THREADS) {
-        int l = -1;
-        float v = 0.f;
-        if (i < left) l = load_entry(k, n0, i, cats, v);  // (entry i from the first row on)
-        const int r = (unsigned)i / (unsigned)k.K, at = r * stride + i - r * k.K;
-        s.l[at] = l;
-        s.v[at] = v;
-    }
+    auto from = [&](const auto *labels, const auto *values) { stage_from<THREADS>(s, labels + first, values + first, k.K, rows * k.K, left, cats); };
+    auto typed = [&](const auto *labels) {
+        if (k.v_dtype == QMRI_F32) from(labels, static_cast<const float *>(k.values));
+        else if (k.v_dtype == QMRI_F16) from(labels, static_cast<const f16_t *>(k.values));
+        else from(labels, static_cast<const bf16_t *>(k.values));
+    };
+    if (k.l_kind == QMRI_L_I32) typed(static_cast<const int *>(k.labels));
+    else typed(static_cast<const long long *>(k.labels));
     __syncthreads();
     return s;
 }
@@ -982,6 +1007,15 @@ struct LaneEntries {
             return teacher_of(k, any, m, sum, others);
         }
     }
+    // the values become weights
+    __device__ __forceinline__ void to_weights(const Teacher &t) {
+        if constexpr (K > 0) {
+#pragma unroll
+            for (int q = 0; q < K; ++q) v[q] = weight(t, v[q]);
+        } else {
+            for (int q = 0; q < k.K; ++q) at.v[q] = weight(t, at.v[q]);
+        }
+    }
     // which of the 32 categories from c are entries
     __device__ __forceinline__ unsigned marks(int c) const {
         unsigned in = 0u;
@@ -1103,7 +1137,8 @@ __global__ __launch_bounds__(256) void distill_wave_kernel(const DistillK k) {
 template <typename T, int K>
 __global__ __launch_bounds__(kPlaneThreads<K>) void distill_grad_planes_kernel(const DistillK k, int parts, int len) {
     extern __shared__ float s_entries[];  // K 0
-    constexpr int B = kPlaneThreads<K>;
+    constexpr int B = kPlaneThreads<K>, WIN = 16;
+    __shared__ float s_w[K == 2 ? 1 : WIN][B];  // (a lane's own column)
     const LogitsK &g = k.g;
     const int cats = g.C + g.bg;
     const long long blocks = (g.rows + B - 1) / B;
@@ -1121,33 +1156,40 @@ __global__ __launch_bounds__(kPlaneThreads<K>) void distill_grad_planes_kernel(c
         T *grad = static_cast<T *>(k.grad) + row_base(g, n, k.gso, k.gsi), *out = grad + c0 * k.gsc;
         unsigned next[8];
         load_classes(p, g.sc, c1 - c0, next);
-        const LaneEntries<K> entries(k, n, cats, at);
+        LaneEntries<K> entries(k, n, cats, at);
         const Teacher t = entries.teacher();
         const GradRow r = grad_row(k, n, t);
-        if constexpr (K == 0) {  // (weights_of)
-            for (int q = 0; q < k.K; ++q) at.v[q] = weight(t, at.v[q]);
-        }
+        entries.to_weights(t);
         for (int c = c0; c < c1; c += 8) {
-            float y[8];
+            const int w0 = (c - c0) & (WIN - 1);
+            if (K != 2 && w0 == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = widen<T>(next[i]);
+                for (int i = 0; i < WIN; ++i) s_w[i][threadIdx.x] = -1.f;
+                entries.each([&](int l, float w) {
+                    const int j = l - g.bg - c;
+                    if ((unsigned)j < (unsigned)WIN) s_w[j][threadIdx.x] = maxn(s_w[j][threadIdx.x], 0.f) + w;
+                });
+            }
+            float y[8], q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] = widen<T>(next[i]);
+                if constexpr (K == 2) {
+                    q[i] = -1.f;
+                    entries.each([&](int l, float w) { q[i] = l - g.bg == c + i ? maxn(q[i], 0.f) + w : q[i]; });
+                } else {
+                    q[i] = s_w[w0 + i][threadIdx.x];
+                }
+            }
             p += 8 * g.sc;
             if (c + 8 < c1) load_classes(p, g.sc, c1 - c - 8, next);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = grad_outside(r, g.c2, y[i]);
+            for (int i = 0; i < 8; ++i) y[i] = grad_either(r, g.c2, y[i], q[i]);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (c + i < c1) out[i * k.gsc] = from_f32<T>(y[i]);
             out += 8 * k.gsc;
         }
-        entries.each_score(z, [&](int l, float, float zl) {
-            const int c = l - g.bg;
-            if (c < c0 || c >= c1) return;
-            float qs = 0.f;  // (the same label twice: each time the sum of all its entries, in their order)
-            if constexpr (K > 0) entries.each([&](int o, float v) { qs += o == l ? weight(t, v) : 0.f; });
-            else qs = at.weights_of(l, k.K);
-            grad[c * k.gsc] = from_f32<T>(grad_inside(r, g.c2, zl, qs));
-        });
     }
 }
 
