@@ -645,15 +645,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || E == 0 ? 6 : 8) void distill
     }
 }
 
-// As if none of the scores were an entry's label; those are written over by the entries' lanes, when the wave's other stores have
-// arrived.
+// The weights of the scores' entries lie in LDS, a column of 16 for a lane (-1: no entry); a row's last vector, moved to the front
+// where it would end behind the row, finds its own in a column of the row's.  (The entries' scores written over after the others
+// wait for the stores: 500 classes in bf16 with five entries 103 us.)
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK k) {
+    constexpr int V = kVec<T>, NV = 16 / V, ROWS = 256 / G, COLS = 256 + ROWS;
     extern __shared__ float s_entries[];  // E 0
-    __shared__ int s_l[E > 0 ? 256 / G * ((G * E) | 1) : 1];  // entry q of a row at row * (G E | 1) + q
-    __shared__ float s_q[E > 0 ? 256 / G * ((G * E) | 1) : 1];
+    __shared__ int s_l[E > 0 ? ROWS * ((G * E) | 1) : 1];  // entry q of a row at row * (G E | 1) + q
+    __shared__ float s_q[E > 0 ? ROWS * ((G * E) | 1) : 1];
+    __shared__ float s_w[16][COLS];
     const LogitsK &g = k.g;
-    constexpr int V = kVec<T>, NV = 16 / V, ROWS = 256 / G;
     const int gl = threadIdx.x % G, cats = g.C + g.bg, row = threadIdx.x / G;
     for (long long n0 = (long long)blockIdx.x * ROWS; n0 < g.rows; n0 += (long long)gridDim.x * ROWS) {
         const long long nr = n0 + row;
@@ -675,46 +677,68 @@ __global__ __launch_bounds__(256) void distill_grad_group_kernel(const DistillK 
         const EntriesOf<G, E> entries(k, n, gl, cats, at);
         const Teacher t = entries.teacher();
         const GradRow r = grad_row(k, n, t);
-        // what follows wants the weights of a row's entries in one place
-        if constexpr (E > 0) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                s_l[row * ((G * E) | 1) + gl + e * G] = entries.l[e];
-                s_q[row * ((G * E) | 1) + gl + e * G] = entries.l[e] >= 0 ? weight(t, entries.v[e]) : 0.f;
+        for (int i = 0; i < 16; ++i) s_w[i][threadIdx.x] = -1.f;
+        for (int e = gl; e < V; e += G) s_w[e][256 + row] = -1.f;
+        // the same label twice: the sum of all its entries, in their order
+        const int last = g.C - V;  // the first class of the row's last vector
+        if constexpr (E < 0) {
+            wave_sync();
+#pragma unroll
+            for (int q = 0; q < -E; ++q) {
+                const int c = entries.l[q] - g.bg;
+                if (entries.l[q] < 0 || c < 0) continue;
+                const float w = weight(t, entries.v[q]);
+                int owner, bit;
+                place_of<G, V>(c, owner, bit);
+                if (owner == (int)threadIdx.x) s_w[bit][owner] = maxn(s_w[bit][owner], 0.f) + w;
+                if (gl == 0 && c >= last) s_w[c - last][256 + row] = maxn(s_w[c - last][256 + row], 0.f) + w;
             }
-            at = {s_l + row * ((G * E) | 1), s_q + row * ((G * E) | 1)};
-        } else if constexpr (E == 0) {
-            for (int q = gl; q < k.K; q += G) at.v[q] = at.l[q] >= 0 ? weight(t, at.v[q]) : 0.f;
+        } else {
+            // (the weights of a row's entries in one place)
+            if constexpr (E > 0) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    s_l[row * ((G * E) | 1) + gl + e * G] = entries.l[e];
+                    s_q[row * ((G * E) | 1) + gl + e * G] = entries.l[e] >= 0 ? weight(t, entries.v[e]) : 0.f;
+                }
+                at = {s_l + row * ((G * E) | 1), s_q + row * ((G * E) | 1)};
+            } else {
+                for (int q = gl; q < k.K; q += G) at.v[q] = at.l[q] >= 0 ? weight(t, at.v[q]) : 0.f;
+            }
+            wave_sync();
+            if constexpr (G == 2) {  // (both lanes go through all entries)
+                for (int q = 0; q < k.K; ++q) {
+                    const int c = at.l[q] - g.bg;
+                    if (at.l[q] < 0 || c < 0) continue;
+                    const float w = at.v[q];
+                    int owner, bit;
+                    place_of<G, V>(c, owner, bit);
+                    if (owner == (int)threadIdx.x) s_w[bit][owner] = maxn(s_w[bit][owner], 0.f) + w;
+                    if (gl == 0 && c >= last) s_w[c - last][256 + row] = maxn(s_w[c - last][256 + row], 0.f) + w;
+                }
+            } else {
+                entries.each([&](int l, float) {
+                    const int c = l - g.bg;
+                    if (c < 0) return;
+                    const float qs = at.weights_of(l, k.K);
+                    int owner, bit;
+                    place_of<G, V>(c, owner, bit);
+                    s_w[bit][owner] = qs;
+                    if (c >= last) s_w[c - last][256 + row] = qs;
+                });
+            }
         }
         wave_sync();
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            // (a vector moved to the front: scores that another lane has too get the same value from both)
-            const int j = (i * G + gl) * V;
+            const int j = (i * G + gl) * V, back = vec_back<T>(g.C - j);
+            const float *w = back ? &s_w[0][256 + row] : &s_w[i * V][threadIdx.x];
             float y[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = grad_outside(r, g.c2, get(x[i], e));
-            if (live && j < g.C) store_vec(out + j - vec_back<T>(g.C - j), pack_vec<T>(y));
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        // the same label twice: every one of its entries sums all of them, in the order of the entries, and writes the same value
-        if constexpr (E < 0) {
-            float w[-E];
-#pragma unroll
-            for (int q = 0; q < -E; ++q) w[q] = entries.l[q] >= 0 ? weight(t, entries.v[q]) : 0.f;
-            entries.each_score(z, [&](int l, float, float zl) {
-                const int c = l - g.bg;
-                float qs = 0.f;
-#pragma unroll
-                for (int q = 0; q < -E; ++q) qs += entries.l[q] == l ? w[q] : 0.f;
-                if (c >= 0 && live && gl == (c & (G - 1))) out[c] = from_f32<T>(grad_inside(r, g.c2, zl, qs));
-            });
-        } else {
-            entries.each_score(z, [&](int l, float, float zl) {
-                const int c = l - g.bg;
-                if (c < 0 || !live) return;
-                out[c] = from_f32<T>(grad_inside(r, g.c2, zl, at.weights_of(l, k.K)));
-            });
+            for (int e = 0; e < V; ++e) y[e] = grad_either(r, g.c2, get(x[i], e), w[e * COLS]);
+            // (scores that another lane has too get the same value from both)
+            if (live && j < g.C) store_vec(out + j - back, pack_vec<T>(y));
         }
         wave_sync();
     }
@@ -1246,10 +1270,16 @@ void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
             else hipLaunchKernelGGL((distill_group_kernel<T, G, -4>), grid, block, 0, st, k);
             return;
         }
+        if (k.K <= 8 && grad) {  // (20 classes, six entries: 183 us and 230)
+            hipLaunchKernelGGL((distill_grad_group_kernel<T, G, -8>), grid, block, 0, st, k);
+            return;
+        }
     }
     if (k.K <= G * E) {
-        if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, E>), grid, block, 0, st, k);
-        else hipLaunchKernelGGL((distill_group_kernel<T, G, E>), grid, block, 0, st, k);
+        if (!grad) hipLaunchKernelGGL((distill_group_kernel<T, G, E>), grid, block, 0, st, k);
+        if constexpr (G > 2) {
+            if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, E>), grid, block, 0, st, k);
+        }
     } else if constexpr (G < 16) {
         const size_t lds = staged_bytes(256 / G, k.K);
         if (lds > 48 * 1024) {
