@@ -1255,7 +1255,7 @@ void small_of(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
 template <typename T, int G>
 void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of((k.g.rows + 256 / G - 1) / (256 / G), num_cu, 64)), block(256);
-    // up to 16 entries a row in registers, or 64 where a row has that many lanes; 256 / G rows of more in LDS (G 2: at most 64 KB)
+    // up to 16 entries a row in registers, or 64 where a row has that many lanes; 256 / G rows of more in LDS (G 2: at most 65 KB)
     constexpr int E = G >= 16 ? 64 / G : 16 / G > 4 ? 4 : 16 / G;
     // One or two entries: all of them in every lane (1000 classes: 74 us instead of 83); with more it pays only where two lanes share a
     // row (20 classes, three entries: 135 and 149 us; 500 classes: 85 and 81)
@@ -1282,7 +1282,7 @@ void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
         }
     } else if constexpr (G < 16) {
         const size_t lds = staged_bytes(256 / G, k.K);
-        if (lds > 48 * 1024) {
+        if (lds > 16 * 1024) {  // (the gradient has 25 KB of its own)
             (void)hipFuncSetAttribute(reinterpret_cast<const void *>(distill_grad_group_kernel<T, G, 0>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
             (void)hipFuncSetAttribute(reinterpret_cast<const void *>(distill_group_kernel<T, G, 0>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         }

@@ -330,6 +330,36 @@ def test_top_counts(top):
             _check_scores(z, dtype, "planes", rng, top=top)
 
 
+@pytest.mark.parametrize("top", [5, 9, 19, 31, 33, 64])
+def test_long_lists_of_the_best_in_planes(top):
+    rng = np.random.default_rng(3000 + top)
+    for i, dtype in enumerate(DTYPES):
+        for rows in (63, 1000):
+            _check_scores(_scores(rng, rows, 70, ("plain", "ties", "masked")[i]), dtype, ("planes", "nchw")[rows == 1000], rng, top=top)
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 4, 5, 8, 9, 12, 16, 17, 33, 64])
+def test_entry_counts(K):
+    """Numbers of teacher's answers around which the kernels hold them elsewhere, in rows that end inside a vector and in whole ones."""
+    rng = np.random.default_rng(4000 + K)
+    for i, C in enumerate((5, 9, 16, 23, 32, 33, 60, 64, 117, 200, 400, 700, 1024, 1300)):
+        for tail in (False, True):
+            for layout, rows in (("rows", 70), ("planes", 67)) if C <= 200 else (("padded", 9),):
+                _check_distill(_scores(rng, rows, C, ("plain", "masked")[i % 2]), DTYPES[(i + K) % 3], layout, rng, K, tail=tail,
+                               bg=bool(i % 4 == 1), index_type=("int32", "int64")[(i + tail) % 2])
+
+
+@pytest.mark.parametrize("C", [1100, 2051])
+def test_many_rows_of_some_thousand_classes(C):
+    """Enough rows for a wave each."""
+    rng = np.random.default_rng(5000 + C)
+    z = _scores(rng, 4099, C)
+    _check_scores(z, "bfloat16", "rows", rng, top=5)
+    for dtype in ("float32", "bfloat16"):
+        _check_scores_grad(z, dtype, "rows", rng)
+        _check_distill(z, dtype, "padded", rng, 5, tail=dtype == "float32")
+
+
 @pytest.mark.parametrize("kind, ignore", [("int32", -1), ("uint8", 255), ("int16", -7), ("int64", -1), ("int64", 2)])
 def test_label_types_and_the_ignored_label(kind, ignore):
     rng = np.random.default_rng(5)
