@@ -441,10 +441,7 @@ struct Cut {
     int segs, len;
 };
 Cut cut_rows(const LogitsK &g, int num_cu, int longest);
-// A wave a row, with no other to wait for, once every SIMD has four rows of its own and rows are not so long that the last ones
-// leave units idle: 50000 rows of 1999 scores in bf16 with a teacher 78 us, with four waves a row 168
-inline bool wave_rows(const LogitsK &g, int num_cu) { return g.C <= 16384 && g.rows >= 16ll * num_cu; }
-// Gradients, which write as much as they read: longer rows are better left to four waves, 4-byte ones sooner (8192 x 8192: bf16 53
+// Gradients by a wave a row, once every SIMD has four rows; longer ones are better left to four waves, 4-byte ones sooner (8192 x 8192: bf16 53
 // us by one wave and 56 by four, fp32 115 and 101; 50000 x 1999 with a teacher: bf16 105 and 194, fp32 178 and 212)
 template <typename T>
 bool wave_rows_grad(const LogitsK &g, int num_cu) {

@@ -1332,12 +1332,12 @@ void launch(const DistillK &k, int num_cu, hipStream_t st) {
     const Cut cut = cut_rows(g, num_cu, k.tail ? kLongest : 1 << 30);
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
     const unsigned marks = (unsigned)(cut.len + 31) / 32 * 4;
-    if (wave_rows(g, num_cu)) {
+    // One wave a row as soon as every SIMD has two rows: its teacher and its loss are then worked out while other waves read (4096 x
+    // 32000 in bf16: 58 us, with four waves a row 68; 1024 x 100003: 74 and 55).  Longer rows of 2-byte scores are better shared (2048 x
+    // 131000: 122 and 113), of 4-byte scores not (197 and 234).
+    if (g.rows >= 8ll * num_cu && (sizeof(T) == 4 || g.C <= 32768)) {
         if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true, 1>), grid, dim3(64), marks, st, k, cut);
         else hipLaunchKernelGGL((distill_block_kernel<T, false, 1>), grid, dim3(64), 0, st, k, cut);
-    } else if (cut.len >= 16384) {
-        if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true, 8>), grid, dim3(512), marks, st, k, cut);
-        else hipLaunchKernelGGL((distill_block_kernel<T, false, 8>), grid, dim3(512), 0, st, k, cut);
     } else {
         if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true, 4>), grid, dim3(256), marks, st, k, cut);
         else hipLaunchKernelGGL((distill_block_kernel<T, false, 4>), grid, dim3(256), 0, st, k, cut);

@@ -1044,13 +1044,13 @@ void launch(const ScoresK &k, int num_cu, hipStream_t st) {
     if (g.C <= 1024) return group<T, 64>(k, false, num_cu, st);
     const Cut cut = cut_rows(g, num_cu, 1 << 30);
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
-    if (wave_rows(g, num_cu)) {
+    // A wave a row, with no other to wait for, where every SIMD has four rows: 50000 x 1999 in bf16 65 us, with the 8 best 116 (four waves
+    // a row: 107, 226).  From 16 KB a row on there is nothing in it (8192 x 8192: 34 and 35), in 4-byte scores it loses (61 and 54).
+    if (g.C <= 16384 / (int)sizeof(T) && g.rows >= 16ll * num_cu) {
         if (k.top) hipLaunchKernelGGL((scores_block_kernel<T, true, 1>), grid, dim3(64), 0, st, k, cut);
         else hipLaunchKernelGGL((scores_block_kernel<T, false, 1>), grid, dim3(64), 0, st, k, cut);
     } else if (k.top) {
         hipLaunchKernelGGL((scores_block_kernel<T, true, 4>), grid, dim3(256), 0, st, k, cut);
-    } else if (cut.len >= 16384) {
-        hipLaunchKernelGGL((scores_block_kernel<T, false, 8>), grid, dim3(512), 0, st, k, cut);
     } else {
         hipLaunchKernelGGL((scores_block_kernel<T, false, 4>), grid, dim3(256), 0, st, k, cut);
     }
