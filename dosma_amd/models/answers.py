@@ -24,11 +24,11 @@ from dosma_amd import _hostpool, _lib
 __all__ = ["LabelScores", "DistillLoss", "label_scores", "label_scores_grad", "distill_loss", "distill_loss_grad"]
 
 #: ``log_prob`` (None without labels), ``entropy`` in nats, ``norm`` (..., 2): the row maximum M and ln sum exp((z - M) / T),
-#: which the gradient needs (M / T + norm[..., 1] is log sum exp(z / T)); None unless asked for; ``top_log_prob`` / ``top_label``
-#: (..., top) or None
+#: which the gradient needs (M / T + norm[..., 1] is log sum exp(z / T)); None unless asked for or needed by a gradient;
+#: ``top_log_prob`` / ``top_label`` (..., top) or None
 LabelScores = namedtuple("LabelScores", "log_prob entropy norm top_log_prob top_label")
 #: ``loss`` in nats, ``norm`` as above, ``log_tail``: log probability outside the teacher's entries (None without the tail); both
-#: None unless ``norm`` is asked for
+#: None unless ``norm`` is asked for or a gradient needs them
 DistillLoss = namedtuple("DistillLoss", "loss norm log_tail")
 
 

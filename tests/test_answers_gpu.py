@@ -708,6 +708,48 @@ def test_captured_and_replayed(shape, K):
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_a_training_step_captured_and_replayed():
+    """Forward and backward by autograd in one graph, replayed with other inputs between eager steps."""
+    torch = torch_()
+    rng = np.random.default_rng(31)
+    z = torch.empty((3, 12, 70), device="cuda", requires_grad=True)  # (B, C, P)
+    lab = torch.empty((3, 70), dtype=torch.int64, device="cuda")
+    t_lab = torch.empty((3, 70, 4), dtype=torch.int32, device="cuda")
+    t_val = torch.empty((3, 70, 4), device="cuda")
+    w = torch.ones((3, 70), device="cuda")
+
+    def fill():
+        with torch.no_grad():
+            z.copy_(torch.from_numpy(rng.standard_normal((3, 12, 70)).astype(np.float32)))
+            t = A.label_scores(torch.from_numpy(rng.standard_normal((3, 12, 70)).astype(np.float32)).cuda(), dim=1, top=4)
+        lab.copy_(torch.from_numpy(rng.integers(0, 12, (3, 70))))
+        t_lab.copy_(t.top_label)
+        t_val.copy_(t.top_log_prob)
+
+    def step():
+        s = A.label_scores(z, lab, dim=1)
+        d = A.distill_loss(z, t_lab, t_val, dim=1, tail=True)
+        return torch.autograd.grad([d.loss, s.log_prob, s.entropy], z, [w, -w, w])[0], d.loss.detach()
+
+    fill()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        fill()
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        del want
+
+
 def test_the_same_bits_every_time():
     torch = torch_()
     for shape, bg in (((5, 100003), False), ((30000, 4), True), ((900, 900), False)):
