@@ -207,9 +207,9 @@ __device__ __forceinline__ Tile<T> load_tile(const T *p, int n) {
     return r;
 }
 
-// The bits of 8 scores, a class `sc` apart, `left` of them there and -inf behind.  (Bits in words of their own, and the whole eight
+// The bits of N scores, a class `sc` apart, `left` of them there and -inf behind.  (Bits in words of their own, and the whole N
 // without a condition: what is packed, converted or branched upon would be waited for on the spot, and these are meant to be in
-// flight while the eight before them are worked on.)
+// flight while the N before them are worked on.)
 template <typename T>
 __device__ __forceinline__ unsigned load_bits(const T *p) {
     if constexpr (sizeof(T) == 4) return *reinterpret_cast<const unsigned *>(p);
@@ -221,15 +221,15 @@ __device__ __forceinline__ float widen(unsigned w) {
     else if constexpr (std::is_same_v<T, bf16_t>) return __uint_as_float(w << 16);
     else return static_cast<float>(__builtin_bit_cast(T, (unsigned short)w));
 }
-template <typename T>
-__device__ __forceinline__ void load_classes(const T *p, long long sc, int left, unsigned (&v)[8]) {
-    if (left >= 8) {
+template <typename T, int N>
+__device__ __forceinline__ void load_classes(const T *p, long long sc, int left, unsigned (&v)[N]) {
+    if (left >= N) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = load_bits(p + i * sc);
+        for (int i = 0; i < N; ++i) v[i] = load_bits(p + i * sc);
     } else {
         const unsigned none = bits_of(static_cast<T>(kNegInf));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < left ? load_bits(p + i * sc) : none;
+        for (int i = 0; i < N; ++i) v[i] = i < left ? load_bits(p + i * sc) : none;
     }
 }
 // Classes that do not lie together, a lane a row: into how many parts (of whole eights) a row is cut so that every compute unit has

@@ -662,7 +662,7 @@ struct LaneBestKey {  // 2-byte scores, labels that fit the unused bits
 // other, so from LDS (a row every top | 1 words) they are written as one piece.
 template <int K>
 constexpr int kPlaneThreads = K > 32 ? 64 : 256;
-template <typename T, int K, bool KEY>
+template <typename T, int K, bool KEY, int CH>
 __global__ __launch_bounds__(kPlaneThreads<K>) void scores_planes_kernel(const ScoresK k) {
     constexpr int B = kPlaneThreads<K>;
     extern __shared__ int s_top[];  // K > 4
@@ -681,19 +681,19 @@ __global__ __launch_bounds__(kPlaneThreads<K>) void scores_planes_kernel(const S
             r = {0.f, 0.f, 1.f, 0.f};
             if (K) best.take(0.f, 0);
         }
-        unsigned next[8];
+        unsigned next[CH];
         load_classes(z, g.sc, g.C, next);
         const T *p = z;
-        for (int c = 0; c < g.C; c += 8) {
-            float x[8];
+        for (int c = 0; c < g.C; c += CH) {
+            float x[CH];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = widen<T>(next[i]);
-            p += 8 * g.sc;
-            if (c + 8 < g.C) load_classes(p, g.sc, g.C - c - 8, next);
+            for (int i = 0; i < CH; ++i) x[i] = widen<T>(next[i]);
+            p += CH * g.sc;
+            if (c + CH < g.C) load_classes(p, g.sc, g.C - c - CH, next);
             add_scores(r, x, g.c2);
             if (K) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) best.take(x[i], c + i + g.bg);
+                for (int i = 0; i < CH; ++i) best.take(x[i], c + i + g.bg);
             }
         }
         RowStat st = {r.m, reference(r.m), 0.f, 0.f};
@@ -998,9 +998,23 @@ void planes(const ScoresK &k, int num_cu, hipStream_t st) {
     constexpr int B = kPlaneThreads<K>;
     const dim3 grid(grid_of((k.g.rows + B - 1) / B, num_cu, 64 * (256 / B))), block(B);
     const size_t lds = K > 4 ? (size_t)B * (k.top | 1) * 4 : 0;
-    // (the last eight classes may reach 7 labels beyond the last)
-    if (sizeof(T) == 2 && k.g.C + k.g.bg + 7 <= (1 << kLabelBits<T>)) hipLaunchKernelGGL((scores_planes_kernel<T, K, sizeof(T) == 2>), grid, block, lds, st, k);
-    else hipLaunchKernelGGL((scores_planes_kernel<T, K, false>), grid, block, lds, st, k);
+    if constexpr (sizeof(T) == 2) {
+        // (the last CH classes may reach CH - 1 labels beyond the last)
+        const bool key = k.g.C + k.g.bg + 15 <= (1 << kLabelBits<T>);
+        if constexpr (K <= 4) {
+            // 16 classes in flight where 2-byte rows are long enough (117 classes in f16: 64 us instead of 73, with the best 75 and 82; 20
+            // classes 22 and 19; 4-byte scores are no faster with it)
+            if (key && k.g.C > 48) {
+                hipLaunchKernelGGL((scores_planes_kernel<T, K, true, 16>), grid, block, lds, st, k);
+                return;
+            }
+        }
+        if (key) {
+            hipLaunchKernelGGL((scores_planes_kernel<T, K, true, 8>), grid, block, lds, st, k);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((scores_planes_kernel<T, K, false, 8>), grid, block, lds, st, k);
 }
 
 template <typename T>
