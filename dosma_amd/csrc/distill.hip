@@ -787,8 +787,9 @@ __device__ __forceinline__ void add_outside(Running &r, const float (&x)[N], flo
         r.t += s;
     }
 }
+// 4-byte scores want 80 registers (4096 x 32000: 99 us, 121 with 64, which spill in the loop); 2-byte ones do with 64.
 template <typename T, bool TAIL, int W>
-__global__ __launch_bounds__(64 * W, 8) void distill_block_kernel(const DistillK k, const Cut cut) {
+__global__ __launch_bounds__(64 * W, sizeof(T) == 4 ? 6 : 8) void distill_block_kernel(const DistillK k, const Cut cut) {
     __shared__ RowStat s_stat[W];
     extern __shared__ unsigned s_bits[];  // TAIL: cut.len bits
     __shared__ int s_back;
@@ -1351,9 +1352,9 @@ void launch(const DistillK &k, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
     const unsigned marks = (unsigned)(cut.len + 31) / 32 * 4;
     // One wave a row as soon as every SIMD has two rows: its teacher and its loss are then worked out while other waves read (4096 x
-    // 32000 in bf16: 58 us, with four waves a row 68; 1024 x 100003: 74 and 55).  Longer rows of 2-byte scores are better shared (2048 x
-    // 131000: 122 and 113), of 4-byte scores not (197 and 234).
-    if (g.rows >= 8ll * num_cu && (sizeof(T) == 4 || g.C <= 32768)) {
+    // 32000 in bf16: 58 us, with four waves a row 68; 1024 x 100003: 74 and 55).  Longer rows are better shared, of 4-byte scores sooner
+    // (bf16 2048 x 131000: 122 and 113; fp32 8192 x 16385: 114 and 106, 50000 x 1999: 88 and 162).
+    if (g.rows >= 8ll * num_cu && g.C <= (sizeof(T) == 4 ? 8192 : 32768)) {
         if (k.tail) hipLaunchKernelGGL((distill_block_kernel<T, true, 1>), grid, dim3(64), marks, st, k, cut);
         else hipLaunchKernelGGL((distill_block_kernel<T, false, 1>), grid, dim3(64), 0, st, k, cut);
     } else {
