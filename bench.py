@@ -427,6 +427,7 @@ class GpuSampler:
         for h in cands:
             clk = os.path.join(h, "freq1_input")
             pw = next((os.path.join(h, f) for f in ("power1_average", "power1_input") if os.path.exists(os.path.join(h, f))), None)
+            self.f_pow = self.f_pow or pw  # (a node without the clock's file still has the power's)
             if os.path.exists(clk) and self._read(clk) is not None:
                 self.how, self.f_clk, self.f_pow = f"hwmon ({os.path.basename(clk)}, {os.path.basename(pw) if pw else 'no power file'})", clk, pw
                 break
@@ -436,6 +437,8 @@ class GpuSampler:
             self.smi = shutil.which("rocm-smi") or "/opt/rocm/bin/rocm-smi"
             if os.path.exists(self.smi):
                 self.how = "rocm-smi --showpower --showclocks (polled)"
+                if self.f_pow:
+                    self.how += f", hwmon {os.path.basename(self.f_pow)}"
 
     @staticmethod
     def _read(path):
@@ -465,6 +468,7 @@ class GpuSampler:
                 self._stop.wait(self.period)
             else:
                 c, w = self._poll_smi()
+                w = w or (self._read(self.f_pow) if self.f_pow else None)
             self.rows.append((time.perf_counter(), c, w))
 
     def __enter__(self):
