@@ -204,16 +204,28 @@ __device__ __forceinline__ float gather(const LogitsK &g, const T *z, int l) {
     return l < g.bg ? 0.f : to_f32(z[(long long)(l - g.bg) * g.sc]);
 }
 // ln of the sum outside the entries, relative to p.ref.  A student that leaves less than 2^-100 out there (its terms vanish next to
-// the maximum's) has it summed again relative to the largest outside: the G lanes read the row once more.  Rare.
+// the maximum's) has it summed again relative to the largest outside, where anyone asks: the G lanes read the row once more.  Rare.
 template <int G, typename T>
 __device__ __forceinline__ float log_outside(const DistillK &k, long long n, const T *z, int gl, int cats, const Student &p, const Teacher &t, float so) {
     if (!k.tail) return 0.f;
-    if (!(so < 7.888609e-31f) || t.rest == 0.f || p.empty) return ln(so);
+    if (!(so < 7.888609e-31f) || (t.rest == 0.f && !k.log_tail) || p.empty) return ln(so);
+    unsigned long long mask = 0ull;  // the entries of up to 64 categories
+    if (cats <= 64) {
+        float v;
+        for (int q = 0; q < k.K; ++q) {
+            const int l = load_entry(k, n, q, cats, v);
+            mask |= l >= 0 ? 1ull << l : 0ull;
+        }
+        if (mask == ~0ull >> (64 - cats)) return kNegInf;
+    }
     auto score = [&](int j) {
+        const float z_j = gather(k.g, z, j);
+        if (z_j == kNegInf) return kNegInf;
+        if (cats <= 64) return mask >> j & 1ull ? kNegInf : z_j;
         float v;
         for (int q = 0; q < k.K; ++q)
             if (load_entry(k, n, q, cats, v) == j) return kNegInf;
-        return gather(k.g, z, j);
+        return z_j;
     };
     float m = kNegInf, s = 0.f;
     for (int j = gl; j < cats; j += G) m = maxn(m, score(j));

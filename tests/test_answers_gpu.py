@@ -473,6 +473,32 @@ def test_a_sure_student_keeps_its_small_tail():
         assert np.all(np.abs(g - want["grad"]) < 2 * tol * (np.abs(want["grad"]) + 1e-3))
 
 
+def test_a_sure_student_of_a_certain_teacher():
+    """The teacher leaves nothing outside its entries: the loss does not look there, ``log_tail`` still says what the student does."""
+    torch = torch_()
+    for C, layout in ((6, "rows"), (5, "planes"), (33, "planes"), (64, "rows"), (100, "rows"), (117, "planes"), (3000, "rows"), (3000, "planes")):
+        rng = np.random.default_rng(7 * C)
+        z = rng.standard_normal((5, C))
+        z[:, 2] += 150.0
+        z[1, 4:] = -np.inf
+        z[2, np.arange(C) != 2] = -np.inf  # nothing else is offered
+        t, dim, held = _tensor(z, "float32", layout, rng)
+        idx = np.tile(np.array([[2, 0]]), (5, 1))
+        val = np.tile(np.array([[0.0, -200.0]], np.float32), (5, 1))
+        ti, tv = torch.from_numpy(idx).cuda(), torch.from_numpy(val).cuda()
+        r = A.distill_loss(t, ti, tv, dim=dim, norm=True, tail=True)
+        want = ao.distill(held, idx, val.astype(float), 1.0, True, np.ones(5))
+        assert np.all(want["rest"] == 0.0) and np.isneginf(want["log_tail"][2])
+        fin = np.isfinite(want["log_tail"])
+        got = _host(r.log_tail)
+        assert np.all(np.isneginf(got[~fin]))
+        assert np.all(np.abs(got[fin] - want["log_tail"][fin]) < U * (3 * 160 + _n(C) + 100))  # (as above)
+    # every category an entry
+    r = A.distill_loss(torch.zeros(4, 12, device="cuda"), torch.arange(12, device="cuda").repeat(4, 1), torch.full((4, 12), np.log(1 / 12), device="cuda"),
+                       norm=True, tail=True)
+    assert np.all(np.isneginf(_host(r.log_tail))) and np.all(np.abs(_host(r.loss)) < 100 * U)
+
+
 def test_a_sure_teacher_keeps_its_small_rest():
     """1 - sum q of a teacher that is all but certain: taken as 1 - e^{v_max} without the cancellation."""
     torch = torch_()
