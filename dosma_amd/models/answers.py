@@ -13,7 +13,10 @@ results are numpy arrays.  ``dim`` is the class axis: -1 for rows, 1 for the (B,
 per-row arguments and results have the shape of ``logits`` without that axis.
 
 A score of -inf is a category that is not offered: probability 0, never an alternative.  A row of nothing but -inf has log
-probability -inf, entropy 0, no alternatives, loss 0 and gradient 0.  NaN or +inf makes the row's results NaN."""
+probability -inf, entropy 0, no alternatives, loss 0 and gradient 0.  NaN or +inf makes the row's results NaN.
+
+Calls on tensors can be captured into a graph, their gradients as well; as with every backward pass in torch, no eager graph of
+the same leaves may be alive while one is captured (a leaf's accumulation stays on the stream that it was first used on)."""
 import sys
 from collections import namedtuple
 
