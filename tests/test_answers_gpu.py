@@ -776,6 +776,46 @@ def test_a_training_step_captured_and_replayed():
         del want
 
 
+@pytest.mark.parametrize("layout", ["rows", "planes"])
+def test_many_answers_captured_and_replayed(layout):
+    """More answers than registers are given to: memory beyond a kernel's usual share is asked for while capturing."""
+    torch = torch_()
+    C, rows, K, dim = 20, 700, 64, -1 if layout == "rows" else 0
+    z = torch.empty((rows, C) if layout == "rows" else (C, rows), device="cuda")
+    idx = torch.full((rows, K), -1, dtype=torch.int32, device="cuda")
+    val = torch.zeros((rows, K), device="cuda")
+    one = torch.ones(rows, device="cuda")
+
+    def fill():
+        z.normal_()
+        t = A.label_scores(torch.randn(rows, C, device="cuda"), top=C)
+        idx[:, :C].copy_(t.top_label)
+        idx[:, C:2 * C].copy_(t.top_label)  # every label twice
+        val[:, :2 * C].copy_(torch.randn(rows, 2 * C, device="cuda"))
+
+    def work():
+        d = A.distill_loss(z, idx, val, dim=dim, norm=True)
+        return d.loss, A.distill_loss_grad(z, idx, val, d.norm, grad_loss=one, dim=dim)
+
+    fill()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for _ in range(3):
+        fill()
+        want = work()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    full = _host(z) if layout == "rows" else _host(z).T
+    ref = ao.distill(full, idx.cpu().numpy(), _host(val), 1.0, False, np.ones(rows))
+    # K + 16 roundings of terms whose weights sum to 1, and of log q, log p below 20
+    assert np.all(np.abs(_host(out[0]) - ref["loss"]) < (K + 16) * U * 40)
+    g = _host(out[1]) if layout == "rows" else _host(out[1]).T
+    assert np.all(np.abs(g - ref["grad"]) < (K + 16) * U * 4)
+
+
 def test_the_same_bits_every_time():
     torch = torch_()
     for shape, bg in (((5, 100003), False), ((30000, 4), True), ((900, 900), False)):
