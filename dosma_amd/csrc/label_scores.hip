@@ -140,6 +140,7 @@ __global__ __launch_bounds__(256) void scores_small_kernel(const ScoresK k) {
 // found one after the other: a maximum over 17 keys a lane, one over the lanes.  200000 x 500 in fp32 80 us (5.0 TB/s, memory), in bf16
 // 51 us (4.0 TB/s); with the three best 111 and 84 us, bound by the vector unit.
 // Without the best: 64 registers, eight waves a SIMD (500 classes in bf16, 200000 rows: 51 us instead of 55 with the code of both).
+// With them 78: held to 64 they spill (104 us instead of 86).  Keys made two scores at a time in packed 16-bit integers are no faster.
 template <typename T, int G, bool TOP>
 __global__ __launch_bounds__(256, TOP ? 4 : 8) void scores_group_kernel(const ScoresK k) {
     const LogitsK &g = k.g;
