@@ -232,6 +232,8 @@ __global__ __launch_bounds__(256, TOP ? 4 : 8) void scores_group_kernel(const Sc
 // A score can belong to the k best only if it is above a floor for which k others are known.  What passes the floor goes into a
 // buffer of the wave's in LDS; a full buffer is cut down to its k best, whose last is the new floor.  The order is (score falling,
 // label rising), so the result does not depend on who came first.
+// No two pairs of a buffer have the same label, and none is an empty slot (label -1): equal scores are told apart by their labels, so
+// a cut leaves at most k <= 64 pairs, which is what makes room for the next 64 and what final_best reads.
 // Which of the wave's 64 N (key, label) pairs are its k best; key 0: none.  The k-th largest key is found bit by bit.
 template <int N, int BITS>
 __device__ __forceinline__ unsigned select_best(const unsigned (&key)[N], const int (&id)[N], int k, bool (&win)[N]) {
@@ -590,8 +592,9 @@ __global__ __launch_bounds__(256) void scores_join_kernel(const ScoresK k, const
             for (int q0 = w * 64; q0 < pairs; q0 += 256) {
                 const int q = q0 + lane, sg = q / k.top, at = q - sg * k.top;
                 const float *a = p + sg * words + 4;
-                const bool in = q < pairs;
-                b.take<BITS>(in ? a[at] : kNegInf, in ? reinterpret_cast<const int *>(a)[k.top + at] : -1, in);
+                // (a segment that offers fewer than k has empty slots behind its last: they are no pairs)
+                const int id = q < pairs ? reinterpret_cast<const int *>(a)[k.top + at] : -1;
+                b.take<BITS>(id >= 0 ? a[at] : kNegInf, id, id >= 0);
             }
             if (b.n > 64) b.cut<BITS>();
             for (int q = b.n + lane; q < 64; q += 64) b.i[q] = -1;

@@ -338,6 +338,22 @@ def test_long_lists_of_the_best_in_planes(top):
             _check_scores(_scores(rng, rows, 70, ("plain", "ties", "masked")[i]), dtype, ("planes", "nchw")[rows == 1000], rng, top=top)
 
 
+@pytest.mark.parametrize("top", [5, 20, 33, 64])
+@pytest.mark.parametrize("C", [60011, 131071])
+def test_best_of_a_long_row_that_offers_few_categories(C, top):
+    """A row cut into segments, most of which offer nothing or less than the list is long: their empty slots are no answers."""
+    rng = np.random.default_rng(C + top)
+    offers = {"a late one": [C - 1071], "three far apart": [1000, C // 2, C - 1071], "the end": range(C - C // 8, C), "nothing": [],
+              "the beginning": range(0, 50), "two segments": range(8192 - 10, 8192 + 10), "one in 997": range(3, C, 997)}
+    for i, (what, those) in enumerate(offers.items()):
+        for rows in (1, 3):
+            z = np.full((rows, C), -np.inf)
+            z[:, list(those)] = rng.standard_normal((rows, len(those))) * 2.5
+            if rows == 3:
+                z[1] = np.where(np.isfinite(z[1]), 1.0, -np.inf)  # all alike: the lowest labels
+            _check_scores(z, DTYPES[(i + rows) % 3], "rows", rng, top=top, bg=(i + rows // 3) % 2 == 1)
+
+
 @pytest.mark.parametrize("K", [1, 2, 3, 4, 5, 8, 9, 12, 16, 17, 33, 64])
 def test_entry_counts(K):
     """Numbers of teacher's answers around which the kernels hold them elsewhere, in rows that end inside a vector and in whole ones."""
