@@ -948,6 +948,9 @@ def _fill_logits(a, ptr, dtype, rows, temperature, background):
 
 
 def _fill_grad(a, ptr, rows):
+    if rows.inner < rows.rows or a.logits.inner < a.logits.rows:  # (one group of rows each: where it ends does not matter)
+        if rows.inner != a.logits.inner:
+            raise ValueError(f"the gradient's rows are counted by {rows.inner}, those of the logits by {a.logits.inner}")
     a.grad = ptr
     a.grad_stride_outer, a.grad_stride_inner, a.grad_stride_class = rows.so, rows.si, rows.sc
 

@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <numeric>
 
 #include "answers.h"
 #include "qmri_internal.h"
@@ -110,11 +111,19 @@ int check_logits(const qmri_logits &l, int device, bool need_data) {
     return QMRI_OK;
 }
 
+// Two axes of n and m elements, s and t apart: do any i < n and j < m other than 0, 0 meet (i s = j t)?
+bool axes_meet(int64_t n, int64_t s, int64_t m, int64_t t) {
+    if (n <= 1 || m <= 1) return false;
+    const int64_t g = std::gcd(s, t);
+    return t / g < n && s / g < m;
+}
+
 int check_grad(const qmri_logits &l, const void *grad, int64_t so, int64_t si, int64_t sc) {
     A_ARG(l.rows == 0 || grad, "grad is NULL");
-    const int64_t inner = l.inner < l.rows ? l.inner : l.rows;
-    A_ARG((l.classes == 1 || sc >= 1) && (inner <= 1 || si >= 1) && (l.rows <= l.inner || so >= 1),
-          "grad must have a place of its own for every score (stride 0 or negative)");
+    const int64_t inner = l.inner < l.rows ? l.inner : l.rows, outer = l.rows == 0 ? 0 : (l.rows + inner - 1) / inner;
+    A_ARG((l.classes == 1 || sc >= 1) && (inner <= 1 || si >= 1) && (outer <= 1 || so >= 1) && !axes_meet(l.classes, sc, inner, si) &&
+              !axes_meet(l.classes, sc, outer, so) && !axes_meet(inner, si, outer, so),
+          "grad must have a place of its own for every score (stride 0 or negative, or rows that meet)");
     return QMRI_OK;
 }
 

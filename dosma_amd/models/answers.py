@@ -48,29 +48,40 @@ def _check_dim(ndim, dim):
     return dim % ndim
 
 
-def _rows_of(shape, strides, dim):
-    """-> (row shape, Rows), or (row shape, None) where the rows need more than two strides."""
-    groups, rows = [], 1
+def _rows_of(shape, strides, dim, beside=None):
+    """-> (row shape, Rows), or (row shape, None) where the rows need more than two strides.
+
+    ``beside``: the strides of another tensor of this shape.  Its rows are counted together with these (one ``inner`` for both), so
+    two axes are merged only where both tensors allow it; -> (row shape, Rows, Rows of the other), None for both where that takes
+    more than two groups."""
+    groups, rows = [], 1  # (length, stride, the other's stride)
     for i, n in enumerate(shape):
         if i == dim:
             continue
         rows *= n
         if n == 1:
             continue
-        st = strides[i]
-        if groups and groups[-1][1] == st * n:
-            groups[-1] = (groups[-1][0] * n, st)
+        st, other = strides[i], 0 if beside is None else beside[i]
+        if groups and groups[-1][1] == st * n and groups[-1][2] == other * n:
+            groups[-1] = (groups[-1][0] * n, st, other)
         else:
-            groups.append((n, st))
+            groups.append((n, st, other))
     row_shape = tuple(shape[:dim]) + tuple(shape[dim + 1:])
-    C, sc = shape[dim], strides[dim] if shape[dim] > 1 else 1
-    if rows == 0 or not groups:
-        return row_shape, _lib.Rows(rows, C, 1, 0, C, sc)
-    if len(groups) == 1:
-        return row_shape, _lib.Rows(rows, C, groups[0][0], 0, groups[0][1], sc)
-    if len(groups) == 2:
-        return row_shape, _lib.Rows(rows, C, groups[1][0], groups[0][1], groups[1][1], sc)
-    return row_shape, None
+    C = shape[dim]
+
+    def geometry(strides, at):
+        sc = strides[dim] if C > 1 else 1
+        if rows == 0 or not groups:
+            return _lib.Rows(rows, C, 1, 0, C, sc)
+        if len(groups) == 1:
+            return _lib.Rows(rows, C, groups[0][0], 0, groups[0][at], sc)
+        if len(groups) == 2:
+            return _lib.Rows(rows, C, groups[1][0], groups[0][at], groups[1][at], sc)
+        return None
+
+    if beside is None:
+        return row_shape, geometry(strides, 1)
+    return row_shape, geometry(strides, 1), geometry(beside, 2)
 
 
 # ---- torch ---------------------------------------------------------------------------------------------------------------
@@ -145,13 +156,27 @@ class _TorchCall:
         self.held = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
         return self.held.data_ptr()
 
-    def grad_like(self, x, dim):
+    def grad_like(self, x, dim, rows):
+        """-> (scores, their Rows, gradient, its Rows); ``rows``: those of the scores alone.  The gradient has the layout of the
+        scores, or dense rows where the two cannot be walked through together in that; the scores are copied where not even these
+        can."""
         g = self.torch.empty_like(x)
-        rows = _rows_of(g.shape, g.stride(), dim)[1]
-        if rows is None or any(st == 0 and n > 1 for n, st in zip(g.shape, g.stride())):
+        if x.is_contiguous():
+            return x, rows, g, rows
+        rows, grad_rows = self._together(x, g, dim)
+        if rows is None:
             g = self.torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            rows = _rows_of(g.shape, g.stride(), dim)[1]
-        return g, rows
+            rows, grad_rows = self._together(x, g, dim)
+        if rows is None:
+            x = x.contiguous()
+            rows, grad_rows = self._together(x, g, dim)
+        return x, rows, g, grad_rows
+
+    @staticmethod
+    def _together(x, g, dim):
+        if any(st == 0 and n > 1 for n, st in zip(g.shape, g.stride())):
+            return None, None
+        return _rows_of(x.shape, x.stride(), dim, g.stride())[1:]
 
 
 def _scores_tensor(x, labels, dim, top, norm, temperature, background, ignore_label):
@@ -189,7 +214,7 @@ def _scores_grad_tensor(x, labels, norm, grad_log_prob, entropy, grad_entropy, d
             entropy = _tensor_arg("entropy", entropy, shape, dev, _F32)
     else:
         entropy = None
-    grad, grad_rows = call.grad_like(x, dim)
+    x, rows, grad, grad_rows = call.grad_like(x, dim, rows)
     _lib.label_scores_grad(x.data_ptr(), _name(x.dtype), rows, grad.data_ptr(), grad_rows, norm.data_ptr(), labels_ptr=_ptr(labels),
                            l_dtype=l_dtype, ignore_label=ignore_label, temperature=temperature, background=background,
                            entropy=_ptr(entropy), grad_log_prob=_ptr(grad_log_prob), grad_entropy=_ptr(grad_entropy),
@@ -224,7 +249,7 @@ def _distill_grad_tensor(x, top_label, values, norm, log_tail, grad_loss, dim, t
     grad_loss = _tensor_arg("grad_loss", grad_loss, shape, dev, _F32)
     if log_tail is not None:
         log_tail = _tensor_arg("log_tail", log_tail, shape, dev, _F32)
-    grad, grad_rows = call.grad_like(x, dim)
+    x, rows, grad, grad_rows = call.grad_like(x, dim, rows)
     _lib.distill_grad(x.data_ptr(), _name(x.dtype), rows, grad.data_ptr(), grad_rows, lab.data_ptr(), _name(lab.dtype),
                       val.data_ptr(), _name(val.dtype), lab.shape[-1], norm.data_ptr(), grad_loss.data_ptr(),
                       log_tail=_ptr(log_tail), tail=tail, temperature=temperature, background=background, device=call.index,

@@ -436,7 +436,8 @@ typedef struct qmri_label_scores_args {
     /* gradient: grad = grad_log_prob d log_prob / dz + grad_entropy d entropy / dz */
     const float *grad_log_prob; /* nullable [rows]; needs labels */
     const float *grad_entropy;  /* nullable [rows]; needs entropy */
-    void *grad;                 /* same type and classes as the logits, rounded once; must not overlap them */
+    void *grad;                 /* same type and classes as the logits, rounded once; must not overlap them.  Row n begins at
+                                   grad + (n / inner) * grad_stride_outer + (n % inner) * grad_stride_inner, `inner` the logits' */
     int64_t grad_stride_outer, grad_stride_inner, grad_stride_class;
     void *workspace;            /* nullable: device memory of at least qmri_label_scores_workspace() bytes, in use until the
                                    call's work is done; NULL: taken from the stream's memory pool (not while capturing) */
@@ -473,7 +474,7 @@ typedef struct qmri_distill_args {
     float *log_tail;       /* [rows] log p_t (tail 1) */
     const float *grad_loss; /* [rows] */
     void *grad;            /* d sum_n grad_loss_n loss_n / dz: same type and classes as the logits, rounded once; must not
-                              overlap them */
+                              overlap them; its rows as in qmri_label_scores_args */
     int64_t grad_stride_outer, grad_stride_inner, grad_stride_class;
     void *workspace;       /* as in qmri_label_scores_args */
     uint64_t workspace_bytes;

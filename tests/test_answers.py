@@ -210,3 +210,99 @@ def test_oracle_gradients_against_differences():
                 dn[i] -= 1e-5
                 num[i] = (fn(up) - fn(dn)) / 2e-5
             assert np.abs(num - g).max() < 1e-8
+
+
+def test_gradients_rows_that_meet_are_refused(lib):
+    """The row axis and the class axis of a gradient must not share places: one group of 6 rows a step apart, classes 3 apart."""
+    for bad in (dict(rows=6, inner=6, grad_stride_inner=1, grad_stride_class=3), dict(grad_stride_inner=2, grad_stride_class=2),
+                dict(rows=6, inner=3, grad_stride_inner=4, grad_stride_outer=8), dict(rows=6, inner=3, grad_stride_inner=9, grad_stride_outer=3)):
+        assert lib.qmri_label_scores_grad_device(ctypes.byref(_scores_args(**bad))) == L.QMRI_ERR_ARG
+        assert b"place of its own" in lib.qmri_last_error()
+        assert lib.qmri_distill_grad_device(ctypes.byref(_distill_args(**bad))) == L.QMRI_ERR_ARG
+        assert b"place of its own" in lib.qmri_last_error()
+
+
+def random_layout(rng, shape, make):
+    """A view of ``shape`` of what ``make(shape)`` gives: permuted in memory, cropped, in steps, repeated."""
+    nd = len(shape)
+    order = rng.permutation(nd) if rng.random() < 0.6 else np.arange(nd)
+    big, cut, rep = [], [], []
+    for n in shape:
+        kind = rng.choice(["whole", "whole", "crop", "step", "repeat"])
+        first, step = (int(rng.integers(0, 3)), 1) if kind == "crop" else (int(rng.integers(0, 2)), int(rng.integers(2, 4))) if kind == "step" else (0, 1)
+        big.append(1 if kind == "repeat" else first + step * n + (int(rng.integers(0, 2)) if kind == "crop" else 0))
+        cut.append(slice(first, first + step * n, step))
+        rep.append(kind == "repeat")
+    t = make([big[i] for i in order]).permute(*[int(i) for i in np.argsort(order)])
+    t = t[tuple(slice(None) if r else c for c, r in zip(cut, rep))]
+    t = t[tuple(slice(0, n) for n in shape)]
+    return t.expand(*shape)
+
+
+def _addresses(shape, strides, dim):
+    """(rows, classes) offsets of the elements."""
+    at = np.zeros(shape, np.int64)
+    for i, (n, st) in enumerate(zip(shape, strides)):
+        at += (np.arange(n) * st).reshape([-1 if k == i else 1 for k in range(len(shape))])
+    return np.moveaxis(at, dim, -1).reshape(-1, shape[dim])
+
+
+def test_scores_and_gradient_are_walked_through_together():
+    """The kernels count the rows of both by one ``inner``: over random crops, steps, repeats and orders of the axes every score's
+    and every gradient's element is numpy's, and the gradient has a place for each."""
+    import torch
+
+    call = object.__new__(A._TorchCall)  # (its constructor asks for a stream)
+    call.torch = torch
+    rng = np.random.default_rng(12)
+    seen = set()
+    for turn in range(4000):
+        nd = int(rng.integers(1, 5))
+        shape = tuple(int(v) for v in rng.integers(1, 5, nd))
+        x = random_layout(rng, shape, lambda s: torch.zeros(s))
+        assert tuple(x.shape) == shape
+        dim = int(rng.integers(0, nd))
+        y, (_, rows) = x, A._rows_of(shape, x.stride(), dim)
+        if rows is None:  # as _tensor_logits
+            y = x.contiguous()
+            rows = A._rows_of(shape, y.stride(), dim)[1]
+        z, rows, g, grad_rows = call.grad_like(y, dim, rows)
+        assert g.shape == x.shape and g.dtype == x.dtype and rows.rows == grad_rows.rows and rows.classes == shape[dim]
+        n = np.arange(rows.rows)[:, None]
+        j = np.arange(rows.classes)[None]
+        for t, r in ((z, rows), (g, grad_rows)):
+            got = (n // rows.inner) * r.so + (n % rows.inner) * r.si + j * r.sc
+            assert np.array_equal(got, _addresses(shape, t.stride(), dim)), (shape, x.stride(), g.stride(), dim)
+        assert len(np.unique(_addresses(shape, g.stride(), dim))) == g.numel()
+        a = L.QmriLabelScoresArgs()
+        L._fill_logits(a, 0, "float32", rows, 1.0, False)
+        L._fill_grad(a, 0, grad_rows)  # (refuses rows counted differently)
+        seen.add((z is x, rows.inner == rows.rows, g.is_contiguous()))
+    assert len(seen) >= 6
+    a = L.QmriLabelScoresArgs()
+    L._fill_logits(a, 0, "float32", L.Rows(6, 4, 3, 100, 4, 1), 1.0, False)
+    with pytest.raises(ValueError, match="counted by"):
+        L._fill_grad(a, 0, L.Rows(6, 4))
+
+
+@pytest.mark.parametrize("shape, make, dim", [
+    ((2, 5, 7), lambda t: t[:, :-1], -1), ((2, 5, 7), lambda t: t[:, 1:], -1), ((2, 6, 5, 4), lambda t: t.permute(0, 3, 1, 2)[:, :, 1:-1, 2:], 1),
+    ((2, 6, 5, 4), lambda t: t.permute(0, 3, 1, 2)[:, :, :, 2:], 1), ((9, 8, 3, 4), lambda t: t[2:-2, 1:-1], -1), ((1, 4, 1), lambda t: t.expand(3, 4, 5), 1), ((3, 1, 6), lambda t: t.expand(3, 5, 6), 2),
+])
+def test_layouts_that_a_gradient_is_asked_for(shape, make, dim):
+    import torch
+
+    call = object.__new__(A._TorchCall)
+    call.torch = torch
+    x = make(torch.zeros(shape))
+    d = dim % x.ndim
+    rows = A._rows_of(x.shape, x.stride(), d)[1]
+    if rows is None:  # (cropped in H and in W of (B, H, W): three strides, copied before)
+        assert shape == (2, 6, 5, 4) and x.shape[2] == 4
+        x = x.contiguous()
+        rows = A._rows_of(x.shape, x.stride(), d)[1]
+    z, rows, g, grad_rows = call.grad_like(x, d, rows)
+    assert z is x  # no copy
+    n, j = np.arange(rows.rows)[:, None], np.arange(rows.classes)[None]
+    for t, r in ((x, rows), (g, grad_rows)):
+        assert np.array_equal((n // rows.inner) * r.so + (n % rows.inner) * r.si + j * r.sc, _addresses(tuple(x.shape), t.stride(), d))

@@ -552,6 +552,78 @@ def test_broadcast_and_many_stride_inputs():
     assert torch.equal(c.top_label, d.top_label) and torch.allclose(c.entropy, d.entropy, rtol=0, atol=100 * U)
 
 
+def _check_gradients_of(t, dim, rng):
+    """The gradients of both operators for a tensor as it lies, against the definitions on the values it holds."""
+    torch = torch_()
+    dim = dim % t.ndim
+    C = t.shape[dim]
+    z = _back(t, dim, C)
+    rows, shp = z.shape[0], _rowshape(t, dim)
+    dev = lambda v: torch.from_numpy(v).reshape(shp + list(v.shape[1:])).cuda()  # noqa: E731
+    lab = rng.integers(0, C, rows)
+    a, b = (rng.standard_normal(rows).astype(np.float32) for _ in range(2))
+    r = A.label_scores(t, dev(lab), dim=dim, norm=True)
+    g = A.label_scores_grad(t, dev(lab), r.norm, grad_log_prob=dev(a), entropy=r.entropy, grad_entropy=dev(b), dim=dim)
+    assert g.shape == t.shape and g.dtype == t.dtype
+    lp, _, ls = ao.log_softmax(z, 1.0)
+    name = str(t.dtype)[6:]
+    want = ao.scores_grad(z, 1.0, lab, a.astype(float), b.astype(float))
+    H, aa, bb = np.abs(ao.scores(z)["entropy"])[:, None], np.abs(a)[:, None], np.abs(b)[:, None]
+    # (as _check_scores_grad)
+    tol = _tol_g(want, lp, ls, aa + bb * (1 + H + np.abs(lp)), 1.0, name, C) + bb * np.exp(lp) * (_tol_h(lp, ls)[:, None] + 8 * U * np.abs(lp)) + 4 * U * aa
+    _same(_back(g, dim, C), want, tol, ("label_scores_grad", tuple(t.shape), t.stride(), dim))
+    K = min(3, C)
+    idx, val = _teacher(rng, rows, C, K, False, 1.0)
+    d = A.distill_loss(t, dev(idx), dev(val.numpy()), dim=dim, norm=True)
+    g = A.distill_loss_grad(t, dev(idx), dev(val.numpy()), d.norm, grad_loss=dev(a), dim=dim)
+    want = ao.distill(z, idx, val.double().numpy(), 1.0, False, a.astype(float))
+    # (as _check_distill without the tail)
+    tol = _tol_g(want["grad"], lp, ls, aa * 2, 1.0, name, C) + aa * (K + 16) * U * (np.exp(lp) + _inside(idx, C, want["q"]))
+    _same(_back(g, dim, C), want["grad"], tol, ("distill_loss_grad", tuple(t.shape), t.stride(), dim))
+
+
+@pytest.mark.parametrize("C", [4, 13, 100, 1500])
+def test_gradients_of_crops_repeats_and_orders_of_the_axes(C):
+    torch = torch_()
+    rng = np.random.default_rng(C + 77)
+    make = lambda s: torch.from_numpy(rng.standard_normal(s).astype(np.float32) * 2).cuda()  # noqa: E731
+    for t, dim in ((make((2, 9, C))[:, :-1], -1), (make((2, 9, C))[:, 1:], -1), (make((3, 7, 6, C)).permute(0, 3, 1, 2)[:, :, 1:-1, 2:], 1),
+                   (make((8, 7, 3, C))[2:-2, 1:-1], -1), (make((1, C, 1)).expand(3, C, 5), 1), (make((4, 1, C)).expand(4, 5, C), -1),
+                   (make((5, C)).expand(3, 5, C), -1), (make((2, C, 8, 9))[:, :, ::2, ::3], 1), (make((C, 3, 8)).permute(1, 0, 2)[:, :, 1:6], 1)):
+        _check_gradients_of(t, dim, rng)
+        _check_gradients_of(t.to(torch.bfloat16) if t.is_contiguous() else t.bfloat16(), dim, rng)
+
+
+def test_gradients_of_random_layouts():
+    from test_answers import random_layout
+
+    torch = torch_()
+    rng = np.random.default_rng(99)
+    for turn in range(60):
+        nd = int(rng.integers(2, 5))
+        shape = [int(v) for v in rng.integers(1, 7, nd)]
+        dim = int(rng.integers(0, nd))
+        shape[dim] = int(rng.choice([3, 8, 9, 40, 130]))
+        t = random_layout(rng, tuple(shape), lambda s: torch.from_numpy(rng.standard_normal(s).astype(np.float32) * 2).cuda())
+        _check_gradients_of(t, dim, rng)
+
+
+def test_backward_through_views():
+    """A next-token loss on ``logits[:, :-1]`` and a class prior repeated over the voxels."""
+    torch = torch_()
+    rng = np.random.default_rng(17)
+    z = torch.from_numpy(rng.standard_normal((2, 6, 50)).astype(np.float32)).cuda().requires_grad_()
+    tok = torch.from_numpy(rng.integers(0, 50, (2, 6))).cuda()
+    (-A.label_scores(z[:, :-1], tok[:, 1:]).log_prob.sum()).backward()
+    want = -ao.scores_grad(_host(z)[:, :-1].reshape(10, 50), 1.0, tok[:, 1:].cpu().numpy().reshape(-1), np.ones(10)).reshape(2, 5, 50)
+    assert np.all(_host(z.grad)[:, -1] == 0) and np.all(np.abs(_host(z.grad)[:, :-1] - want) < 200 * U)
+    bias = torch.from_numpy(rng.standard_normal(4).astype(np.float32)).cuda().requires_grad_()
+    lab = torch.from_numpy(rng.integers(0, 4, (3, 70))).cuda()
+    A.label_scores(bias.view(1, 4, 1).expand(3, 4, 70), lab, dim=1).log_prob.sum().backward()
+    want = ao.scores_grad(np.tile(_host(bias), (210, 1)), 1.0, lab.cpu().numpy().reshape(-1), np.ones(210)).sum(0)
+    assert np.all(np.abs(_host(bias.grad) - want) < 210 * 40 * U)  # (210 gradients, each within 40 u, summed in 32 bits)
+
+
 def test_nothing_is_written_outside_the_results():
     """The scores lie inside a larger array; the gradient's neighbours and the rows behind the last one stay as they were."""
     torch = torch_()
