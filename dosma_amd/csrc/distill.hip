@@ -426,7 +426,7 @@ struct StagedEntries {
         return s;
     }
 };
-inline size_t staged_bytes(int rows, int K) { return (size_t)rows * (K | 1) * 8; }
+constexpr size_t staged_bytes(int rows, int K) { return (size_t)rows * (K | 1) * 8; }
 template <int THREADS, typename L, typename V>
 __device__ __forceinline__ void stage_from(const StagedEntries &s, const L *labels, const V *values, int K, int all, long long left, int cats) {
     for (int i0 = threadIdx.x; i0 < all; i0 += 8 * THREADS) {  // (eight of each under way together)
@@ -1276,8 +1276,14 @@ void small_of(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
         default: return small<T, 8>(k, grad, num_cu, st);
     }
 }
+// The kernel's limit of LDS raised to what any call of it asks for: the limit is the kernel's, not the call's, and another thread's
+// call may come between this and the launch.
+template <int ROWS, typename F>
+hipError_t allow_staged(F *kernel) {
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)staged_bytes(ROWS, QMRI_MAX_TOP));
+}
 template <typename T, int G>
-void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
+hipError_t group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of((k.g.rows + 256 / G - 1) / (256 / G), num_cu, 64)), block(256);
     // up to 16 entries a row in registers, or 64 where a row has that many lanes; 256 / G rows of more in LDS (G 2: at most 65 KB)
     constexpr int E = G >= 16 ? 64 / G : 16 / G > 4 ? 4 : 16 / G;
@@ -1286,17 +1292,17 @@ void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
     if (k.K <= 2) {
         if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, -2>), grid, block, 0, st, k);
         else hipLaunchKernelGGL((distill_group_kernel<T, G, -2>), grid, block, 0, st, k);
-        return;
+        return hipSuccess;
     }
     if constexpr (G == 2) {
         if (k.K <= 4) {
             if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, -4>), grid, block, 0, st, k);
             else hipLaunchKernelGGL((distill_group_kernel<T, G, -4>), grid, block, 0, st, k);
-            return;
+            return hipSuccess;
         }
         if (k.K <= 8 && grad) {  // (20 classes, six entries: 183 us and 230)
             hipLaunchKernelGGL((distill_grad_group_kernel<T, G, -8>), grid, block, 0, st, k);
-            return;
+            return hipSuccess;
         }
     }
     if (k.K <= G * E) {
@@ -1306,13 +1312,15 @@ void group(const DistillK &k, bool grad, int num_cu, hipStream_t st) {
         }
     } else if constexpr (G < 16) {
         const size_t lds = staged_bytes(256 / G, k.K);
-        if (lds > 16 * 1024) {  // (the gradient has 25 KB of its own)
-            (void)hipFuncSetAttribute(reinterpret_cast<const void *>(distill_grad_group_kernel<T, G, 0>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            (void)hipFuncSetAttribute(reinterpret_cast<const void *>(distill_group_kernel<T, G, 0>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        // (the gradient has 25 KB of its own)
+        if (lds > 16 * 1024) {
+            const hipError_t e = grad ? allow_staged<256 / G>(distill_grad_group_kernel<T, G, 0>) : allow_staged<256 / G>(distill_group_kernel<T, G, 0>);
+            if (e != hipSuccess) return e;
         }
         if (grad) hipLaunchKernelGGL((distill_grad_group_kernel<T, G, 0>), grid, block, lds, st, k);
         else hipLaunchKernelGGL((distill_group_kernel<T, G, 0>), grid, block, lds, st, k);
     }
+    return hipSuccess;
 }
 template <typename T>
 void planes(const DistillK &k, int num_cu, hipStream_t st) {
@@ -1342,16 +1350,19 @@ void planes_grad(const DistillK &k, int num_cu, hipStream_t st) {
 }
 
 template <typename T>
-void launch(const DistillK &k, int num_cu, hipStream_t st) {
+hipError_t launch(const DistillK &k, int num_cu, hipStream_t st) {
     const LogitsK &g = k.g;
     const bool contig = contiguous(g);
-    if (g.C <= 8) return small_of<T>(k, false, num_cu, st);
+    if (g.C <= 8) {
+        small_of<T>(k, false, num_cu, st);
+        return hipSuccess;
+    }
     if (!contig) {
         if (lane_rows(g, num_cu))
             planes<T>(k, num_cu, st);
         else
             hipLaunchKernelGGL(distill_wave_kernel<T>, dim3(grid_of((g.rows + 3) / 4, num_cu, 32)), dim3(256), 0, st, k);
-        return;
+        return hipSuccess;
     }
     if (g.C <= 32) return group<T, 2>(k, false, num_cu, st);
     if (g.C <= 64) return group<T, 4>(k, false, num_cu, st);
@@ -1373,15 +1384,20 @@ void launch(const DistillK &k, int num_cu, hipStream_t st) {
         else hipLaunchKernelGGL((distill_block_kernel<T, false, 4>), grid, dim3(256), 0, st, k, cut);
     }
     if (cut.segs > 1) hipLaunchKernelGGL(distill_join_kernel<T>, dim3(grid_of(g.rows, num_cu, 64)), dim3(64), 0, st, k, cut);
+    return hipSuccess;
 }
 
 template <typename T>
-void launch_grad(const DistillK &k, int num_cu, hipStream_t st) {
+hipError_t launch_grad(const DistillK &k, int num_cu, hipStream_t st) {
     const LogitsK &g = k.g;
     const bool contig = contiguous(g) && (k.gsc == 1 || g.C == 1);
-    if (g.C <= 8) return small_of<T>(k, true, num_cu, st);
+    if (g.C <= 8) {
+        small_of<T>(k, true, num_cu, st);
+        return hipSuccess;
+    }
     if (!contig) {
-        return planes_grad<T>(k, num_cu, st);
+        planes_grad<T>(k, num_cu, st);
+        return hipSuccess;
     }
     if (g.C <= 32) return group<T, 2>(k, true, num_cu, st);
     if (g.C <= 64) return group<T, 4>(k, true, num_cu, st);
@@ -1399,6 +1415,7 @@ void launch_grad(const DistillK &k, int num_cu, hipStream_t st) {
     const dim3 grid(grid_of(g.rows * cut.segs, num_cu, 64));
     if (wave_rows_grad<T>(g, num_cu)) hipLaunchKernelGGL((distill_grad_block_kernel<T, 1>), grid, dim3(64), 0, st, k, cut);
     else hipLaunchKernelGGL((distill_grad_block_kernel<T, 4>), grid, dim3(256), 0, st, k, cut);
+    return hipSuccess;
 }
 
 }  // namespace
@@ -1411,18 +1428,16 @@ size_t distill_workspace_bytes(const DistillK &k, int, int num_cu) {
 
 hipError_t distill_launch(const DistillK &k, int dtype, int num_cu, hipStream_t st) {
     (void)hipGetLastError();
-    if (dtype == QMRI_F32) launch<float>(k, num_cu, st);
-    else if (dtype == QMRI_F16) launch<f16_t>(k, num_cu, st);
-    else launch<bf16_t>(k, num_cu, st);
-    return hipGetLastError();
+    const hipError_t e = dtype == QMRI_F32 ? launch<float>(k, num_cu, st) : dtype == QMRI_F16 ? launch<f16_t>(k, num_cu, st) : launch<bf16_t>(k, num_cu, st);
+    const hipError_t last = hipGetLastError();  // (cleared in either case)
+    return e != hipSuccess ? e : last;
 }
 
 hipError_t distill_grad_launch(const DistillK &k, int dtype, int num_cu, hipStream_t st) {
     (void)hipGetLastError();
-    if (dtype == QMRI_F32) launch_grad<float>(k, num_cu, st);
-    else if (dtype == QMRI_F16) launch_grad<f16_t>(k, num_cu, st);
-    else launch_grad<bf16_t>(k, num_cu, st);
-    return hipGetLastError();
+    const hipError_t e = dtype == QMRI_F32 ? launch_grad<float>(k, num_cu, st) : dtype == QMRI_F16 ? launch_grad<f16_t>(k, num_cu, st) : launch_grad<bf16_t>(k, num_cu, st);
+    const hipError_t last = hipGetLastError();  // (cleared in either case)
+    return e != hipSuccess ? e : last;
 }
 
 }  // namespace qmri

@@ -904,6 +904,42 @@ def test_many_answers_captured_and_replayed(layout):
     assert np.all(np.abs(g - ref["grad"]) < (K + 16) * U * 4)
 
 
+def test_threads_with_few_and_many_answers():
+    """Calls of one kernel from several threads at once, with different amounts of LDS: the limit is the kernel's, not the call's."""
+    import threading
+
+    torch = torch_()
+    C, rows = 20, 900
+    z = torch.randn(rows, C, device="cuda")
+    sets = []
+    for K in (9, 17, 33, 64):
+        idx = torch.randint(0, C, (rows, K), device="cuda", dtype=torch.int32)
+        val = torch.randn(rows, K, device="cuda")
+        d = A.distill_loss(z, idx, val, norm=True)
+        g = A.distill_loss_grad(z, idx, val, d.norm, grad_loss=torch.ones(rows, device="cuda"))
+        sets.append((idx, val, d, g))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(idx, val, d, g):
+        try:
+            one = torch.ones(rows, device="cuda")
+            for _ in range(100):
+                now = A.distill_loss(z, idx, val, norm=True)
+                grad = A.distill_loss_grad(z, idx, val, now.norm, grad_loss=one)
+            torch.cuda.synchronize()
+            assert torch.equal(now.loss, d.loss) and torch.equal(grad, g)
+        except Exception as e:  # (a thread's own exceptions reach nobody)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=s) for s in sets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
 def test_the_same_bits_every_time():
     torch = torch_()
     for shape, bg in (((5, 100003), False), ((30000, 4), True), ((900, 900), False)):
