@@ -16,7 +16,8 @@ A score of -inf is a category that is not offered: probability 0, never an alter
 probability -inf, entropy 0, no alternatives, loss 0 and gradient 0.  NaN or +inf makes the row's results NaN.
 
 Calls on tensors can be captured into a graph, their gradients as well; as with every backward pass in torch, no eager graph of
-the same leaves may be alive while one is captured (a leaf's accumulation stays on the stream that it was first used on)."""
+the same leaves may be alive while one is captured (a leaf's accumulation stays on the stream that it was first used on).  Derivatives are reverse mode and first order; tensors
+with a forward-mode tangent are refused."""
 import sys
 from collections import namedtuple
 
@@ -95,12 +96,20 @@ def _name(dtype):
     return name
 
 
+def _no_tangent(name, t):
+    # (a dual tensor does not require gradients, so the derivative asked for would come back as none, which reads as zero)
+    ad = sys.modules["torch"].autograd.forward_ad
+    if getattr(ad, "_current_level", 0) >= 0 and ad.unpack_dual(t).tangent is not None:  # (the level: a tenth of the time of the question)
+        raise ValueError(f"{name}: forward-mode derivatives are not offered")
+
+
 def _tensor_logits(x, dim):
     """-> (scores, axis, shape of the rows, Rows); a copy of the scores where their rows need more than two strides."""
     if not x.is_cuda:
         raise ValueError("logits must be a tensor on the GPU or a numpy array")
     if _name(x.dtype) not in _lib.SCORE_DTYPES:
         raise ValueError(f"logits must be float32, float16 or bfloat16, got {x.dtype}")
+    _no_tangent("logits", x)
     ndim = x.ndim
     dim = _check_dim(ndim, dim)
     if dim == ndim - 1 and x.is_contiguous():
@@ -123,6 +132,8 @@ def _tensor_arg(name, t, shape, device, dtypes, last=()):
         raise ValueError(f"{name} is on {t.device}, the logits are on {device}")
     if _name(t.dtype) not in dtypes:
         raise ValueError(f"{name} must be one of {', '.join(sorted(dtypes))}, got {t.dtype}")
+    if t.is_floating_point():
+        _no_tangent(name, t)
     return t if t.is_contiguous() else t.contiguous()
 
 

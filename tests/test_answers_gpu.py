@@ -993,6 +993,26 @@ def test_empty_tensors():
     assert d.loss.shape == (0,)
 
 
+def test_forward_mode_is_refused():
+    """A dual tensor does not require gradients: without the refusal its tangent would be lost without a word."""
+    torch = torch_()
+    fw = torch.autograd.forward_ad
+    z, one = torch.randn(3, 4, device="cuda"), torch.ones(3, device="cuda")
+    lab, idx, val = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, 2, dtype=torch.int32, device="cuda"), torch.zeros(3, 2, device="cuda")
+    s, d = A.label_scores(z, lab, norm=True), A.distill_loss(z, idx, val, norm=True)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: A.label_scores(dual(z), lab), lambda: A.label_scores(dual(z)), lambda: A.distill_loss(dual(z), idx, val),
+                     lambda: A.distill_loss(z, idx, dual(val)), lambda: A.label_scores_grad(dual(z), lab, s.norm, grad_log_prob=one),
+                     lambda: A.label_scores_grad(z, lab, dual(s.norm), grad_log_prob=one),
+                     lambda: A.label_scores_grad(z, lab, s.norm, grad_log_prob=dual(one)),
+                     lambda: A.distill_loss_grad(z, idx, val, d.norm, grad_loss=dual(one))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        # a primal inside the level is an ordinary tensor
+        assert torch.equal(A.label_scores(z, lab).log_prob, s.log_prob)
+
+
 def test_refusals_on_tensors():
     torch = torch_()
     z = torch.zeros(3, 4, device="cuda")
