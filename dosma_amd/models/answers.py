@@ -110,6 +110,8 @@ def _tensor_logits(x, dim):
     if _name(x.dtype) not in _lib.SCORE_DTYPES:
         raise ValueError(f"logits must be float32, float16 or bfloat16, got {x.dtype}")
     _no_tangent("logits", x)
+    if x.is_neg():  # (``c.conj().imag``: the memory holds the values with the other sign)
+        x = x.resolve_neg()
     ndim = x.ndim
     dim = _check_dim(ndim, dim)
     if dim == ndim - 1 and x.is_contiguous():
@@ -134,6 +136,8 @@ def _tensor_arg(name, t, shape, device, dtypes, last=()):
         raise ValueError(f"{name} must be one of {', '.join(sorted(dtypes))}, got {t.dtype}")
     if t.is_floating_point():
         _no_tangent(name, t)
+        if t.is_neg():
+            t = t.resolve_neg()
     return t if t.is_contiguous() else t.contiguous()
 
 

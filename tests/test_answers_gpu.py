@@ -993,6 +993,35 @@ def test_empty_tensors():
     assert d.loss.shape == (0,)
 
 
+def test_views_whose_memory_has_the_other_sign():
+    """The imaginary part of a conjugate is a view that torch negates when it is read."""
+    torch = torch_()
+    neg = lambda *s: torch.view_as_complex(torch.randn(*s, 2, device="cuda")).conj().imag  # noqa: E731
+    for shape, dim in (((5, 6), -1), ((2, 40, 3), 1), ((3, 2000), -1)):
+        z = neg(*shape)
+        plain = z.resolve_neg().contiguous()
+        assert z.is_neg() and not plain.is_neg()
+        d = dim % len(shape)
+        rows = list(shape[:d] + shape[d + 1:])
+        lab = torch.zeros(rows, dtype=torch.int64, device="cuda")
+        a, b = A.label_scores(z, lab, dim=dim, top=2, norm=True), A.label_scores(plain, lab, dim=dim, top=2, norm=True)
+        assert torch.equal(a.top_label, b.top_label) and torch.allclose(a.log_prob, b.log_prob, rtol=0, atol=100 * U)
+        w = neg(*rows)
+        kw = dict(entropy=b.entropy, dim=dim)
+        g = A.label_scores_grad(z, lab, b.norm, grad_log_prob=w, grad_entropy=w, **kw)
+        h = A.label_scores_grad(plain, lab, b.norm, grad_log_prob=w.resolve_neg(), grad_entropy=w.resolve_neg(), **kw)
+        assert not g.is_neg() and torch.allclose(g, h, rtol=0, atol=100 * U)
+        idx, val = torch.zeros(rows + [2], dtype=torch.int32, device="cuda"), neg(*rows, 2)
+        idx[..., 1] = 1
+        assert torch.allclose(A.distill_loss(z, idx, val, dim=dim).loss, A.distill_loss(plain, idx, val.resolve_neg(), dim=dim).loss,
+                              rtol=0, atol=200 * U)
+        c = torch.view_as_complex(torch.randn(*shape, 2, device="cuda")).requires_grad_()
+        A.label_scores(c.conj().imag, lab, dim=dim).entropy.sum().backward()
+        x = (-c.detach().imag).contiguous().requires_grad_()
+        A.label_scores(x, lab, dim=dim).entropy.sum().backward()
+        assert torch.allclose(c.grad.imag, -x.grad, rtol=0, atol=100 * U)
+
+
 def test_forward_mode_is_refused():
     """A dual tensor does not require gradients: without the refusal its tangent would be lost without a word."""
     torch = torch_()
