@@ -335,7 +335,7 @@ def _array_logits(x, dim):
 
 
 def _array_arg(name, a, shape, dtypes, last=None):
-    a = np.ascontiguousarray(a)
+    a = np.asarray(a, order="C")  # (one row: no axis; ascontiguousarray would add one)
     want = tuple(shape) + (() if last is None else (last,))
     if a.shape != want:
         raise ValueError(f"{name} has shape {a.shape}, expected {want}")

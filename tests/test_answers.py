@@ -306,3 +306,14 @@ def test_layouts_that_a_gradient_is_asked_for(shape, make, dim):
     n, j = np.arange(rows.rows)[:, None], np.arange(rows.classes)[None]
     for t, r in ((x, rows), (g, grad_rows)):
         assert np.array_equal((n // rows.inner) * r.so + (n % rows.inner) * r.si + j * r.sc, _addresses(tuple(x.shape), t.stride(), d))
+
+
+def test_a_single_rows_arguments_have_no_axis():
+    for label in (2, np.int32(2), np.array(2, np.uint8)):
+        a = A._array_arg("labels", label, (), L.L_KINDS)
+        assert a.shape == () and a == 2
+    assert A._array_arg("norm", np.zeros(2, np.float32), (), ("float32",), 2).shape == (2,)
+    with pytest.raises(ValueError, match="labels has shape"):
+        A._array_arg("labels", np.zeros(1, np.int32), (), L.L_KINDS)
+    t = np.arange(6, dtype=np.int32).reshape(2, 3).T
+    assert A._array_arg("labels", t, (3, 2), L.L_KINDS).flags.c_contiguous

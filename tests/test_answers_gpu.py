@@ -982,6 +982,30 @@ def test_numpy_arrays():
     assert empty.log_prob.shape == (0,) and empty.top_label.shape == (0, 2)
 
 
+def test_one_row_without_an_axis():
+    """(C,) scores: the row's arguments and results have no axis, as tensors and as arrays."""
+    torch = torch_()
+    rng = np.random.default_rng(6)
+    for C in (4, 700):
+        z = rng.standard_normal(C).astype(np.float32)
+        idx, val = np.array([1, 0], np.int32), np.zeros(2, np.float32)
+        want, wd = ao.scores(z[None].astype(float), 1.0, np.array([2]), 3), ao.distill(z[None].astype(float), idx[None], val[None], w=np.ones(1))
+        g_want = ao.scores_grad(z[None].astype(float), 1.0, np.array([2]), np.ones(1))[0]
+        one = np.float32(1.0)
+        for conv in (lambda v: v, lambda v: torch.from_numpy(np.asarray(v)).cuda()):
+            back = lambda v: v if isinstance(v, np.ndarray) else _host(v)  # noqa: E731
+            r = A.label_scores(conv(z), conv(np.int64(2)), top=3, norm=True)
+            assert r.log_prob.shape == () and r.entropy.shape == () and r.norm.shape == (2,) and r.top_label.shape == (3,)
+            _same(back(r.log_prob), want["log_prob"][0], 100 * U)
+            assert np.array_equal(back(r.top_label), want["top_label"][0])
+            g = A.label_scores_grad(conv(z), conv(np.int64(2)), r.norm, grad_log_prob=conv(one))
+            _same(back(g), g_want, 100 * U)
+            d = A.distill_loss(conv(z), conv(idx), conv(val), norm=True)
+            assert d.loss.shape == ()
+            _same(back(d.loss), wd["loss"][0], 100 * U)
+            _same(back(A.distill_loss_grad(conv(z), conv(idx), conv(val), d.norm, grad_loss=conv(one))), wd["grad"][0], 100 * U)
+
+
 def test_empty_tensors():
     torch = torch_()
     z = torch.zeros((0, 4), device="cuda", requires_grad=True)
