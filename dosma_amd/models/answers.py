@@ -335,7 +335,8 @@ def _array_logits(x, dim):
 
 
 def _array_arg(name, a, shape, dtypes, last=None):
-    a = np.asarray(a, order="C")  # (one row: no axis; ascontiguousarray would add one)
+    a = np.asarray(a)
+    a = np.asarray(a, dtype=a.dtype.newbyteorder("="), order="C")  # (one row: no axis; ascontiguousarray would add one)
     want = tuple(shape) + (() if last is None else (last,))
     if a.shape != want:
         raise ValueError(f"{name} has shape {a.shape}, expected {want}")
@@ -412,7 +413,7 @@ def _teacher_arrays(top_label, values, shape, tail):
     top_label = np.asarray(top_label)
     K = top_label.shape[-1] if top_label.ndim else 0
     values = np.asarray(values)
-    if values.dtype == np.float64:
+    if values.dtype.name == "float64":  # (of either byte order)
         values = values.astype(np.float32)
     return _array_arg("top_label", top_label, shape, ("int32", "int64"), K), _array_arg("values", values, shape, _lib.SCORE_DTYPES, K), K
 

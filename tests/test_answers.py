@@ -317,3 +317,17 @@ def test_a_single_rows_arguments_have_no_axis():
         A._array_arg("labels", np.zeros(1, np.int32), (), L.L_KINDS)
     t = np.arange(6, dtype=np.int32).reshape(2, 3).T
     assert A._array_arg("labels", t, (3, 2), L.L_KINDS).flags.c_contiguous
+
+
+def test_arrays_of_the_other_byte_order():
+    """As files hold them (big-endian label volumes): the type's name is the same, the bytes are not."""
+    lab = np.array([0, 1, 2], np.int32)
+    for t in (">i4", ">i2", ">i8", "<i4", "u1"):
+        a = A._array_arg("labels", lab.astype(t), (3,), L.L_KINDS)
+        assert a.dtype.isnative and np.array_equal(a, lab) and np.array_equal(np.frombuffer(a.tobytes(), a.dtype.name), lab)
+    for t in (">f4", ">f2", ">f8", "f8", "f4"):
+        _, v, _ = A._teacher_arrays(lab[:, None], np.array([[0.5], [-2.0], [7.0]]).astype(t), (3,), False)
+        assert v.dtype.isnative and v.dtype.itemsize < 8 and np.array_equal(v[:, 0], [0.5, -2.0, 7.0])
+    for t in (">f4", ">f2", ">f8"):
+        x, _, _, _ = A._array_logits(np.array([[0.5, -2.0]]).astype(t), -1)
+        assert x.dtype.isnative and np.array_equal(x[0], [0.5, -2.0])
