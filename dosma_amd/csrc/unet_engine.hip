@@ -1207,6 +1207,15 @@ static hipError_t load_batch(Unet *U, const float *src, long long count, hipStre
     return qmri::scale_copy_launch(src, count, std::ldexp(1.f, -U->act_shift), U->in.as<float>(), st);
 }
 
+// The volume buffer for n voxels.  An allocation that fails has given the old buffer back: none is there until the next one succeeds.
+static hipError_t grow_volume(Unet *U, long long n) {
+    if (U->vol_cap >= n) return hipSuccess;
+    U->vol_cap = 0;
+    const hipError_t e = U->vol.alloc((size_t)n * 4);
+    if (e == hipSuccess) U->vol_cap = n;
+    return e;
+}
+
 extern "C" {
 
 int qmri_unet2d_forward(void *handle, const float *x, int32_t S, int32_t x_on_device, int32_t whiten,
@@ -1224,10 +1233,7 @@ int qmri_unet2d_forward(void *handle, const float *x, int32_t S, int32_t x_on_de
     // the volume on the device (whitening needs whole-volume statistics, seg_model.py:127)
     const float *xd = x;
     if (!x_on_device || whiten) {
-        if (U->vol_cap < n) {
-            U_TRY(U->vol.alloc((size_t)n * 4));
-            U->vol_cap = n;
-        }
+        U_TRY(grow_volume(U, n));
         if (!x_on_device) {
             U_TRY(hipMemcpyAsync(U->vol.p, x, (size_t)n * 4, hipMemcpyHostToDevice, st));
             xd = U->vol.as<float>();
@@ -1292,15 +1298,13 @@ int qmri_unet2d_segment_volume(void *handle, const float *vol_hws, int32_t S, in
     const long long P = (long long)U->H * U->W;
     const long long n = (long long)S * P;
     if (U->seg_cap < n) {
+        U->seg_cap = 0;  // (as in grow_volume)
         U_TRY(U->vol_in.alloc((size_t)n * 4));
         U_TRY(U->mask_all.alloc((size_t)n * 4));  // 4 bytes per pixel (classes padded to 4)
         U_TRY(U->mask_planes.alloc((size_t)n * U->ncls));
         U->seg_cap = n;
     }
-    if (U->vol_cap < n) {
-        U_TRY(U->vol.alloc((size_t)n * 4));
-        U->vol_cap = n;
-    }
+    U_TRY(grow_volume(U, n));
     U_TRY(hipMemcpyAsync(U->vol_in.p, vol_hws, (size_t)n * 4, hipMemcpyHostToDevice, st));
     U_TRY(qmri::transpose_ps_launch(U->vol_in.as<float>(), P, S, U->vol.as<float>(), st));
     if (whiten) U_TRY(qmri::whiten_launch(U->vol.as<float>(), n, whiten_eps, U->stats.as<double>(), U->vol.as<float>(), st));
@@ -1386,10 +1390,7 @@ int qmri_unet2d_score_volume(void *handle, const qmri_unet2d_score_args *a) {
         U_TRY(hipMemcpyAsync(planes.p, a->teacher_log_prob, (size_t)n * E * 4, hipMemcpyHostToDevice, st));
         U_TRY(qmri::planes_to_rows_launch(planes.p, 0, P, S, E, ev.p, st));
     }
-    if (U->vol_cap < n) {
-        U_TRY(U->vol.alloc((size_t)n * 4));
-        U->vol_cap = n;
-    }
+    U_TRY(grow_volume(U, n));
     U_TRY(hipMemcpyAsync(planes.p, a->vol_hws, (size_t)n * 4, hipMemcpyHostToDevice, st));
     U_TRY(qmri::transpose_ps_launch(planes.as<float>(), P, S, U->vol.as<float>(), st));
     if (a->whiten) U_TRY(qmri::whiten_launch(U->vol.as<float>(), n, a->whiten_eps, U->stats.as<double>(), U->vol.as<float>(), st));

@@ -119,3 +119,21 @@ def test_engine_refusals(weights):
     empty = eng.score_volume(np.zeros((64, 32, 0), np.float32), top=1)
     assert empty["top_label"].shape == (1, 64, 32, 0)
     assert L.load().qmri_unet2d_score_volume(None, None) == L.QMRI_ERR_ARG
+
+
+def test_a_volume_too_large_for_the_memory_leaves_the_model_usable(weights):
+    """The allocation is refused (17 TB, nothing is read), and the next volume finds its buffers."""
+    m = IWOAIOAIUnet2DNormalized((64, 32, 1), weights, force_weights=True)
+    eng, v = m.seg_model, volume(3)
+    first = m.generate_scores(v, top=2)
+    mask = m.generate_mask(v)["fc"].volume
+    import torch
+
+    x = torch.zeros((1, 64, 32), device="cuda")
+    for _ in range(2):
+        with pytest.raises(L.QmriError):
+            eng.forward_device(x.data_ptr(), 2 ** 31 - 1, None, None, whiten=True)
+        again = m.generate_scores(v, top=2)
+        assert np.array_equal(again.entropy.volume, first.entropy.volume)
+        assert np.array_equal(again.top_labels[1].volume, first.top_labels[1].volume)
+        assert np.array_equal(m.generate_mask(v)["fc"].volume, mask)
