@@ -11,13 +11,17 @@ exporting buffer object), so callers own their results exactly as before; nothin
 free list plus blocks still owned by live results (pinned memory cannot be swapped); beyond it ``empty()`` hands out plain
 numpy arrays.  ``DOSMA_AMD_HOST_POOL=0`` switches the pool off as well.
 
-Fork: ROCm maps page-locked allocations so that a ``fork()``ed child does not inherit them; the library re-enables
-inheritance on every block (``qmri_host_alloc``: ``madvise(MADV_DOFORK)``), so a ``multiprocessing`` worker forked while
-results are alive can still READ them (tests/test_hostpool.py::test_forked_child_reads_a_pooled_result); a child never
-frees or recycles the parent's blocks.
+Fork: ROCm maps page-locked allocations so that a ``fork()``ed child does not inherit them.  Blocks of ordinary memory are made
+inheritable again by the library (``qmri_host_alloc``: ``madvise(MADV_DOFORK)``).  Where the runtime maps them from the device's
+file instead (``HSA_USERPTR_FOR_PAGED_MEM=0``) the kernel refuses that for the mapping's kind (EINVAL), and nothing lies at the
+block's address in the child: then ``os.fork`` puts an ordinary copy of every block that a live result holds there (the copy is
+made before the fork, of live blocks only; the parent keeps none of it).  Either way a ``multiprocessing`` worker forked while
+results are alive can READ them (tests/test_hostpool.py::test_forked_child_reads_a_pooled_result); a child never frees or recycles
+the parent's blocks.
 """
 import atexit
 import ctypes
+import gc
 import os
 import threading
 import weakref
@@ -33,6 +37,59 @@ _cached = 0                 # bytes on the free list
 _live = 0                   # bytes handed out and not yet released
 _closed = False
 _pid = os.getpid()          # blocks belong to the process that allocated them (a forked worker never frees or reuses them)
+_held = {}                  # blocks of live results: pointer -> bytes
+_apart = set()              # blocks a forked child does not inherit
+_copies = []                # during a fork: (block, its copy, bytes)
+
+# <sys/mman.h> of Linux
+_PROT_RW, _MAP_PRIVATE_ANON, _MREMAP_MOVE_FIXED, _MADV_DOFORK = 0x3, 0x22, 0x3, 11
+_libc = ctypes.CDLL(None, use_errno=True)
+_libc.mmap.restype = ctypes.c_void_p
+_libc.mmap.argtypes = [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_long]
+_libc.munmap.argtypes = [ctypes.c_void_p, ctypes.c_size_t]
+_libc.mremap.restype = ctypes.c_void_p
+_libc.mremap.argtypes = [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p]
+_libc.madvise.argtypes = [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int]
+
+
+def _inherited(ptr, size):
+    """Whether a forked child has the block (asked after the library has tried to make it so)."""
+    return _libc.madvise(ptr, size, _MADV_DOFORK) == 0
+
+
+def _before_fork():
+    _lock.acquire()  # (no other thread gives a block back, or takes one, before the child has its copies)
+    if _closed or os.getpid() != _pid or not _apart:
+        return
+    collects = gc.isenabled()
+    gc.disable()         # (nor does a finalizer on this one)
+    try:
+        for ptr, size in _held.items():
+            if ptr in _apart:
+                to = _libc.mmap(None, size, _PROT_RW, _MAP_PRIVATE_ANON, -1, 0)
+                if to not in (None, ctypes.c_void_p(-1).value):  # (no memory for it: the child is without this block)
+                    ctypes.memmove(to, ptr, size)
+                    _copies.append((ptr, to, size))
+    finally:
+        if collects:
+            gc.enable()
+
+
+def _after_fork_parent():
+    while _copies:
+        _, to, size = _copies.pop()
+        _libc.munmap(to, size)
+    _lock.release()
+
+
+def _after_fork_child():
+    while _copies:
+        ptr, to, size = _copies.pop()
+        _libc.mremap(to, size, size, _MREMAP_MOVE_FIXED, ptr)  # (the pages move, no second copy)
+    _lock.release()
+
+
+os.register_at_fork(before=_before_fork, after_in_parent=_after_fork_parent, after_in_child=_after_fork_child)
 
 
 def _cap():
@@ -49,6 +106,7 @@ def _release(ptr, size):
     cap = _cap()
     with _lock:
         _live -= size
+        _held.pop(ptr, None)
         if _cached + _live + size <= cap:
             lst = _free.get(size)
             if lst is None:
@@ -58,6 +116,7 @@ def _release(ptr, size):
             return
     try:
         from dosma_amd import _lib
+        _apart.discard(ptr)
         _lib.load().qmri_host_free(ctypes.c_void_p(ptr))
     except Exception:       # pragma: no cover - nothing sensible to do in a finalizer
         pass
@@ -108,10 +167,13 @@ def empty(shape, dtype):
             lib = _lib.load()
             out = ctypes.c_void_p()
             while drop:
+                _apart.discard(drop[-1][1])
                 lib.qmri_host_free(ctypes.c_void_p(drop[-1][1]))
                 drop.pop()
             if lib.qmri_device_count() > 0 and lib.qmri_host_alloc(size, ctypes.byref(out)) == 0 and out.value:
                 ptr = out.value
+                if not _inherited(ptr, size):
+                    _apart.add(ptr)
         except Exception:
             ptr = None
         if ptr is None:
@@ -121,6 +183,8 @@ def empty(shape, dtype):
                     _free.setdefault(sz, []).append(p)
                     _cached += sz
             return np.empty(shape, dt)
+    with _lock:
+        _held[ptr] = size
     buf = (ctypes.c_ubyte * size).from_address(ptr)
     fin = weakref.finalize(buf, _release, ptr, size)
     fin.atexit = False  # nothing to recycle at interpreter exit (and no HIP call from an exit handler or a forked child)
@@ -139,6 +203,7 @@ def trim():
         from dosma_amd import _lib
         lib = _lib.load()
         for p, _ in blocks:
+            _apart.discard(p)
             lib.qmri_host_free(ctypes.c_void_p(p))
 
 

@@ -316,8 +316,9 @@ int qmri_host_alloc(uint64_t bytes, void **out) {
     // ROCm marks page-locked host allocations MADV_DONTFORK: a fork()ed child (a multiprocessing worker -- the reference's own
     // parallelism, dosma/core/fitting.py:860-868) that touches a result array it inherited would fault.  Results handed to
     // Python live in these blocks (dosma_amd/_hostpool.py), so inheritance is switched back on: the child gets ordinary
-    // copy-on-write pages of the parent's data (it never owns, frees or DMA-targets the block).  Best effort: a platform that
-    // refuses leaves the block as the runtime made it.
+    // copy-on-write pages of the parent's data (it never owns, frees or DMA-targets the block).  Best effort: where the
+    // runtime maps the block from the device's file the kernel refuses (EINVAL) and the block stays as it is; the pool then gives
+    // the child a copy.
     const uintptr_t a0 = reinterpret_cast<uintptr_t>(*out) & ~(uintptr_t)4095;
     const uintptr_t a1 = (reinterpret_cast<uintptr_t>(*out) + bytes + 4095) & ~(uintptr_t)4095;
     (void)madvise(reinterpret_cast<void *>(a0), (size_t)(a1 - a0), MADV_DOFORK);

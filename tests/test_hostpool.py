@@ -17,6 +17,70 @@ def test_small_or_gpu_less_requests_are_plain_numpy():
         assert b.shape == (1 << 20,) and _hostpool.cached_bytes() == 0
 
 
+class _AnonymousBlocks:
+    """The library's allocator for a test without a GPU: memory that a forked child does not inherit, as ROCm maps it."""
+
+    def __init__(self):
+        self.live = {}
+
+    def qmri_device_count(self):
+        return 1
+
+    def qmri_host_alloc(self, size, out):
+        p = _hostpool._libc.mmap(None, size, 3, 0x22, -1, 0)
+        assert _hostpool._libc.madvise(p, size, 10) == 0  # MADV_DONTFORK
+        self.live[p] = size
+        out._obj.value = p
+        return 0
+
+    def qmri_host_free(self, p):
+        assert _hostpool._libc.munmap(p, self.live.pop(p.value)) == 0
+
+
+@pytest.mark.parametrize("refused", [False, True])
+def test_a_forked_child_reads_results_it_does_not_inherit(monkeypatch, refused):
+    """``refused``: the kernel does not make the blocks inheritable (a mapping of the device's file): os.fork brings copies."""
+    import os
+
+    from dosma_amd import _lib
+
+    lib = _AnonymousBlocks()
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    if refused:
+        monkeypatch.setattr(_hostpool, "_inherited", lambda ptr, size: False)
+    _hostpool.trim()
+    a, b = _hostpool.empty(300_000, np.float64), _hostpool.empty((1000, 600), np.float32)
+    gone = _hostpool.empty(1 << 20, np.float64)
+    a[:], b[:], gone[:] = np.arange(a.size), 7.0, 1.0
+    del gone  # (back on the free list: nobody reads it)
+    gc.collect()
+    mapped = len(lib.live)
+    pid = os.fork()
+    if pid == 0:
+        code = 3
+        try:
+            ok = np.array_equal(a, np.arange(a.size)) and bool((b == 7.0).all())
+            a[0] = -1.0                # the child's own pages
+            grandchild = os.fork()     # its children inherit them as ordinary memory
+            if grandchild == 0:
+                os._exit(0 if a[0] == -1.0 and a[5] == 5.0 else 1)
+            _, status = os.waitpid(grandchild, 0)
+            c = _hostpool.empty(1 << 20, np.float64)  # no block of the parent's
+            c[:] = 0.0
+            del a, b, c
+            gc.collect()
+            code = 0 if ok and status == 0 else 2
+        finally:
+            os._exit(code)
+    _, status = os.waitpid(pid, 0)
+    assert os.WIFEXITED(status) and os.WEXITSTATUS(status) == 0, f"child status {status:#x}"
+    assert a[0] == 0.0 and len(lib.live) == mapped and not _hostpool._copies
+    del a, b
+    gc.collect()
+    _hostpool.trim()
+    assert not lib.live and not _hostpool._held and not _hostpool._apart and _hostpool.cached_bytes() == 0
+
+
 @pytest.mark.gpu
 def test_results_are_owned_by_the_caller_and_blocks_are_recycled():
     import dosma_amd as dm
