@@ -594,7 +594,7 @@ __global__ __launch_bounds__(256) void scores_join_kernel(const ScoresK k, const
                 const float *a = p + sg * words + 4;
                 // (a segment that offers fewer than k has empty slots behind its last: they are no pairs)
                 const int id = q < pairs ? reinterpret_cast<const int *>(a)[k.top + at] : -1;
-                b.take<BITS>(id >= 0 ? a[at] : kNegInf, id, id >= 0);
+                b.take<BITS>(q < pairs ? a[at] : kNegInf, id, id >= 0);
             }
             if (b.n > 64) b.cut<BITS>();
             for (int q = b.n + lane; q < 64; q += 64) b.i[q] = -1;
