@@ -2,7 +2,7 @@
 
 The reference returns freshly allocated numpy arrays (``dosma/core/fitting.py:205-215``: ``np.full`` + scatter).  On the
 GPU path a fresh 0.7 GB result costs more than the fit: the operating system zero-fills every page on first touch
-(65 ms per GB on the benchmark host, DESIGN.md section 10) and the download has to go through a staging buffer.  Here large
+(65 ms per GB on the benchmark host) and the download has to go through a staging buffer.  Here large
 results live in ``hipHostMalloc`` memory handed out by ``empty()``: the pages are resident and the copy is a true DMA.  A
 block goes back to the free list when the last numpy view of it is garbage-collected (a ``weakref`` finalizer on the
 exporting buffer object), so callers own their results exactly as before; nothing is ever overwritten under them.

@@ -441,10 +441,10 @@ struct Cut {
     int segs, len;
 };
 Cut cut_rows(const LogitsK &g, int num_cu, int longest);
-// Classes that do not lie together: a lane a row as soon as the rows give every compute unit half a wave, below that a wave a row (kernel
+// Classes that do not lie together: a lane a row as soon as every compute unit has 32 rows (half a wave), below that a wave a row (kernel
 // times in f16, wave and lane: 200 classes 1000 rows 3.6 and 10.1 us, 8000 rows 7.4 and 10.3, 16000 rows 15.8 and 10.3; with the three
-// best 7.3 and 14.1, 18.7 and 14.4, 31.2 and 14.6; distillation 4.6 and 16.0, 9.4 and 16.2, 20.0 and 16.2).  Rows of up to 64 classes are
-// read by a lane in a few rounds: always.
+// best 7.3 and 14.1, 18.7 and 14.4, 31.2 and 14.6; distillation 4.6 and 16.0, 9.4 and 16.2, 20.0 and 16.2).  The rule does not look at the best:
+// with them a wave a row is behind already at 8000 rows.  Rows of up to 64 classes are read by a lane in a few rounds: always.
 inline bool lane_rows(const LogitsK &g, int num_cu) { return g.C <= 64 || g.rows >= 32ll * num_cu; }
 // Gradients by a wave a row, once every SIMD has four rows; longer ones are better left to four waves, 4-byte ones sooner (8192 x 8192: bf16 53
 // us by one wave and 56 by four, fp32 115 and 101; 50000 x 1999 with a teacher: bf16 105 and 194, fp32 178 and 212)

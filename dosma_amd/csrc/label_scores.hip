@@ -552,7 +552,8 @@ __global__ __launch_bounds__(64 * W, TOP ? 6 : sizeof(T) == 4 ? 6 : 8) void scor
 }
 
 // The segments' parts of a row together: a block a row, its waves a quarter of the segments each.  One row of 131071 scores in bf16
-// with the 20 best: 7.4 us for its 32 segments and 7.3 us here, both of them latency.
+// with the 20 best: 8 us for its 32 segments and 8 us here, both of them latency (here: the bitwise searches over 640 pairs that are in order
+// already).
 template <typename T>
 __global__ __launch_bounds__(256) void scores_join_kernel(const ScoresK k, const Cut cut) {
     __shared__ RowStat s_stat[4];
@@ -1020,7 +1021,7 @@ void planes(const ScoresK &k, int num_cu, hipStream_t st) {
         const bool key = k.g.C + k.g.bg + 15 <= (1 << kLabelBits<T>);
         if constexpr (K <= 4) {
             // 16 classes in flight where 2-byte rows are long enough (117 classes in f16: 64 us instead of 73, with the best 75 and 82; 20
-            // classes 22 and 19; 4-byte scores are no faster with it)
+            // classes 22 and 19; nothing between is measured; 4-byte scores are no faster with it)
             if (key && k.g.C > 48) {
                 hipLaunchKernelGGL((scores_planes_kernel<T, K, true, 16>), grid, block, lds, st, k);
                 return;
