@@ -387,8 +387,9 @@ int qmri_region_stats_device(const qmri_region_stats_args *args, void *hip_strea
 
 /* ------------------------------------------------------------------------------------------------------------------
  * ---- What a network's answers say: log probabilities, entropy, alternatives, distillation ---------------------------
- * The reference keeps `model.predict(...) > 0.5` and nothing else of a network's answer (dosma/models/oaiunet2d.py:305-316).  The entries below read the category scores themselves -- of qmri_unet2d_forward, or of any other
- * network -- as one softmax per row (voxel, token, ...):
+ * The reference keeps `model.predict(...) > 0.5` and nothing else of a network's answer (dosma/models/oaiunet2d.py:305-316).
+ * The entries below read the category scores themselves -- of qmri_unet2d_forward, or of any other network -- as one softmax per
+ * row (voxel, token, ...):
  *     p_j = exp((z_j - M) / T) / s,   M = max z,   s = sum_j exp((z_j - M) / T)
  * `background` adds an implicit category 0 of score 0 in front of the C classes (category = class + 1).  For the networks of
  * this library, whose classes have sigmoid heads, that is the distribution of the label under the condition that a voxel
