@@ -15,11 +15,11 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libqmri_hip.so")
 SOURCES = ["qmri_capi.hip", "monoexp_lm.hip", "linfit.hip", "lm_generic.hip", "unet_kernels.hip", "unet_rw.hip", "unet_s3.hip", "unet_c4.hip", "unet_d4.hip", "unet_enc0.hip", "unet_engine.hip", "dess.hip", "region_stats.hip",
-           "label_scores.hip", "distill.hip", "answers_capi.hip"]
+           "label_scores.hip", "distill.hip", "answers_planes.hip", "answers_capi.hip"]
 ARCH = "gfx950"
 # packed fp32 instructions are kept out of these sources: their sums must not depend on the form the compiler picks
 _NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-EXTRA_FLAGS = {"label_scores.hip": _NO_PACKED, "distill.hip": _NO_PACKED}
+EXTRA_FLAGS = {"label_scores.hip": _NO_PACKED, "distill.hip": _NO_PACKED, "answers_planes.hip": _NO_PACKED}
 
 
 def _hipcc():

@@ -459,6 +459,9 @@ hipError_t label_scores_grad_launch(const ScoresK &k, int dtype, int num_cu, hip
 hipError_t distill_launch(const DistillK &k, int dtype, int num_cu, hipStream_t st);
 size_t distill_workspace_bytes(const DistillK &k, int dtype, int num_cu);
 hipError_t distill_grad_launch(const DistillK &k, int dtype, int num_cu, hipStream_t st);
+// (S, P, K) rows of float32 or int32 labels -> (K, P, S) planes of float32 or uint8, and back (answers_planes.hip)
+hipError_t rows_to_planes_launch(const void *x, int is_label, long long P, int S, int K, void *y, hipStream_t stream);
+hipError_t planes_to_rows_launch(const void *x, int kind, long long P, int S, int K, void *y, hipStream_t stream);
 
 }  // namespace qmri
 #endif

@@ -299,8 +299,6 @@ hipError_t cast_launch(const void *x, long long n, void *y, int to_bf16, hipStre
 hipError_t transpose_ps_launch(const float *x, long long P, int S, float *y, hipStream_t stream);
 hipError_t mask_planes_launch(const unsigned char *mask_sp4, long long P, int S, int C, unsigned char *out,
                               hipStream_t stream);
-hipError_t rows_to_planes_launch(const void *x, int is_label, long long P, int S, int K, void *y, hipStream_t stream);
-hipError_t planes_to_rows_launch(const void *x, int kind, long long P, int S, int K, void *y, hipStream_t stream);
 hipError_t absmax_launch(const float *x, long long n, unsigned int *out, hipStream_t stream);
 hipError_t scale_copy_launch(const float *x, long long n, float f, float *y, hipStream_t stream);
 int whiten_stats_doubles();  // size of whiten_launch's `stats` buffer: [sum, sum of squares, mean, -] + the per-block partial sums
